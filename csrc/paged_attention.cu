@@ -1,0 +1,832 @@
+// Attention of new tokens over a paged cache, in 16 bits or as e4m3 codes with a scale for each (page, head) (csrc/paged_append.cu writes it).
+//
+// Sequence b has lengths[b] tokens in pages table[b, ..], the last n of which are the call's rows (n = 1 without starts); row i sees the positions up to its
+// own, the last `window` of them where one is given.  The R = H / G query heads of a K/V head share its keys: a row of the products is a (token, head) pair.
+//
+//   s = scale q.k,   m = max s,   l = sum 2^(s - m),   out = sum 2^(s - m) v / l          (s in units of log2 e)
+//
+// Bound: the keys and values are read once, 2 D bytes a (key, head) in e4m3, for 4 R D operations; up to some hundred operations a byte the memory bounds it.
+//
+// One producer warp copies tiles of 64 keys and values by TMA into a ring of stages (page by page, 128-byte swizzle), four consumer warps multiply with
+// mma.sync m16n8k16: either every warp takes 16 keys of the tile for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
+// memory), or 16 of 64 rows for all keys (ROWS 64: several new tokens).
+//
+// Every operand comes from shared memory in 16-byte pieces: the order of the channels within a product's sum is free as long as the queries follow it, and so is
+// the order of the keys as long as the values follow it.  A lane (g, t) reads bytes 16 t .. 16 t + 15 (and every 64 on) of key row pi(g), pi(n) = n for even n
+// and n ^ 4 for odd n, and channels 16 g .. 16 g + 15 of the four value rows that its probabilities belong to; with the swizzle neither conflicts.
+//
+// e4m3 to f16 takes three operations for two numbers: the code's seven low bits at bit 7 of a half are the number times 2^-8, subnormals too, and no code gives
+// an infinity or NaN, so that keys past a sequence's end need no care beside their zero probabilities.  Queries in bf16 are scaled by a power of two for each row
+// into f16's range.  With M = max (s + log2 v_scale) beside m, the probabilities times the page's value scale stay within f16 whatever the scales: 2^(s + log2
+// v_scale - M), and the result is taken times 2^(M - m) / l.
+//
+// Work is cut into equal shares of tiles, one for each resident CTA, whatever the lengths: a share may begin and end inside a (sequence, head).  Such pieces go to
+// a workspace of the call, and a second launch joins them in the order of the keys.
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace tyr {
+
+constexpr int kKeys = 64;                      // keys of a tile
+constexpr int kWarps = 4;                      // consumer warps
+
+struct PagedAttnArgs {
+  const void* q;                               // [rows, H, D]; element strides below
+  void* out;                                   // [rows, H, D]
+  const void *k_pages, *v_pages;               // [pages, G, P, D]
+  const float *k_scale, *v_scale;              // [pages, G] (null: 16-bit pages)
+  const int *table, *lengths, *starts;         // [B, width], [B], [B + 1] (nullable)
+  float* part;                                 // workspace (see part_floats)
+  int* err;
+  long long q_row, q_head, table_row;
+  int rows, B, H, G, D, P, pages, width, window, whole;
+  float scale;
+};
+static_assert(sizeof(PagedAttnArgs) == 160, "as ops/paged_cache.py packs it");
+
+struct PartHead { int row, heads, used, last, slot, pad[3]; };      // a (sequence, head, row tile) that begins in this CTA's share and ends in CTA `last`'s
+
+struct Seq { int row, n, len, tile0, tiles, row_tiles; };
+
+// Rows, keys and tiles of sequence b; none where the operands do not go together (recorded).
+template <int ROWS>
+__device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
+  Seq s;
+  s.len = a.lengths[b];
+  s.row = a.starts ? a.starts[b] : b;
+  s.n = a.starts ? a.starts[b + 1] - s.row : (s.len > 0 ? 1 : 0);
+  if (s.n != 0 && (s.n < 0 || s.row < 0 || s.row + s.n > a.rows || s.len < s.n || (s.len - 1) / a.P >= a.width)) {
+    report_error(a.err, ERR_BOUNDS, b);
+    s.n = 0;
+  }
+  const int first = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
+  s.tile0 = first / kKeys;
+  s.tiles = s.n == 0 ? 0 : (s.len + kKeys - 1) / kKeys - s.tile0;
+  s.row_tiles = s.n == 0 ? 0 : (s.n * (a.H / a.G) + ROWS - 1) / ROWS;
+  return s;
+}
+__device__ __forceinline__ int seq_work(const PagedAttnArgs& a, const Seq& s) { return a.G * s.row_tiles * (a.whole ? 1 : s.tiles); }
+
+__device__ __forceinline__ long long warp_sum64(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// This CTA's share of the work, walked piece by piece: a piece is a run of tiles of one (sequence, head, row tile).  Every warp walks it for itself.
+template <int ROWS>
+struct Share {
+  const PagedAttnArgs& a;
+  long long at, end, before, per;              // in tiles (items where shares are whole items); `before`: work of the sequences before b
+  int b, lane;
+  Seq s;
+  int head, row_tile, x0, x1, first, last;     // the piece: tiles first .. last - 1 that its rows see, x0 .. x1 of the item's
+  bool begins, ends;
+  long long item_end;
+
+  __device__ __forceinline__ Share(const PagedAttnArgs& args, int lane_) : a(args), lane(lane_) {
+    long long sum = 0;
+    for (int i = lane; i < a.B; i += 32) sum += seq_work(a, seq_of<ROWS>(a, i));
+    const long long total = warp_sum64(sum);
+    per = (total + gridDim.x - 1) / gridDim.x;
+    at = min(static_cast<long long>(blockIdx.x) * per, total);
+    end = min(at + per, total);
+    before = 0;
+    b = 0;
+    if (at >= end) return;
+    for (int base = 0; base < a.B; base += 32) {
+      const long long mine = base + lane < a.B ? seq_work(a, seq_of<ROWS>(a, base + lane)) : 0;
+      long long upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + upto > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = base + l;
+        before += __shfl_sync(0xffffffffu, upto - mine, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    s = seq_of<ROWS>(a, b);
+  }
+  __device__ __forceinline__ bool next() {
+    if (at >= end) return false;
+    while (at - before >= seq_work(a, s)) {
+      before += seq_work(a, s);
+      if (++b >= a.B) return false;
+      s = seq_of<ROWS>(a, b);
+    }
+    const int off = static_cast<int>(at - before), unit = a.whole ? 1 : s.tiles, item = off / unit;
+    head = item / s.row_tiles;
+    row_tile = item - head * s.row_tiles;
+    x0 = off - item * unit;
+    const long long left = end - at;
+    x1 = left < unit - x0 ? x0 + static_cast<int>(left) : unit;
+    item_end = at - x0 + unit;
+    begins = x0 == 0;
+    ends = x1 == unit;
+    at += x1 - x0;
+    // tiles that the piece's rows see
+    const int R = a.H / a.G, held = s.len - s.n, i0 = row_tile * ROWS / R, i1 = min(s.n, (row_tile * ROWS + ROWS - 1) / R + 1) - 1;
+    const int lo = a.window > 0 ? max(0, held + i0 - a.window + 1) : 0;
+    first = lo / kKeys;
+    last = (held + i1) / kKeys + 1;
+    if (!a.whole) {
+      first = max(first, s.tile0 + x0);
+      last = min(last, s.tile0 + x1);
+    }
+    return true;
+  }
+};
+
+template <bool F8, int D>
+struct Tile {
+  static constexpr int kBytes = F8 ? 1 : 2;
+  static constexpr int kRow = D * kBytes < 128 ? D * kBytes : 128;          // bytes of a row in a box
+  static constexpr int kBoxes = D * kBytes / kRow;
+  static constexpr int kSize = kKeys * D * kBytes;                          // of the keys, and of the values
+  static constexpr int kChunks = D * kBytes / 16;
+  static constexpr int kRun = F8 && D >= 128 ? 16 : 8;                      // channels of a box that a lane takes of a value row
+  static constexpr int kStages = kSize <= 4096 ? 6 : (kSize <= 8192 ? 4 : (kSize <= 16384 ? 3 : 2));
+  // 16-byte piece c of row r
+  static __device__ __forceinline__ uint32_t at(uint32_t base, int r, int c) {
+    constexpr int per = kRow / 16;
+    const int swizzle = kRow == 128 ? r & 7 : (r >> 1) & 3;
+    return base + (c / per) * (kKeys * kRow) + r * kRow + (((c % per) ^ swizzle) << 4);
+  }
+};
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t pt_prmt(uint32_t x, uint32_t y, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(sel));
+  return r;
+}
+// codes in bytes 1 and 3 -> two halves, times 2^-8; bytes 0 and 2 do not matter
+__device__ __forceinline__ uint32_t halves_of_codes(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
+
+template <typename T> struct Num;
+template <> struct Num<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 two(uint32_t u) { return unpack_bf16x2(u); }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { return pack_bf16x2(x, y); }
+};
+template <> struct Num<__half> {
+  static __device__ __forceinline__ float2 two(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+// c (rows g and, with NR 2, g + 8) += a b; M is the operands' type.
+template <typename M, int NR>
+__device__ __forceinline__ void mma(float (&c)[2 * NR], const uint32_t (&x)[2 * NR], uint32_t b0, uint32_t b1) {
+  float z0 = 0.f, z1 = 0.f;
+  float &c2 = NR == 2 ? c[2 * NR - 2] : z0, &c3 = NR == 2 ? c[2 * NR - 1] : z1;
+  const uint32_t a0 = x[0], a2 = x[NR], a1 = NR == 2 ? x[1] : 0u, a3 = NR == 2 ? x[2 * NR - 1] : 0u;
+  if constexpr (sizeof(M) == 2 && __is_same(M, __half)) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c2), "+f"(c3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c2), "+f"(c3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ float pt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Floats of the workspace for `ctas` shares: heads of split items, then two pieces a share of ROWS rows: {m, l, M, -} and D sums each.
+__host__ __device__ inline long long part_floats(int ctas, int rows, int D) { return static_cast<long long>(ctas) * (8 + 2LL * rows * (4 + D)); }
+__device__ __forceinline__ float* part_stats(const PagedAttnArgs& a, int ctas, int rows, int piece) { return a.part + ctas * 8LL + static_cast<long long>(piece) * rows * 4; }
+__device__ __forceinline__ float* part_sums(const PagedAttnArgs& a, int ctas, int rows, int piece) {
+  return a.part + ctas * 8LL + 2LL * ctas * rows * 4 + static_cast<long long>(piece) * rows * a.D;
+}
+
+template <typename T>
+__device__ __forceinline__ void write4(T* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(Num<T>::pack(v.x, v.y), Num<T>::pack(v.z, v.w));
+}
+
+// T: type of the queries, the results and 16-bit pages; NR: rows of a lane (1: at most 8 rows in a tile of 16).
+template <typename T, bool F8, int D, int ROWS, int NR>
+__global__ void __launch_bounds__((kWarps + 1) * 32) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
+                                                                           const __grid_constant__ CUtensorMap map_v) {
+  using TL = Tile<F8, D>;
+  using M = typename std::conditional<F8, __half, T>::type;                 // operands of the products
+  constexpr int STAGES = TL::kStages, KSTEPS = D / 16, NTILES = D / 8;
+  constexpr int GROUPS = ROWS == 16 ? 1 : kKeys / 16;                       // runs of 16 keys a warp takes of a tile
+  constexpr bool QREG = D <= 128;                                           // the queries' fragments stay in registers
+  constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end; in e4m3 pages it meets the codes' 2^-8
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* extra = smem + STAGES * 2 * TL::kSize;
+  float2* s_scale = reinterpret_cast<float2*>(extra);                       // [STAGES][4]: scale of the keys, log2 of the values'
+  uint64_t* full = reinterpret_cast<uint64_t*>(extra + STAGES * 32);
+  uint64_t* empty = full + STAGES;
+  float* s_stats = reinterpret_cast<float*>(empty + STAGES);                // [4][16][4], joining warps (ROWS 16)
+  uint4* s_q = reinterpret_cast<uint4*>(s_stats + 256);                     // fragments of the queries, QREG false: [warps that differ][KSTEPS][32]
+  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][D] (ROWS 16)
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kWarps);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncthreads();
+  pdl_wait();
+  const int R = a.H / a.G;
+  Share<ROWS> sh(a, lane);
+  int stage = 0;
+  uint32_t phase = 0;
+
+  if (warp == kWarps) {
+    // ---- producer ---------------------------------------------------------------------------------------------------
+    const int page_rows = min(a.P, kKeys), per_tile = kKeys / page_rows;
+    while (sh.next()) {
+      const int last_page = (sh.s.len - 1) / a.P;
+      const int* table = a.table + sh.b * a.table_row;
+      int batch = -1, id = 0;                       // pages 32 batch .. of the sequence, one a lane
+      float2 scale = make_float2(1.f, 0.f);
+      for (int tile = sh.first; tile < sh.last; ++tile) {
+        const int p0 = tile * kKeys / a.P;
+        if (p0 >> 5 != batch) {
+          batch = p0 >> 5;
+          const int p = batch * 32 + lane;
+          id = p <= last_page ? table[p] : 0;
+          if (id < 0 || id >= a.pages) {
+            report_error(a.err, ERR_BOUNDS, id);
+            id = 0;
+          }
+          if (F8) scale = make_float2(a.k_scale[static_cast<long long>(id) * a.G + sh.head], log2f(a.v_scale[static_cast<long long>(id) * a.G + sh.head]));
+        }
+        const int n = min(per_tile, last_page - p0 + 1), from = (p0 & 31) + lane;
+        const int page = __shfl_sync(0xffffffffu, id, from & 31);
+        const float2 sc = make_float2(__shfl_sync(0xffffffffu, scale.x, from & 31), __shfl_sync(0xffffffffu, scale.y, from & 31));
+        if (!mbar_wait(empty + stage, phase ^ 1, a.err, 1)) return;
+        if (F8 && lane < per_tile) s_scale[stage * 4 + lane] = sc;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(full + stage, static_cast<uint32_t>(2 * n * page_rows * D * TL::kBytes));
+        __syncwarp();
+        if (lane < n) {
+          uint8_t* dst = smem + stage * 2 * TL::kSize + lane * page_rows * TL::kRow;
+          const int row = (tile * kKeys) % a.P, z = page * a.G + sh.head;
+#pragma unroll
+          for (int c = 0; c < TL::kBoxes; ++c) {
+            tma_load_3d(dst + c * kKeys * TL::kRow, &map_k, full + stage, c * (TL::kRow / TL::kBytes), row, z);
+            tma_load_3d(dst + TL::kSize + c * kKeys * TL::kRow, &map_v, full + stage, c * (TL::kRow / TL::kBytes), row, z);
+          }
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- consumers ------------------------------------------------------------------------------------------------------
+  const int g = lane >> 2, t = lane & 3, pi = g & 1 ? g ^ 4 : g;
+  const int tid = threadIdx.x;
+  // rows of no sequence
+  for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps) {
+    const bool none = a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0;
+    if (none)
+      for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * D + i) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  PartHead head{0, 0, 0, -1, 0, {0, 0, 0}};
+  if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
+  bool first_piece = true;
+  while (sh.next()) {
+    const int held = sh.s.len - sh.s.n, used = min(ROWS, sh.s.n * R - sh.row_tile * ROWS);         // rows of this tile
+    const int warp_row = ROWS == 16 ? 0 : warp * 16;
+    // ---- queries: this lane's rows, their places and their fragments -------------------------------------------------
+    uint32_t qa[QREG ? KSTEPS : 1][2 * NR];
+    float factor[NR];
+    int pos[NR];
+    if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");                // the last piece's fragments are no longer read
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int in_tile = warp_row + g + 8 * r, row = sh.row_tile * ROWS + in_tile, i = row / R;
+      const bool there = in_tile < used;
+      pos[r] = there ? held + i : -1;
+      const T* src = static_cast<const T*>(a.q) + (there ? (sh.s.row + i) * a.q_row + (sh.head * R + row % R) * a.q_head : 0);
+      constexpr int PIECES = TL::kChunks / 4;                                // 16-byte pieces of a key row that a lane takes
+      constexpr int PER = F8 ? 16 : 8;                                       // channels of one
+      uint32_t raw[PIECES][PER / 2];
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+        for (int e = 0; e < PER / 8; ++e) {
+          const uint4 u = there ? *reinterpret_cast<const uint4*>(src + PER * (t + 4 * c) + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+          raw[c][4 * e] = u.x; raw[c][4 * e + 1] = u.y; raw[c][4 * e + 2] = u.z; raw[c][4 * e + 3] = u.w;
+        }
+      factor[r] = a.scale * 1.4426950408889634f;
+      if constexpr (F8) {
+        float up = 1.f;
+        if constexpr (!__is_same(T, __half)) {                               // bf16 to f16: the row's largest magnitude to 1 .. 2
+          float top = 0.f;
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+            for (int e = 0; e < PER / 2; ++e) {
+              const float2 v = Num<T>::two(raw[c][e]);
+              top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+          up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          factor[r] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        }
+        factor[r] *= 256.f;                                                  // of the keys' codes
+        const uint32_t* flat = &raw[0][0];
+        // channels {0, 2} and {1, 3} of every four, as the codes' even and odd bytes come out
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+          uint32_t x = flat[2 * ks], y = flat[2 * ks + 1];
+          if constexpr (!__is_same(T, __half)) {
+            const float2 u = Num<T>::two(x), v = Num<T>::two(y);
+            x = Num<__half>::pack(u.x * up, u.y * up);
+            y = Num<__half>::pack(v.x * up, v.y * up);
+          }
+          const uint32_t even = pt_prmt(x, y, 0x5410), odd = pt_prmt(x, y, 0x7632);
+          if constexpr (QREG) {
+            qa[ks][r] = even;
+            qa[ks][NR + r] = odd;
+          } else if (ROWS != 16 || warp == 0) {
+            uint32_t* dst = reinterpret_cast<uint32_t*>(s_q + ((ROWS == 16 ? 0 : warp) * KSTEPS + ks) * 32 + lane);
+            dst[r] = even;
+            dst[NR + r] = odd;
+          }
+        }
+      } else {
+        const uint32_t* flat = &raw[0][0];
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+          if constexpr (QREG) {
+            qa[ks][r] = flat[2 * ks];
+            qa[ks][NR + r] = flat[2 * ks + 1];
+          } else if (ROWS != 16 || warp == 0) {
+            uint32_t* dst = reinterpret_cast<uint32_t*>(s_q + ((ROWS == 16 ? 0 : warp) * KSTEPS + ks) * 32 + lane);
+            dst[r] = flat[2 * ks];
+            dst[NR + r] = flat[2 * ks + 1];
+          }
+        }
+      }
+    }
+    if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");
+    // every key of tiles from `clear0` to before `clear1` is seen by all rows of the piece
+    const int p_first = held + sh.row_tile * ROWS / R, p_last = held + (sh.row_tile * ROWS + used - 1) / R;
+    const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + kKeys - 1) / kKeys : 0, clear1 = (p_first + 1) / kKeys;
+
+    float m[NR], l[NR], top[NR], o[NTILES][2 * NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) m[r] = top[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NTILES; ++i)
+#pragma unroll
+      for (int e = 0; e < 2 * NR; ++e) o[i][e] = 0.f;
+
+    for (int tile = sh.first; tile < sh.last; ++tile) {
+      if (!mbar_wait(full + stage, phase, a.err, 2)) return;
+      const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
+      const int group0 = ROWS == 16 ? warp : 0;
+      // ---- scores ------------------------------------------------------------------------------------------------------
+      float s[GROUPS][2][2 * NR];
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2 * NR; ++e) s[j][h][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < TL::kChunks / 4; ++c) {
+        constexpr int STEPS = F8 ? 4 : 2;
+        uint32_t qs[STEPS][2 * NR];
+#pragma unroll
+        for (int w = 0; w < STEPS; ++w) {
+          if constexpr (QREG) {
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) qs[w][e] = qa[c * STEPS + w][e];
+          } else {
+            const uint32_t addr = smem_u32(s_q + ((ROWS == 16 ? 0 : warp) * KSTEPS + c * STEPS + w) * 32 + lane);
+            if constexpr (NR == 2) {
+              const uint4 u = lds128(addr);
+              qs[w][0] = u.x; qs[w][1] = u.y; qs[w][2] = u.z; qs[w][3] = u.w;
+            } else {
+              const uint2 u = lds64(addr);
+              qs[w][0] = u.x; qs[w][1] = u.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 u = lds128(TL::at(kb, 16 * (group0 + j) + 8 * h + pi, t + 4 * c));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            if constexpr (F8) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mma<M, NR>(s[j][h], qs[i], halves_of_codes(w[i] << 8), halves_of_codes(w[i]));
+            } else {
+              mma<M, NR>(s[j][h], qs[0], w[0], w[1]);
+              mma<M, NR>(s[j][h], qs[1], w[2], w[3]);
+            }
+          }
+      }
+      // ---- running maxima --------------------------------------------------------------------------------------------------
+      const int key0 = tile * kKeys;
+      const bool masked = tile < clear0 || tile >= clear1;
+      float mx[NR], mt[NR], lv[GROUPS];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) mx[r] = mt[r] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        float ks = 1.f;
+        lv[j] = 0.f;
+        if constexpr (F8) {
+          const int at = a.P >= kKeys ? 0 : 16 * (group0 + j) / a.P;
+          const float2 sc = s_scale[stage * 4 + at];
+          ks = sc.y == sc.y ? sc.x : sc.y;                                   // a page whose values hold no numbers shows at the keys that are seen
+          lv[j] = sc.y == sc.y ? sc.y : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float f = factor[r] * ks;
+          float top_j = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = s[j][h][2 * r + e] * f;
+              if (masked) {
+                const int key = key0 + 16 * (group0 + j) + 8 * h + (e == 0 ? 2 * t : (2 * t + 1) ^ 4);
+                if (key > pos[r] || (a.window > 0 && key <= pos[r] - a.window)) v = -INFINITY;
+              }
+              s[j][h][2 * r + e] = v;
+              top_j = fmaxf(top_j, v);
+            }
+          mx[r] = fmaxf(mx[r], top_j);
+          if (F8) mt[r] = fmaxf(mt[r], top_j + lv[j]);
+        }
+      }
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        if (F8) {
+          mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xffffffffu, mt[r], 1));
+          mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xffffffffu, mt[r], 2));
+        } else {
+          mt[r] = mx[r];
+        }
+        grew |= mx[r] > m[r] || mt[r] > top[r];
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float m_new = fmaxf(m[r], mx[r]), t_new = fmaxf(top[r], mt[r]);
+          l[r] *= m[r] == m_new ? 1.f : pt_exp2(m[r] - m_new);
+          const float f = top[r] == t_new ? 1.f : pt_exp2(top[r] - t_new);
+          m[r] = m_new;
+          top[r] = t_new;
+#pragma unroll
+          for (int i = 0; i < NTILES; ++i) {
+            o[i][2 * r] *= f;
+            o[i][2 * r + 1] *= f;
+          }
+        }
+      }
+      // ---- probabilities and their product with the values --------------------------------------------------------------------
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        uint32_t pa[2 * NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float ref = m[r] == -INFINITY ? 0.f : m[r];
+          // 16-bit pages: no scales, top == m
+          const float by = F8 ? (lv[j] == -INFINITY ? 0.f : pt_exp2(fminf(lv[j] + ref - top[r], 100.f) + kShift)) : (__is_same(M, __half) ? 256.f : 1.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p0 = pt_exp2(s[j][h][2 * r] - ref), p1 = pt_exp2(s[j][h][2 * r + 1] - ref);
+            l[r] += p0 + p1;
+            pa[h * NR + r] = Num<M>::pack(p0 * by, p1 * by);
+          }
+        }
+        const int row = 16 * (group0 + j) + 2 * t, row1 = 16 * (group0 + j) + ((2 * t + 1) ^ 4);
+        const int left = F8 || !masked ? 16 : sh.s.len - (key0 + 16 * (group0 + j));      // 16-bit pages: what lies past the end may be no number
+        if constexpr (F8 && D == 64) {
+          const uint32_t at = (g & 1) * 8;
+          const uint2 x = lds64(TL::at(vb, row, g >> 1) + at), y = lds64(TL::at(vb, row1, g >> 1) + at);
+          const uint2 z = lds64(TL::at(vb, row + 8, g >> 1) + at), u = lds64(TL::at(vb, row1 + 8, g >> 1) + at);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int e = i & 3;
+            const uint32_t sel = (4 + e) << 12 | e << 4;
+            mma<M, NR>(o[i], pa, halves_of_codes(pt_prmt(i < 4 ? x.x : x.y, i < 4 ? y.x : y.y, sel)), halves_of_codes(pt_prmt(i < 4 ? z.x : z.y, i < 4 ? u.x : u.y, sel)));
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < TL::kBoxes; ++c) {
+            const uint4 xs = lds128(TL::at(vb, row, 8 * c + g)), ys = lds128(TL::at(vb, row1, 8 * c + g));
+            const uint4 zs = lds128(TL::at(vb, row + 8, 8 * c + g)), us = lds128(TL::at(vb, row1 + 8, 8 * c + g));
+            uint32_t x[4] = {xs.x, xs.y, xs.z, xs.w}, y[4] = {ys.x, ys.y, ys.z, ys.w}, z[4] = {zs.x, zs.y, zs.z, zs.w}, u[4] = {us.x, us.y, us.z, us.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if constexpr (F8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t sel = (4 + e) << 12 | e << 4;
+                  mma<M, NR>(o[c * 16 + 4 * w + e], pa, halves_of_codes(pt_prmt(x[w], y[w], sel)), halves_of_codes(pt_prmt(z[w], u[w], sel)));
+                }
+              } else {
+                if (left < 16) {
+                  if (2 * t >= left) x[w] = 0u;
+                  if (((2 * t + 1) ^ 4) >= left) y[w] = 0u;
+                  if (2 * t + 8 >= left) z[w] = 0u;
+                  if (((2 * t + 1) ^ 4) + 8 >= left) u[w] = 0u;
+                }
+                mma<M, NR>(o[c * 8 + 2 * w], pa, pt_prmt(x[w], y[w], 0x5410), pt_prmt(z[w], u[w], 0x5410));
+                mma<M, NR>(o[c * 8 + 2 * w + 1], pa, pt_prmt(x[w], y[w], 0x7632), pt_prmt(z[w], u[w], 0x7632));
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + stage);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    // ---- the piece's result: in units of 2^top where the keys have scales, l over the lanes of a row ----------------------------------
+    constexpr float kUndo = !F8 && __is_same(M, __half) ? 1.f / 256.f : 1.f;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (!F8) top[r] = m[r];
+    }
+    const bool done = sh.begins && sh.ends;
+    const int slot = first_piece ? 0 : 1, piece = 2 * blockIdx.x + slot;
+    const long long first_row = sh.s.row;
+    // channels c * 8 kRun + 2 t kRun + (0 .. 2 kRun - 1) of rows g and g + 8: o[c kRun + i][e] is the one at e kRun + i
+    if constexpr (ROWS == 16) {
+      asm volatile("bar.sync 1, 128;" ::: "memory");                        // the last piece's sums are no longer read
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (t == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + g + 8 * r) * 4) = make_float4(m[r], l[r], top[r], 0.f);
+        float* dst = s_sum + (warp * 8 * NR + g + 8 * r) * D;
+#pragma unroll
+        for (int c = 0; c < NTILES / TL::kRun; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < TL::kRun; i += 4)
+              *reinterpret_cast<float4*>(dst + c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i) =
+                  make_float4(o[c * TL::kRun + i][2 * r + e], o[c * TL::kRun + i + 1][2 * r + e], o[c * TL::kRun + i + 2][2 * r + e], o[c * TL::kRun + i + 3][2 * r + e]);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = tid * 4; i < used * D; i += kWarps * 32 * 4) {
+        const int r = i / D, d = i % D;
+        float mm = -INFINITY, tt = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
+          mm = fmaxf(mm, st.x);
+          tt = fmaxf(tt, st.z);
+        }
+        float ll = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
+          if (st.x != -INFINITY) ll += st.y * pt_exp2(st.x - mm);
+          if (st.z != -INFINITY) {
+            const float f = pt_exp2(st.z - tt);
+            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * D + d);
+            v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+          }
+        }
+        if (done) {
+          const int row = sh.row_tile * ROWS + r;
+          const float f = ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(tt - mm) : 1.f) / ll : 0.f;
+          write4(static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        } else {
+          *reinterpret_cast<float4*>(part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(r) * D + d) = make_float4(v.x * kUndo, v.y * kUndo, v.z * kUndo, v.w * kUndo);
+          if (d == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + r * 4) = make_float4(mm, ll, tt, 0.f);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int in_tile = warp_row + g + 8 * r, row = sh.row_tile * ROWS + in_tile;
+        if (in_tile >= used) continue;
+        const float f = !done ? kUndo : l[r] > 0.f || l[r] != l[r] ? kUndo * (F8 ? pt_exp2(top[r] - m[r]) : 1.f) / l[r] : 0.f;
+        T* dst = static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D;
+        float* sums = part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(in_tile) * D;
+#pragma unroll
+        for (int c = 0; c < NTILES / TL::kRun; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < TL::kRun; i += 4) {
+              const int d = c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i;
+              const float4 v = make_float4(o[c * TL::kRun + i][2 * r + e] * f, o[c * TL::kRun + i + 1][2 * r + e] * f, o[c * TL::kRun + i + 2][2 * r + e] * f,
+                                           o[c * TL::kRun + i + 3][2 * r + e] * f);
+              if (done) write4(dst + d, v);
+              else *reinterpret_cast<float4*>(sums + d) = v;
+            }
+        if (!done && t == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + in_tile * 4) = make_float4(m[r], l[r], top[r], 0.f);
+      }
+    }
+    if (sh.begins && !sh.ends) head = {sh.s.row, sh.head, used, static_cast<int>((sh.item_end - 1) / sh.per), slot, {sh.row_tile, 0, 0}};
+    first_piece = false;
+  }
+  if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
+}
+
+// Joins the pieces of the item that begins in share blockIdx.x and goes on in the next ones; row by row over blockIdx.y, a lane for 4 channels, the pieces dealt
+// out to the groups of lanes and added up in their order.
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_constant__ PagedAttnArgs a, int ctas) {
+  pdl_entry();
+  __shared__ float4 s_v[128];
+  __shared__ float s_l[128];
+  const PartHead h = *reinterpret_cast<const PartHead*>(a.part + blockIdx.x * 8LL);
+  if (h.last < 0) return;
+  const int lanes = a.D / 4, d = threadIdx.x % lanes * 4, group = threadIdx.x / lanes, groups = 128 / lanes, R = a.H / a.G;
+  const int n = h.last - static_cast<int>(blockIdx.x) + 1;
+  auto piece_of = [&](int i) { return i == 0 ? 2 * static_cast<int>(blockIdx.x) + h.slot : 2 * (static_cast<int>(blockIdx.x) + i); };
+  for (int r = blockIdx.y; r < h.used; r += gridDim.y) {
+    float m = -INFINITY, top = -INFINITY;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+      const float4 st = *reinterpret_cast<const float4*>(part_stats(a, ctas, ROWS, piece_of(i)) + r * 4);
+      m = fmaxf(m, st.x);
+      top = fmaxf(top, st.z);
+    }
+    m = warp_max(m);
+    top = warp_max(top);
+    float l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = group; i < n; i += groups) {
+      const int piece = piece_of(i);
+      const float4 st = *reinterpret_cast<const float4*>(part_stats(a, ctas, ROWS, piece) + r * 4);
+      const float4 x = *reinterpret_cast<const float4*>(part_sums(a, ctas, ROWS, piece) + static_cast<long long>(r) * a.D + d);
+      if (st.x != -INFINITY) l += st.y * pt_exp2(st.x - m);
+      if (st.z != -INFINITY) {
+        const float f = pt_exp2(st.z - top);
+        v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+      }
+    }
+    s_v[threadIdx.x] = v;
+    s_l[threadIdx.x] = l;
+    __syncthreads();
+    if (group == 0) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 x = s_v[k * lanes + threadIdx.x];
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        l += s_l[k * lanes + threadIdx.x];
+      }
+      const int row = h.pad[0] * ROWS + r;
+      const float f = l > 0.f || l != l ? pt_exp2(top - m) / l : 0.f;
+      write4(static_cast<T*>(a.out) + ((h.row + static_cast<long long>(row / R)) * a.H + h.heads * R + row % R) * a.D + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    }
+    __syncthreads();
+  }
+}
+
+typedef CUresult (*PagedEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Pages as [pages * G, P, D]; boxes of 128 bytes (a whole row where it is shorter) of min(P, 64) tokens of one page and head.
+template <bool F8, int D>
+int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
+  static const PagedEncodeFn encode = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<PagedEncodeFn>(ptr) : nullptr;
+  }();
+  if (encode == nullptr) return -20;
+  using TL = Tile<F8, D>;
+  const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(a.P), static_cast<cuuint64_t>(a.pages) * a.G};
+  const cuuint64_t strides[2] = {D * TL::kBytes, static_cast<cuuint64_t>(a.P) * D * TL::kBytes};
+  const cuuint32_t box[3] = {TL::kRow / TL::kBytes, static_cast<cuuint32_t>(a.P < kKeys ? a.P : kKeys), 1}, step[3] = {1, 1, 1};
+  const CUresult r = encode(map, F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, TL::kRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 4000 + static_cast<int>(r);
+}
+
+template <typename T, bool F8, int D, int ROWS, int NR>
+struct PagedLaunch {
+  using TL = Tile<F8, D>;
+  static constexpr int kSmem = 1024 + TL::kStages * (2 * TL::kSize + 32 + 16) + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * D * 4 : 0);
+  // CTAs that the device holds at once
+  static int resident() {
+    static const int n = [] {
+      const auto kernel = paged_attention_kernel<T, F8, D, ROWS, NR>;
+      int per = 0, dev = 0, sms = 0;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return 0;
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, (kWarps + 1) * 32, kSmem) != cudaSuccess) return 0;
+      if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+      return per * sms;
+    }();
+    return n;
+  }
+  static int ctas(const PagedAttnArgs& a) {
+    const int R = a.H / a.G;
+    const long long row_tiles = a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS);
+    const long long tiles = a.whole ? 1 : (static_cast<long long>(a.width) * a.P + kKeys - 1) / kKeys;
+    const long long most = row_tiles * a.G * tiles, n = resident();
+    return static_cast<int>(most < n ? most : n);
+  }
+  static int run(const PagedAttnArgs& a, cudaStream_t stream) {
+    CUtensorMap mk, mv;
+    int r = page_map<F8, D>(&mk, a.k_pages, a);
+    if (r == 0) r = page_map<F8, D>(&mv, a.v_pages, a);
+    if (r != 0) return r;
+    const int n = ctas(a);
+    if (n <= 0) return -21;
+    cudaError_t e = launch_dependent(paged_attention_kernel<T, F8, D, ROWS, NR>, dim3(n), dim3((kWarps + 1) * 32), kSmem, stream, a, mk, mv);
+    if (e != cudaSuccess || a.whole) return static_cast<int>(e);
+    const int R = a.H / a.G, rows = a.starts ? 16 : (R < ROWS ? R : ROWS);
+    return static_cast<int>(launch_dependent(paged_attention_join_kernel<T, ROWS>, dim3(n, rows), dim3(128), 0, stream, a, n));
+  }
+};
+
+// Floats of workspace (`floats` given) or the launches.
+template <typename T, bool F8, int D>
+int paged_form(const PagedAttnArgs& a, int rows, cudaStream_t stream, long long* floats) {
+  const int R = a.H / a.G;
+  if (rows == 64) {
+    using L = PagedLaunch<T, F8, D, 64, 2>;
+    if (floats) return *floats = part_floats(L::ctas(a), 64, D), 0;
+    return L::run(a, stream);
+  }
+  if (a.starts == nullptr && R <= 8) {
+    using L = PagedLaunch<T, F8, D, 16, 1>;
+    if (floats) return *floats = part_floats(L::ctas(a), 16, D), 0;
+    return L::run(a, stream);
+  }
+  using L = PagedLaunch<T, F8, D, 16, 2>;
+  if (floats) return *floats = part_floats(L::ctas(a), 16, D), 0;
+  return L::run(a, stream);
+}
+template <typename T, bool F8>
+int paged_dim(const PagedAttnArgs& a, int rows, cudaStream_t stream, long long* floats) {
+  switch (a.D) {
+    case 64: return paged_form<T, F8, 64>(a, rows, stream, floats);
+    case 128: return paged_form<T, F8, 128>(a, rows, stream, floats);
+    case 256: return paged_form<T, F8, 256>(a, rows, stream, floats);
+  }
+  return -2;
+}
+
+}  // namespace tyr
+
+using namespace tyr;
+
+// dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows: 16 or 64 of a tile.  With `floats` only the workspace is asked for.
+extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int rows, void* stream, long long* floats) {
+  const PagedAttnArgs& a = *static_cast<const PagedAttnArgs*>(packed);
+  if (a.rows <= 0 || a.B <= 0 || a.H <= 0 || a.G <= 0 || a.H % a.G != 0 || a.pages <= 0 || a.width <= 0 || a.window < 0) return -1;
+  if (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) return -2;
+  if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64)) return -3;
+  // a sequence's work and the pages' rows are counted in 32 bits
+  const long long tiles = (static_cast<long long>(a.width) * a.P + kKeys - 1) / kKeys;
+  if ((static_cast<long long>(a.rows) * (a.H / a.G) / rows + 1) * a.G * tiles > 0x7fffffffLL || static_cast<long long>(a.pages) * a.G > 0x7fffffffLL) return -4;
+  if (static_cast<long long>(a.width) * a.P > 0x7fffffffLL || static_cast<long long>(a.rows) * a.H > 0x7fffffffLL) return -5;
+  const bool f8 = a.k_scale != nullptr;
+  if (dtype == 0) return f8 ? paged_dim<__nv_bfloat16, true>(a, rows, (cudaStream_t)stream, floats) : paged_dim<__nv_bfloat16, false>(a, rows, (cudaStream_t)stream, floats);
+  if (dtype == 1) return f8 ? paged_dim<__half, true>(a, rows, (cudaStream_t)stream, floats) : paged_dim<__half, false>(a, rows, (cudaStream_t)stream, floats);
+  return -6;
+}

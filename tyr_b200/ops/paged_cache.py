@@ -1,0 +1,301 @@
+"""A paged K/V cache for batches of ragged sequences: new tokens' keys and values written with their norms and rotation on the way (csrc/paged_append.cu), and
+attention over the pages (csrc/paged_attention.cu).
+
+Pages ``[pages, kv heads, page, head size]`` hold ``page`` tokens each, in 16 bits or as e4m3 codes in units of a scale for each (page, head).  Sequence ``b`` has
+``lengths[b]`` tokens, the new ones among them, at ``table[b, position // page]``; its new tokens are rows ``starts[b] .. starts[b + 1] - 1`` of the operands and its
+last positions.  Without ``starts`` every sequence has one row, and none where its length is 0.  Lengths, starts and table live on the device: a step has no shapes
+that depend on them and can be replayed from a CUDA graph.  A page that is written belongs to one sequence; full pages may be shared.
+
+On the GPU, operands that do not go together (a page outside the cache, a length beyond the table or the rotation) are left out and recorded
+(:func:`tyr_b200.ops._common.raise_on_device_error`).  The CPU path states the same contract in plain PyTorch, refuses them, and is the oracle of the numerics tests."""
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+from typing import List, Optional, Tuple
+
+import torch
+
+from .._native import register_signatures
+from ._common import check, cur_stream, err_word, lib, ptr
+
+E4M3 = torch.float8_e4m3fn
+LARGEST = 448.0                     # of e4m3
+LEAST_EXPONENT = -100               # of a page's scale
+HEAD_SIZES = (64, 128, 256)
+PAGE_SIZES = (16, 32, 64, 128)
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+# capacity up to which the keys of a (sequence, head) are not cut into pieces
+WHOLE_MAX_KEYS = 256
+
+
+@register_signatures
+def _sigs(lib_):
+    P, I = ctypes.c_void_p, ctypes.c_int
+    if hasattr(lib_, "tyr_paged_append"):
+        lib_.tyr_paged_append.argtypes, lib_.tyr_paged_append.restype = [P, I, P], I
+    if hasattr(lib_, "tyr_paged_attention"):
+        lib_.tyr_paged_attention.argtypes, lib_.tyr_paged_attention.restype = [P, I, I, P, ctypes.POINTER(ctypes.c_longlong)], I
+
+
+# the kernels' argument blocks, as csrc/paged_append.cu and csrc/paged_attention.cu declare them
+_APPEND = struct.Struct("@16Q7q11if0q")
+_ATTEND = struct.Struct("@11Q3q10if0q")
+
+
+class PagedStore:
+    """The pages of one layer: ``k`` and ``v`` [pages, kv heads, page, head size] in e4m3, bf16 or fp16, and the scales [pages, kv heads] of e4m3 pages."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.device != k.device or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("paged store: k and v are contiguous [pages, kv heads, page, head size] of one type and device")
+        if (dtype == E4M3) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
+            raise ValueError("paged store: e4m3 pages need k_scale and v_scale, other pages have none")
+        if k_scale is not None:
+            for s in (k_scale, v_scale):
+                if s.shape != shape[:2] or s.dtype != torch.float32 or not s.is_contiguous() or s.device != k.device:
+                    raise ValueError("paged store: scales are contiguous fp32 [pages, kv heads] beside the pages")
+        elif dtype not in (torch.bfloat16, torch.float16) and k.is_cuda or not dtype.is_floating_point:
+            raise ValueError(f"paged store: pages in {dtype} are not supported")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @staticmethod
+    def allocate(pages: int, kv_heads: int, page: int, head_dim: int, device, dtype: torch.dtype = E4M3) -> "PagedStore":
+        if min(pages, kv_heads, page, head_dim) <= 0:
+            raise ValueError("paged store: sizes must be positive")
+        k, v = (torch.zeros((pages, kv_heads, page, head_dim), dtype=dtype, device=device) for _ in range(2))
+        if dtype != E4M3:
+            return PagedStore(k, v)
+        return PagedStore(k, v, *(torch.full((pages, kv_heads), 2.0 ** LEAST_EXPONENT, dtype=torch.float32, device=device) for _ in range(2)))
+
+    @property
+    def page(self) -> int:
+        return self.k.shape[2]
+
+    def values(self, pages: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What these pages hold, fp32 [len(pages), kv heads, page, head size] of the keys and of the values."""
+        k, v = self.k[pages].float(), self.v[pages].float()
+        if self.k_scale is None:
+            return k, v
+        return k * self.k_scale[pages][..., None, None], v * self.v_scale[pages][..., None, None]
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+
+
+def _together(what: str, store: PagedStore, rows: int, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor]) -> None:
+    B = lengths.shape[0]
+    if lengths.dim() != 1 or B == 0 or lengths.dtype != torch.int32 or lengths.stride(0) != 1:
+        raise ValueError(f"{what}: lengths are contiguous int32 [sequences]")
+    if table.dim() != 2 or table.shape[0] != B or table.shape[1] == 0 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError(f"{what}: the table is int32 [sequences, pages] with contiguous rows")
+    if starts is None:
+        if rows != B:
+            raise ValueError(f"{what}: {rows} rows for {B} sequences need starts")
+    elif starts.dim() != 1 or starts.shape[0] != B + 1 or starts.dtype != torch.int32 or starts.stride(0) != 1:
+        raise ValueError(f"{what}: starts are contiguous int32 [sequences + 1]")
+    dev = store.k.device
+    if table.device != dev or lengths.device != dev or (starts is not None and starts.device != dev):
+        raise ValueError(f"{what}: store, table, lengths and starts lie on different devices")
+
+
+def _on_gpu(what: str, store: PagedStore, dtype: torch.dtype) -> int:
+    """The kernels' number of the operands' type; refuses what they do not serve."""
+    D, P, number = store.k.shape[3], store.k.shape[2], _DTYPES.get(dtype)
+    if number is None or (store.k_scale is None and store.k.dtype != dtype):
+        raise ValueError(f"{what}: operands in {dtype} over pages in {store.k.dtype} are not supported")
+    if D not in HEAD_SIZES or P not in PAGE_SIZES:
+        raise ValueError(f"{what}: heads of {D} in pages of {P} are not supported (heads of {HEAD_SIZES}, pages of {PAGE_SIZES})")
+    if (store.k.data_ptr() | store.v.data_ptr()) & 15:
+        raise ValueError(f"{what}: pages must lie at multiples of 16 bytes")
+    return number
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, heads, D] as the kernels read it: whole heads, 16-byte aligned."""
+    return t if t.stride(2) == 1 and (t.stride(0) | t.stride(1)) & 7 == 0 and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _spans(what: str, store: PagedStore, rows: int, table, lengths, starts) -> List[Tuple[int, int, int, List[int]]]:
+    """CPU: (first row, rows, length, pages) of every sequence, refusing what does not go together."""
+    lens = lengths.tolist()
+    at = list(range(rows + 1)) if starts is None else starts.tolist()
+    out, P = [], store.page
+    for b, n in enumerate(lens):
+        new = at[b + 1] - at[b] if starts is not None else int(n > 0)
+        if new < 0 or at[b] < 0 or at[b] + new > rows or n < new:
+            raise ValueError(f"{what}: sequence {b} has rows {at[b]} to {at[b + 1]} of {rows} and {n} tokens")
+        need = -(-n // P) if new else 0
+        if need > table.shape[1]:
+            raise ValueError(f"{what}: sequence {b} has {n} tokens and {table.shape[1]} pages of {P}")
+        pages = table[b, :need].tolist()
+        if any(not 0 <= p < store.k.shape[0] for p in pages):
+            raise ValueError(f"{what}: sequence {b} names a page outside the {store.k.shape[0]} of the cache")
+        out.append((at[b], new, n, pages))
+    return out
+
+
+def _turned(x: torch.Tensor, weight, cos, sin, eps: float, one_plus_w: bool) -> torch.Tensor:
+    """Norm, then rotation of channels (i, i + half), rounded nowhere; x: [rows, heads, D], cos / sin: [rows, half]."""
+    x = x if x.dtype == torch.float64 else x.float()
+    if weight is not None:
+        w = weight.to(x.dtype) + (1.0 if one_plus_w else 0.0)
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w
+    if cos is None:
+        return x
+    half, c, s = cos.shape[-1], cos.to(x.dtype)[:, None], sin.to(x.dtype)[:, None]
+    a, b = x[..., :half], x[..., half:2 * half]
+    return torch.cat([a * c - b * s, a * s + b * c, x[..., 2 * half:]], -1)
+
+
+def page_scale(amax: torch.Tensor) -> torch.Tensor:
+    """2^e with the smallest e >= LEAST_EXPONENT that keeps magnitudes up to ``amax`` within e4m3; NaN where one is not finite."""
+    m, x = torch.frexp(amax.float())
+    e = torch.where(amax > 0, x - 9 + (m > 0.875).int(), LEAST_EXPONENT).clamp_min(LEAST_EXPONENT)
+    return torch.where(torch.isfinite(amax), torch.ldexp(torch.ones_like(m), e), math.nan)
+
+
+def _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w):
+    rows, P = k.shape[0], store.page
+    spans = _spans("paged_append", store, rows, table, lengths, starts)
+    if cos is not None and any(new and n > cos.shape[0] for _, new, n, _ in spans):
+        raise ValueError(f"paged_append: a position lies outside the {cos.shape[0]} of the rotation")
+    out = None if q is None else torch.zeros_like(q, memory_format=torch.contiguous_format)
+    for row, new, n, pages in spans:
+        c, s = (None, None) if cos is None else (cos[n - new:n], sin[n - new:n])
+        if q is not None:
+            out[row:row + new] = _turned(q[row:row + new], q_weight, c, s, eps, one_plus_w).to(q.dtype)
+        fresh = (_turned(k[row:row + new], k_weight, c, s, eps, one_plus_w), v[row:row + new])
+        for j in range((n - new) // P, -(-n // P) if new else 0):
+            lo, hi, page = max(n - new, j * P), min(n, (j + 1) * P), pages[j]
+            for x, kept, scales in zip(fresh, (store.k, store.v), (store.k_scale, store.v_scale)):
+                x, held = x[lo - n + new:hi - n + new].transpose(0, 1), lo - j * P
+                if scales is not None:
+                    x = x.float()
+                    scale = page_scale(x.abs().amax((1, 2)))
+                    if held:
+                        scale = torch.maximum(scale, scales[page])              # NaN where either is
+                        grown = (scale > scales[page])[:, None, None]
+                        old = kept[page, :, :held]
+                        moved = (old.float() * (scales[page] / scale)[:, None, None]).to(kept.dtype)
+                        kept[page, :, :held] = torch.where(grown, moved.float(), old.float()).to(kept.dtype)
+                    scales[page] = scale
+                    x = torch.where(torch.isnan(scale)[:, None, None], 0.0, x / scale[:, None, None])
+                kept[page, :, held:hi - j * P] = x.to(kept.dtype)
+    return out
+
+
+def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                 q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, one_plus_w: bool = False) -> Optional[torch.Tensor]:
+    """Writes the new tokens' keys and values ``[rows, kv heads, D]`` into their pages and returns the queries ``[rows, heads, D]`` (when given) as attention takes
+    them; rows of no sequence come back as zeros.
+
+    Keys and queries get their RMS norm over the head (with ``k_weight`` / ``q_weight`` [D], ``1 + weight`` with ``one_plus_w``), then channels ``i`` and ``i + half``
+    are turned by the row's position (``cos``, ``sin`` fp32 [positions, half]), in 32 bits with one rounding at the end.  Operands may be strided views.
+
+    e4m3 pages: the scale of a (page, head) is the smallest power of two, 2^-100 at least, that keeps its largest magnitude within 448.  It grows with later tokens of
+    the page, whose older codes are rescaled (exactly, unless they leave e4m3's normal range); the first slot of a page starts it anew.  A value that is not finite
+    makes it NaN until then, and so the attention of all that sees the page."""
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != store.k.shape[1] or k.shape[2] != store.k.shape[3] or k.shape[0] == 0:
+        raise ValueError(f"paged_append: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit pages {tuple(store.k.shape)}")
+    rows, G, D = k.shape
+    dev = store.k.device
+    if k.device != dev or v.device != dev:
+        raise ValueError("paged_append: k, v and the store lie on different devices")
+    _together("paged_append", store, rows, table, lengths, starts)
+    if q is not None and (q.dim() != 3 or q.shape[0] != rows or q.shape[2] != D or q.shape[1] == 0 or q.dtype != k.dtype or q.device != dev):
+        raise ValueError(f"paged_append: queries {tuple(q.shape)} do not fit keys {tuple(k.shape)}")
+    if (cos is None) != (sin is None):
+        raise ValueError("paged_append: cos and sin go together")
+    half = 0
+    if cos is not None:
+        half = cos.shape[-1]
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] == 0 or half == 0 or 2 * half > D or cos.device != dev or sin.device != dev:
+            raise ValueError(f"paged_append: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} do not fit heads of {D}")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (D,) or w.device != dev):
+            raise ValueError(f"paged_append: norm weights are [{D}] beside the pages")
+    if not k.is_cuda:
+        return _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w)
+    number = _on_gpu("paged_append", store, k.dtype)
+    if half % 8:
+        raise ValueError(f"paged_append: the rotation turns a multiple of 16 channels, got {2 * half}")
+    k, v = _rows_of(k), _rows_of(v)
+    tables, weights = (), (None, None)
+    if half:
+        tables = tuple(t if t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() & 15 == 0 else _aligned(t.float()) for t in (cos, sin))
+    if q_weight is not None or k_weight is not None:
+        weights = tuple(None if w is None else _aligned(w.to(k.dtype)) for w in (q_weight, k_weight))
+    out, H, q_at, out_at, q_row, q_head = None, 0, 0, 0, 0, 0
+    if q is not None:
+        q, H = _rows_of(q), q.shape[1]
+        out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+        q_at, out_at, q_row, q_head = q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1)
+    at = lambda t: 0 if t is None else t.data_ptr()
+    packed = _APPEND.pack(q_at, k.data_ptr(), v.data_ptr(), out_at, store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(),
+                          lengths.data_ptr(), at(starts), tables[0].data_ptr() if half else 0, tables[1].data_ptr() if half else 0, at(weights[0]), at(weights[1]),
+                          err_word(dev).data_ptr(), q_row, q_head, k.stride(0), k.stride(1), v.stride(0), v.stride(1), table.stride(0),
+                          rows, lengths.shape[0], H, G, D, store.k.shape[2], store.k.shape[0], table.shape[1], cos.shape[0] if half else 0, half, int(one_plus_w), eps)
+    check(lib().tyr_paged_append(packed, number, cur_stream(dev)), "paged_append")
+    return out
+
+
+def _attend_ref(q, store, table, lengths, starts, window, scale):
+    rows, H, D = q.shape
+    G, wide = store.k.shape[1], torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros((rows, H, D), dtype=q.dtype, device=q.device)
+    for row, new, n, pages in _spans("paged_attention", store, rows, table, lengths, starts):
+        if not new:
+            continue
+        k, v = (t.to(wide).transpose(0, 1).reshape(G, -1, D)[:, :n] for t in store.values(torch.tensor(pages)))
+        s = torch.einsum("ngrd,gld->grnl", q[row:row + new].to(wide).reshape(new, G, H // G, D), k) * scale
+        if store.v_scale is not None:                    # a page whose values hold no numbers shows at the keys that are seen, as in the kernel
+            s, v = s.masked_fill(torch.isnan(v[..., 0])[:, None, None], math.nan), torch.nan_to_num(v, nan=0.0)
+        ago = torch.arange(n - new, n)[:, None] - torch.arange(n)
+        s = s.masked_fill((ago < 0) | (ago >= (window or n)), -math.inf)
+        out[row:row + new] = torch.einsum("grnl,gld->ngrd", s.softmax(-1), v).reshape(new, H, D).to(q.dtype)
+    return out
+
+
+def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                    window: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of the new tokens' queries ``[rows, heads, D]`` over their sequences' pages, which hold the new tokens already -> ``[rows, heads, D]``; rows of no
+    sequence come back as zeros.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
+    if q.dim() != 3 or q.shape[0] == 0 or q.shape[2] != store.k.shape[3] or q.shape[1] == 0 or q.shape[1] % store.k.shape[1] or q.device != store.k.device:
+        raise ValueError(f"paged_attention: queries {tuple(q.shape)} on {q.device} do not fit pages {tuple(store.k.shape)} on {store.k.device}")
+    rows, H, D = q.shape
+    if window is not None and window <= 0:
+        raise ValueError(f"paged_attention: the window must be positive, got {window}")
+    _together("paged_attention", store, rows, table, lengths, starts)
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    if not q.is_cuda:
+        return _attend_ref(q, store, table, lengths, starts, window, scale)
+    number = _on_gpu("paged_attention", store, q.dtype)
+    q, B = _rows_of(q), lengths.shape[0]
+    pages, G, P, _ = store.k.shape
+    dev, width = q.device, table.shape[1]
+    out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+    tile = 64 if starts is not None and rows * (H // G) > 16 * B else 16
+    whole = width * P <= WHOLE_MAX_KEYS
+    at = lambda t: 0 if t is None else t.data_ptr()
+    tail = (rows, B, H, G, D, P, pages, width, min(window or 0, 2 ** 30), int(whole), scale)
+    head = (q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(), lengths.data_ptr(), at(starts))
+    mid = (err_word(dev).data_ptr(), q.stride(0), q.stride(1), table.stride(0))
+    stream = cur_stream(dev)
+    work, floats = None, ctypes.c_longlong(0)
+    if not whole:
+        rc = lib().tyr_paged_attention(_ATTEND.pack(*head, 0, *mid, *tail), number, tile, stream, ctypes.byref(floats))
+        if rc != 0:
+            raise RuntimeError(f"tyr_b200 native call paged_attention failed with code {rc}")
+        work = torch.empty(floats.value, dtype=torch.float32, device=dev)
+    check(lib().tyr_paged_attention(_ATTEND.pack(*head, at(work), *mid, *tail), number, tile, stream, None), "paged_attention")
+    return out
