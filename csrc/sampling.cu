@@ -1,0 +1,639 @@
+// One token a row from its logits: temperature, top-k, top-p, min-p, and the draw from a given uniform number.
+//
+//   w_i = 2^((l_i - max l) log2(e) / T);  order by (logit descending, index ascending);  the first k stay;  of these those with (weight before them) < p Z, Z the sum
+//   of the first k;  of these those with w >= min_p;  the token is the first index, in vocabulary order, whose cumulative weight exceeds u times the sum of what stays.
+//
+// A token is a whole number: what decides it is computed in 64 bits (a relative error of 1e-7 in the sums would move one draw in some thousand over a flat
+// vocabulary).  2^t is the table method of P. T. P. Tang (1989): 2^(k/32) from a table that lies across a warp's lanes, times a polynomial of degree 5 in the rest.
+//
+// A cluster of CTAs holds a row in shared memory: it is read once.  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
+// decide, by exact sums above, in and below the bin that the counts suggest.  What is left of a bin goes into a list that one CTA sorts; equal logits beyond the list
+// are cut by their indices alone.  top-k up to the list's size needs no counts over all: the k-th largest of the threads' maxima bounds the k-th logit from below, and
+// the few logits above it are listed.  Compiled without fast math.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace tyr {
+namespace cg = cooperative_groups;
+
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleBins = 2048, kSampleList = 1024, kSampleCluster = 16;
+constexpr int kSampleSlice = 16384, kSampleLargest = 40960;                // logits of a CTA: with two of them on an SM, and at most
+
+struct SampleArgs {
+  const void* logits;                    // [rows, V], row stride below
+  const void* draws;                     // [rows] fp32 or fp64
+  const float *temperature, *top_p, *min_p;      // [rows] (null: the numbers below)
+  const int* top_k;
+  long long* token;
+  long long row;
+  int rows, V, slice, draws64, k;
+  float t, p, m;
+};
+static_assert(sizeof(SampleArgs) == 96, "as ops/sampling.py packs it");
+
+struct Place { uint32_t key, index; };                                     // what comes no later in the order stays
+
+__device__ __forceinline__ uint32_t key_of(float x) {                      // 0: never chosen (-inf, NaN, behind the row)
+  const uint32_t b = __float_as_uint(x);
+  if (!(x > -INFINITY)) return 0u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ bool stays(uint32_t key, uint32_t index, Place c) { return key > c.key || (key == c.key && index <= c.index); }
+
+__device__ __forceinline__ float load_logit(const float* p) { return *p; }
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_scan_d(double v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+struct Weights {                         // 2^((x - top) c), all lanes of a warp together
+  double table, top, c;
+  __device__ __forceinline__ double operator()(float x) const {
+    const double t = fmax((static_cast<double>(x) - top) * c, -1000.0);
+    constexpr double kMagic = 211106232532992.0;                           // 1.5 * 2^47: its last place is 2^-5
+    const double r = t + kMagic, f = t - (r - kMagic);
+    const int k = __double2loint(r);
+    // ln2^i / i!
+    const double e = fma(f, fma(f, fma(f, fma(f, fma(f, 1.3333558146428443e-3, 9.618129107628477e-3), 5.550410866482158e-2), 2.402265069591007e-1), 6.931471805599453e-1), 1.0);
+    const double w = __shfl_sync(0xffffffffu, table, k & 31) * e;
+    return __hiloint2double(__double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
+  }
+};
+
+struct Partial { double above, in, below; uint32_t count, low, high, pad; };
+
+struct SampleShared {
+  uint32_t bins[kSampleBins], total[kSampleBins];
+  unsigned long long list[kSampleList];
+  double weight[kSampleList];
+  double warp_sums[kSampleCluster * kSampleWarps];                                   // of all warps of the cluster
+  Partial part[kSampleCluster], warp_part[kSampleWarps];
+  float tops[kSampleCluster], warp_top[kSampleWarps];
+  uint32_t scan[kSampleWarps], listed, counts[kSampleCluster * kSampleWarps];
+  double scan_d[kSampleWarps];
+  Place cut;
+  int found, flag;
+};
+
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s, uint32_t& total) {      // inclusive
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = v;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) {
+    if (i < warp) before += s[i];
+    total += s[i];
+  }
+  return v + before;
+}
+__device__ __forceinline__ double block_scan_d(double v, double* s, double& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_scan_d(v, lane);
+  __syncthreads();
+  if (lane == 31) s[warp] = v;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) {
+    if (i < warp) before += s[i];
+    total += s[i];
+  }
+  return v + before;
+}
+// n items of a power of two, largest first
+__device__ __forceinline__ void block_sort(unsigned long long* v, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const unsigned long long x = v[a], y = v[b];
+        if ((x < y) == ((a & size) == 0)) {
+          v[a] = y;
+          v[b] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
+  constexpr int WARPS = kSampleWarps;
+  pdl_trigger();
+  cluster_arrive();                                                        // no CTA writes into another's shared memory before that one runs
+  pdl_wait();
+  extern __shared__ float s_logits[];
+  __shared__ SampleShared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* logits = static_cast<const T*>(a.logits) + row * a.row;
+  // a CTA's slice and a warp's part of it are consecutive; a lane looks at every 32nd
+  const int per_warp = a.slice / WARPS, its = per_warp / 32, base = rank * a.slice + warp * per_warp + lane;
+  float* x = s_logits + warp * per_warp + lane;
+  const auto clean = [](float v) { return v == 0.f ? 0.f : (v != v ? -INFINITY : v); };        // -0 is 0, NaN is never chosen
+  {
+    constexpr int VEC = 16 / sizeof(T);
+    const int first = base - lane, here = max(0, min(per_warp, a.V - first));
+    float* part = x - lane;
+    int done = 0;
+    if ((reinterpret_cast<uintptr_t>(logits + first) & 15) == 0) {
+      done = here / VEC * VEC;
+#pragma unroll 8
+      for (int i = lane * VEC; i < done; i += 32 * VEC) {
+        const uint4 u = *reinterpret_cast<const uint4*>(logits + first + i);
+        T v[VEC];
+        *reinterpret_cast<uint4*>(v) = u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) part[i + e] = clean(load_logit(v + e));
+      }
+    }
+#pragma unroll 16
+    for (int i = done + lane; i < per_warp; i += 32) part[i] = i < here ? clean(load_logit(logits + first + i)) : -INFINITY;
+    __syncwarp();
+  }
+  const float T_row = a.temperature ? a.temperature[row] : a.t, p_row = a.top_p ? a.top_p[row] : a.p, m_row = a.min_p ? a.min_p[row] : a.m;
+  const int k_row = a.top_k ? a.top_k[row] : a.k;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int j = 0; j < its; ++j) top = fmaxf(top, x[32 * j]);
+  float own_top = top;
+  top = warp_max(top);
+  if (lane == 0) s.warp_top[warp] = top;
+  if (tid == 0) s.listed = 0, s.found = -1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, s.warp_top[i]);
+  cluster_wait();
+  if (tid < C) cluster.map_shared_rank(s.tops, tid)[rank] = top;
+  for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
+  cluster.sync();
+  for (int i = 0; i < C; ++i) top = fmaxf(top, s.tops[i]);
+  const auto index_of = [&](int j) { return static_cast<uint32_t>(base + 32 * j); };
+
+  if (top == -INFINITY || !(T_row > 0.f)) {                                // nothing to choose from, or the largest: the lowest index that holds it
+    uint32_t first = 0xffffffffu;
+    for (int j = its - 1; j >= 0; --j)
+      if (x[32 * j] == top && top > -INFINITY) first = index_of(j);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.scan[warp] = first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 1; i < WARPS; ++i) first = min(first, s.scan[i]);
+      cluster.map_shared_rank(s.counts, 0)[rank] = first;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int i = 0; i < C; ++i) first = min(first, s.counts[i]);
+      a.token[row] = first == 0xffffffffu ? -1 : static_cast<long long>(first);
+    }
+    return;
+  }
+  if (top == INFINITY) {                                                   // infinite logits share the draw
+#pragma unroll 4
+    for (int j = 0; j < its; ++j) x[32 * j] = x[32 * j] == INFINITY ? 0.f : -INFINITY;
+    own_top = own_top == INFINITY ? 0.f : -INFINITY;
+    top = 0.f;
+  }
+  const double c = 1.4426950408889634 / static_cast<double>(T_row);
+  const Weights weigh{exp2(lane / 32.0), static_cast<double>(top), c};
+  const double u = a.draws64 ? static_cast<const double*>(a.draws)[row] : static_cast<double>(static_cast<const float*>(a.draws)[row]);
+  const double p = p_row, m = fmin(static_cast<double>(m_row), 1.0);
+  const bool by_mass = p < 1.0;
+  const float per_bin = fminf(static_cast<float>(c * 64.0), 1e30f);        // bins of 1/64 of a factor of two
+  const auto bin_of = [&](float v) { return v > -INFINITY ? static_cast<int>(fminf((top - v) * per_bin, static_cast<float>(kSampleBins - 1))) : kSampleBins; };
+
+  // the counts of all CTAs' bins, in every CTA
+  const auto merge_bins = [&]() {
+    cluster.sync();
+    const int per = (kSampleBins + C - 1) / C;
+    for (int i = rank * per + tid; i < min(kSampleBins, (rank + 1) * per); i += kSampleThreads) {
+      uint32_t n = 0;
+      for (int r = 0; r < C; ++r) n += cluster.map_shared_rank(s.bins, r)[i];
+      for (int r = 0; r < C; ++r) cluster.map_shared_rank(s.total, r)[i] = n;
+    }
+    cluster.sync();
+  };
+  // first bin up to which the merged counts reach `want` (kSampleBins: none); all threads
+  const auto bin_reaching = [&](uint32_t want) {
+    constexpr int PER = kSampleBins / kSampleThreads;
+    uint32_t n[PER], sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += n[i] = s.total[tid * PER + i];
+    uint32_t upto = block_scan(sum, s.scan, total) - sum;
+    if (tid == 0) s.found = kSampleBins;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (upto < want && upto + n[i] >= want) s.found = tid * PER + i;
+      upto += n[i];
+    }
+    __syncthreads();
+    return s.found;
+  };
+  // puts what `take` names into CTA 0's list; its length (beyond the list's end: too many), in every CTA after a cluster.sync()
+  const auto gather = [&](auto take) {
+    SampleShared* lead = cluster.map_shared_rank(&s, 0);
+#pragma unroll 4
+    for (int j = 0; j < its; ++j) {
+      const uint32_t key = key_of(x[32 * j]);
+      if (key != 0 && take(x[32 * j], key, index_of(j))) {
+        const uint32_t at = atomicAdd(&lead->listed, 1u);
+        if (at < kSampleList) lead->list[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j);
+      }
+    }
+    cluster.sync();
+    return lead->listed;
+  };
+  const auto list_power = [&](int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
+    return size;
+  };
+
+  Place cut{1u, 0xffffffffu};                                              // keeps all
+
+  // ---- top-k -------------------------------------------------------------------------------------------------------------
+  if (k_row > 0 && k_row < a.V) {
+    bool listed = false;
+    if (k_row <= kSampleList) {
+      const int own = bin_of(own_top);
+      if (own < kSampleBins) atomicAdd(&s.bins[own], 1u);
+      merge_bins();
+      const int bin = bin_reaching(k_row);                                 // none: fewer maxima than k
+      const uint32_t n = gather([&](float v, uint32_t, uint32_t) { return bin < kSampleBins && bin_of(v) <= bin; });
+      listed = bin < kSampleBins && n <= kSampleList;
+      if (listed) {
+        // ---- all that can stay lies in CTA 0's list ----------------------------------------------------------------------------
+        cluster.sync();                                                    // the others have read its length
+        if (rank != 0) return;
+        const int size = list_power(n);
+        block_sort(s.list, size);
+        const int kept = min(static_cast<int>(n), k_row);
+        constexpr int PER = kSampleList / kSampleThreads;
+        double w[PER], sum = 0.0, total;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int at = tid * PER + i;
+          const double v = weigh(at < kept ? value_of(static_cast<uint32_t>(s.list[at] >> 32)) : 0.f);
+          w[i] = at < kept ? v : 0.0;
+          sum += w[i];
+        }
+        double before = block_scan_d(sum, s.scan_d, total) - sum;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int at = tid * PER + i;
+          const bool in = at < kept && (at == 0 || (w[i] >= m && (!by_mass || before < p * total)));
+          before += w[i];
+          s.weight[at] = in ? w[i] : 0.0;
+        }
+        __syncthreads();
+        // into vocabulary order: ~index in the upper half sorts the lowest first
+        unsigned long long moved[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int at = tid * PER + i;
+          moved[i] = at < size && s.weight[at] > 0.0 ? s.list[at] << 32 | static_cast<unsigned>(at) : 0ull;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (tid * PER + i < size) s.list[tid * PER + i] = moved[i];
+        if (tid == 0) s.found = 0x7fffffff, s.flag = 0;
+        block_sort(s.list, size);
+        double v[PER];
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int at = tid * PER + i;
+          v[i] = at < size && s.list[at] != 0 ? s.weight[static_cast<uint32_t>(s.list[at])] : 0.0;
+          sum += v[i];
+        }
+        double upto = block_scan_d(sum, s.scan_d, total) - sum;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          upto += v[i];
+          if (v[i] > 0.0) {
+            atomicMax(&s.flag, tid * PER + i);
+            if (upto > u * total) atomicMin(&s.found, tid * PER + i);
+          }
+        }
+        __syncthreads();
+        if (tid == 0) a.token[row] = ~static_cast<uint32_t>(s.list[min(s.found, s.flag)] >> 32);
+        return;
+      }
+      cluster.sync();
+      if (tid == 0) s.listed = 0;
+      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
+      cluster.sync();
+    }
+  }
+
+  // One cut in the order: by the number of what stays (k), or by its weight (below p times the weight of all that the present cut keeps).
+  const auto select = [&](bool mass, uint32_t k) {
+    uint32_t low = 0, high = 0xffffffffu, above_n = 0;
+    double above = 0.0, aim = 0.0;
+    bool first = true;
+    int shift = 0;
+    uint32_t in_n;
+    // bins of the present interval: by value over all, then by key
+    const auto place = [&](float v, uint32_t key) { return first ? bin_of(v) : static_cast<int>((high - key) >> shift); };
+    const auto inside = [&](uint32_t key, uint32_t index) { return key != 0 && key >= low && key <= high && stays(key, index, cut); };
+    while (true) {
+#pragma unroll 4
+      for (int j = 0; j < its; ++j) {
+        const uint32_t key = key_of(x[32 * j]);
+        if (inside(key, index_of(j))) atomicAdd(&s.bins[place(x[32 * j], key)], 1u);
+      }
+      merge_bins();
+      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
+      int bin;
+      Partial all;
+      // weights above, in and below a bin of the interval
+      const auto weigh_bin = [&](int b) {
+        Partial q{0.0, 0.0, 0.0, 0u, 0xffffffffu, 0u, 0u};
+#pragma unroll 4
+        for (int j = 0; j < its; ++j) {
+          const uint32_t key = key_of(x[32 * j]);
+          const bool is_in = inside(key, index_of(j));
+          const int at = is_in ? place(x[32 * j], key) : 0;
+          if (mass && __any_sync(0xffffffffu, is_in)) {
+            const double w = weigh(x[32 * j] > -INFINITY ? x[32 * j] : top);
+            if (is_in) (at < b ? q.above : at == b ? q.in : q.below) += w;
+          }
+          if (is_in && at == b) {
+            ++q.count;
+            q.low = min(q.low, key);
+            q.high = max(q.high, key);
+          }
+        }
+        q.above = warp_sum_d(q.above), q.in = warp_sum_d(q.in), q.below = warp_sum_d(q.below);
+        q.count = __reduce_add_sync(0xffffffffu, q.count);
+        q.low = __reduce_min_sync(0xffffffffu, q.low);
+        q.high = __reduce_max_sync(0xffffffffu, q.high);
+        const auto join = [](Partial& x, const Partial& y) {
+          x.above += y.above, x.in += y.in, x.below += y.below, x.count += y.count;
+          x.low = min(x.low, y.low), x.high = max(x.high, y.high);
+        };
+        if (lane == 0) s.warp_part[warp] = q;
+        __syncthreads();
+        q = s.warp_part[0];
+#pragma unroll
+        for (int i = 1; i < WARPS; ++i) join(q, s.warp_part[i]);
+        if (tid < C) cluster.map_shared_rank(s.part, tid)[rank] = q;
+        cluster.sync();
+        q = s.part[0];
+        for (int i = 1; i < C; ++i) join(q, s.part[i]);
+        cluster.sync();
+        return q;
+      };
+      if (!mass) {
+        bin = bin_reaching(k - above_n);
+        if (bin == kSampleBins) return;                                    // no more than k to choose from
+        all = weigh_bin(bin);
+        // what lies above the bin, from the counts
+        uint32_t n = 0, total;
+        for (int i = tid; i < bin; i += kSampleThreads) n += s.total[i];
+        block_scan(n, s.scan, total);
+        above_n += total;
+      } else {
+        // where the counts, each taken at its bin's middle, reach the aim; exact sums then say how far off that is
+        constexpr int PER = kSampleBins / kSampleThreads;
+        double est[PER], sum = 0.0, total;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int b = tid * PER + i;
+          const double mid = first ? static_cast<double>(top) - (b + 0.5) / static_cast<double>(per_bin)
+                                   : static_cast<double>(value_of(max(low, high - min(high - low, (static_cast<uint32_t>(b) << shift) + ((1u << shift) >> 1)))));
+          est[i] = s.total[b] ? s.total[b] * exp2(fmax((mid - static_cast<double>(top)) * c, -1000.0)) : 0.0;
+          sum += est[i];
+        }
+        const double est_before = block_scan_d(sum, s.scan_d, total) - sum;
+        double want = first ? p * total : aim - above;
+        int least = 0, most = kSampleBins - 1;
+        while (true) {
+          if (tid == 0) s.found = kSampleBins, s.flag = least;
+          __syncthreads();
+          double upto = est_before;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int b = tid * PER + i;
+            upto += est[i];
+            if (s.total[b] && b >= least && b <= most) {
+              if (upto >= want) atomicMin(&s.found, b);
+              atomicMax(&s.flag, b);                                       // the last that holds any
+            }
+          }
+          __syncthreads();
+          bin = min(s.found, s.flag);
+          // the estimate of what lies above it
+          if (tid == bin / PER) {
+            double e = est_before;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              if (tid * PER + i < bin) e += est[i];
+            s.scan_d[0] = e;
+          }
+          __syncthreads();
+          const double est_above = s.scan_d[0];
+          all = weigh_bin(bin);
+          if (first) aim = fmax(p * (all.above + all.in + all.below), 1e-300);
+          const double goal = aim - above;
+          if (goal <= all.above && bin > least) most = bin - 1;             // the cut lies further up ...
+          else if (goal > all.above + all.in && bin < most) least = bin + 1;     // ... or down
+          else break;
+          want = goal + (est_above - all.above);
+        }
+        above += all.above;
+      }
+      in_n = all.count;
+      low = all.low;
+      high = all.high;
+      if (low >= high || in_n <= kSampleList) break;
+      first = false;
+      shift = 0;
+      while (((high - low) >> shift) >= static_cast<uint32_t>(kSampleBins)) ++shift;
+    }
+    const auto member = [&](uint32_t key, uint32_t index) { return key >= low && key <= high && stays(key, index, cut); };
+    if (in_n <= kSampleList) {
+      const uint32_t n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); });
+      if (rank == 0) {
+        block_sort(s.list, list_power(n));
+        int last;                                                          // the last of the list that stays
+        if (!mass) {
+          last = static_cast<int>(k - above_n) - 1;
+        } else {
+          constexpr int PER = kSampleList / kSampleThreads;
+          double w[PER], sum = 0.0, total;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int at = tid * PER + i;
+            const double v = weigh(at < static_cast<int>(n) ? value_of(static_cast<uint32_t>(s.list[at] >> 32)) : 0.f);
+            w[i] = at < static_cast<int>(n) ? v : 0.0;
+            sum += w[i];
+          }
+          double before = above + block_scan_d(sum, s.scan_d, total) - sum;
+          if (tid == 0) s.flag = 0;
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            if (tid * PER + i < static_cast<int>(n) && before < aim) atomicMax(&s.flag, tid * PER + i);
+            before += w[i];
+          }
+          __syncthreads();
+          last = s.flag;
+        }
+        if (tid < C) {
+          const unsigned long long it = s.list[last];
+          cluster.map_shared_rank(&s, tid)->cut = Place{static_cast<uint32_t>(it >> 32), ~static_cast<uint32_t>(it)};
+        }
+      }
+    } else {
+      // more equal logits than the list holds: the first ones in vocabulary order
+      double w = weigh(value_of(high));
+      const double take = mass ? ceil((aim - above) / w) : static_cast<double>(k - above_n);
+      const uint32_t want = take >= in_n ? in_n : take < 1.0 ? 1u : static_cast<uint32_t>(take);
+      uint32_t n = 0;
+#pragma unroll 4
+      for (int j = 0; j < its; ++j) n += member(key_of(x[32 * j]), index_of(j)) ? 1u : 0u;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane < C) cluster.map_shared_rank(s.counts, lane)[rank * WARPS + warp] = n;
+      cluster.sync();
+      uint32_t before = 0;
+      for (int i = lane; i < rank * WARPS + warp; i += 32) before += s.counts[i];
+      before = __reduce_add_sync(0xffffffffu, before);
+      if (before < want && before + n >= want) {
+#pragma unroll 4
+        for (int j = 0; j < its; ++j) {
+          const uint32_t in = __ballot_sync(0xffffffffu, member(key_of(x[32 * j]), index_of(j)));
+          const uint32_t mine = before + __popc(in & ((2u << lane) - 1u));
+          if (before < want && before + __popc(in) >= want && (in >> lane & 1) && mine == want)
+            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&s, r)->cut = Place{high, index_of(j)};
+          before += __popc(in);
+        }
+      }
+    }
+    cluster.sync();
+    cut = s.cut;
+    if (tid == 0) s.listed = 0;
+    cluster.sync();
+  };
+  if (k_row > 0 && k_row < a.V) select(false, k_row);
+  if (by_mass) select(true, 0);
+
+  // ---- the draw ------------------------------------------------------------------------------------------------------------
+  const auto weight_of = [&](int j) {
+    const uint32_t key = key_of(x[32 * j]);
+    const bool in = key != 0 && stays(key, index_of(j), cut);
+    if (!__any_sync(0xffffffffu, in)) return 0.0;
+    const double w = weigh(in ? x[32 * j] : top);
+    return in && w >= m ? w : 0.0;
+  };
+  double sum = 0.0;
+#pragma unroll 4
+  for (int j = 0; j < its; ++j) sum += weight_of(j);
+  sum = warp_sum_d(sum);
+  if (lane < C) cluster.map_shared_rank(s.warp_sums, lane)[rank * WARPS + warp] = sum;
+  cluster.sync();
+  // the warp in which the cumulative weight passes the aim, else the last that holds any
+  const int n = C * WARPS, each = (n + 31) / 32;
+  double mine = 0.0;
+  for (int i = lane * each; i < min(n, (lane + 1) * each); ++i) mine += s.warp_sums[i];
+  const double upto_lane = warp_scan_d(mine, lane), aim = u * __shfl_sync(0xffffffffu, upto_lane, 31);
+  double before = upto_lane - mine, before_at = 0.0, before_last = 0.0;
+  uint32_t passes = 0xffffffffu, last = 0;
+  for (int i = lane * each; i < min(n, (lane + 1) * each); ++i) {
+    const double v = s.warp_sums[i];
+    if (v > 0.0) {
+      if (passes == 0xffffffffu && before + v > aim) passes = i, before_at = before;
+      last = i, before_last = before;
+    }
+    before += v;
+  }
+  const uint32_t first_past = __reduce_min_sync(0xffffffffu, passes), last_any = __reduce_max_sync(0xffffffffu, last);
+  const int at = first_past == 0xffffffffu ? last_any : first_past;
+  before_at = __shfl_sync(0xffffffffu, first_past == 0xffffffffu ? before_last : before_at, at / each);
+  if (at == rank * WARPS + warp) {
+    double upto = before_at;
+    uint32_t chosen = 0, found = 0;
+#pragma unroll 4
+    for (int j = 0; j < its; ++j) {
+      const double w = weight_of(j), c_j = upto + warp_scan_d(w, lane);
+      const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0), past = __ballot_sync(0xffffffffu, w > 0.0 && c_j > aim);
+      if (!found && any) chosen = __shfl_sync(0xffffffffu, index_of(j), past ? __ffs(past) - 1 : 31 - __clz(any));
+      found |= past;
+      upto = __shfl_sync(0xffffffffu, c_j, 31);
+    }
+    if (lane == 0) a.token[row] = chosen;
+  }
+}
+
+template <typename T>
+int sample_form(SampleArgs a, cudaStream_t stream) {
+  static const cudaError_t ready = [] {
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleLargest * 4);
+  }();
+  if (ready != cudaSuccess) return static_cast<int>(ready);
+  // the fewest CTAs a row that leave room for two on an SM; more while there are few rows
+  int ctas = 1;
+  while (ctas < kSampleCluster && (static_cast<long long>(ctas) * kSampleSlice < a.V || (a.rows * ctas * 2 <= 148 && ctas * kSampleThreads * 4 < a.V))) ctas *= 2;
+  if (static_cast<long long>(ctas) * kSampleLargest < a.V) return -2;
+  a.slice = (a.V + ctas * kSampleThreads - 1) / (ctas * kSampleThreads) * kSampleThreads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = a.slice * 4;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+}
+
+}  // namespace tyr
+
+using namespace tyr;
+
+// dtype: 0 = bf16, 1 = fp16, 2 = fp32 (the logits)
+extern "C" TYR_EXPORT int tyr_sample(const void* packed, int dtype, void* stream) {
+  const SampleArgs& a = *static_cast<const SampleArgs*>(packed);
+  if (a.rows <= 0 || a.V <= 0 || a.rows > (1 << 26)) return -1;
+  switch (dtype) {
+    case 0: return sample_form<__nv_bfloat16>(a, (cudaStream_t)stream);
+    case 1: return sample_form<__half>(a, (cudaStream_t)stream);
+    case 2: return sample_form<float>(a, (cudaStream_t)stream);
+  }
+  return -3;
+}

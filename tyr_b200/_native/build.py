@@ -36,7 +36,7 @@ NVCC_FLAGS = [
 ]
 # Units whose results are carried through thousands of steps, stand for the fp32 mode or go to a store that later steps read: division, square root and
 # functions as they are written (a kernel that takes an approximation names it) and no flushing of denormals.  Every other unit is compiled with fast math.
-PRECISE_UNITS = ("delta_general", "attention_general", "depth_average", "flux_tables", "gates", "joint_attention", "latent", "lightning", "mix_conv", "paged_append", "prompt_mix", "rotary_store",
+PRECISE_UNITS = ("delta_general", "attention_general", "depth_average", "flux_tables", "gates", "joint_attention", "latent", "lightning", "mix_conv", "paged_append", "prompt_mix", "rotary_store", "sampling",
                  "selective_scan")
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-pthread"]
 
