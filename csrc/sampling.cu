@@ -28,10 +28,10 @@ struct SampleArgs {
   const int* top_k;
   long long* token;
   long long row;
-  int rows, V, slice, draws64, k;
-  float t, p, m;
+  double t, p, m;
+  int rows, V, slice, draws64, k, pad;
 };
-static_assert(sizeof(SampleArgs) == 96, "as ops/sampling.py packs it");
+static_assert(sizeof(SampleArgs) == 112, "as ops/sampling.py packs it");
 
 struct Place { uint32_t key, index; };                                     // what comes no later in the order stays
 
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     for (int i = done + lane; i < per_warp; i += 32) part[i] = i < here ? clean(load_logit(logits + first + i)) : -INFINITY;
     __syncwarp();
   }
-  const float T_row = a.temperature ? a.temperature[row] : a.t, p_row = a.top_p ? a.top_p[row] : a.p, m_row = a.min_p ? a.min_p[row] : a.m;
+  const double T_row = a.temperature ? a.temperature[row] : a.t, p = a.top_p ? a.top_p[row] : a.p, m = fmin(a.min_p ? a.min_p[row] : a.m, 1.0);
   const int k_row = a.top_k ? a.top_k[row] : a.k;
   float top = -INFINITY;
 #pragma unroll 4
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   for (int i = 0; i < C; ++i) top = fmaxf(top, s.tops[i]);
   const auto index_of = [&](int j) { return static_cast<uint32_t>(base + 32 * j); };
 
-  if (top == -INFINITY || !(T_row > 0.f)) {                                // nothing to choose from, or the largest: the lowest index that holds it
+  if (top == -INFINITY || !(T_row > 0.0)) {                                // nothing to choose from, or the largest: the lowest index that holds it
     uint32_t first = 0xffffffffu;
     for (int j = its - 1; j >= 0; --j)
       if (x[32 * j] == top && top > -INFINITY) first = index_of(j);
@@ -220,10 +220,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     own_top = own_top == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
   }
-  const double c = 1.4426950408889634 / static_cast<double>(T_row);
+  const double c = 1.4426950408889634 / T_row;
   const Weights weigh{exp2(lane / 32.0), static_cast<double>(top), c};
   const double u = a.draws64 ? static_cast<const double*>(a.draws)[row] : static_cast<double>(static_cast<const float*>(a.draws)[row]);
-  const double p = p_row, m = fmin(static_cast<double>(m_row), 1.0);
   const bool by_mass = p < 1.0;
   const float per_bin = fminf(static_cast<float>(c * 64.0), 1e30f);        // bins of 1/64 of a factor of two
   const auto bin_of = [&](float v) { return v > -INFINITY ? static_cast<int>(fminf((top - v) * per_bin, static_cast<float>(kSampleBins - 1))) : kSampleBins; };

@@ -47,8 +47,7 @@ def check(logits, draws, dev, **kw):
     at = lambda name, b, default: default if kw.get(name) is None else (kw[name][b].item() if torch.is_tensor(kw[name]) else kw[name])
     rows, checked = logits.double().numpy(), 0
     for b in range(B):
-        want, near = draw_of(rows[b], draws[b].item(), np.float64(np.float32(at("temperature", b, 1.0))), at("top_k", b, 0), np.float64(np.float32(at("top_p", b, 1.0))),
-                             np.float64(np.float32(at("min_p", b, 0.0))))
+        want, near = draw_of(rows[b], draws[b].item(), at("temperature", b, 1.0), at("top_k", b, 0), at("top_p", b, 1.0), at("min_p", b, 0.0))
         if near > 1e-12:
             checked += 1
             assert got[b].item() == want, (b, got[b].item(), want, near)

@@ -17,7 +17,7 @@ from ._common import check, cur_stream, lib
 MAX_VOCAB = 16 * 40960                  # logits that a cluster's shared memory holds
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 # the kernel's argument block, as csrc/sampling.cu declares it
-_ARGS = struct.Struct("@8q5i3f")
+_ARGS = struct.Struct("@8q3d6i")
 
 Setting = Union[float, torch.Tensor]
 
@@ -68,7 +68,8 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
 
     With w = exp((logit - the row's largest) / ``temperature``) and the tokens in the order of their logits, equal ones by index: the first ``top_k`` stay (0 or None:
     all), of these those whose predecessors hold less than ``top_p`` of their weight (1: all; the first always stays), of these those with w >= ``min_p``.  The token is
-    the first one, by index, at which the weight of what stays exceeds the row's draw times the whole.  All of it is decided in 64 bits.
+    the first one, by index, at which the weight of what stays exceeds the row's draw times the whole.  All of it is decided in 64 bits, and a
+    setting given as a number counts as such.
 
     A temperature of 0 takes the largest logit, the lowest index among equals.  -inf and NaN are never chosen, infinite logits share the draw; a row with nothing to
     choose from gives -1.  Every setting is a number or holds one for each row (fp32; ``top_k`` int32), on the logits' device."""
@@ -93,7 +94,7 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
         logits = logits.contiguous()
     draws = draws.contiguous()
     token = torch.empty(B, dtype=torch.int64, device=logits.device)
-    packed = _ARGS.pack(logits.data_ptr(), draws.data_ptr(), t_at, p_at, m_at, k_at, token.data_ptr(), logits.stride(0), B, V, 0, draws.dtype == torch.float64,
-                        min(int(k), V), t, p, m)
+    packed = _ARGS.pack(logits.data_ptr(), draws.data_ptr(), t_at, p_at, m_at, k_at, token.data_ptr(), logits.stride(0), t, p, m, B, V, 0, draws.dtype == torch.float64,
+                        min(int(k), V), 0)
     check(lib().tyr_sample(packed, number, cur_stream(logits.device)), "sample")
     return token
