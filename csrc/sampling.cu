@@ -61,28 +61,30 @@ __device__ __forceinline__ double warp_scan_d(double v, int lane) {
   return v;
 }
 
-struct Weights {                         // 2^((x - top) c), all lanes of a warp together
+struct Weights {                         // 2^((x - top) c), all lanes of a warp together; 2^-900, next to nothing, where it would be less and for -inf
   double table, top, c;
   __device__ __forceinline__ double operator()(float x) const {
-    const double t = fmax((static_cast<double>(x) - top) * c, -1000.0);
+    const double far = (static_cast<double>(x) - top) * c;                  // never positive: as unsigned numbers, the larger the further
+    const double t = __hiloint2double(static_cast<int>(min(static_cast<uint32_t>(__double2hiint(far)), 0xC08C2000u)), __double2loint(far));
     constexpr double kMagic = 211106232532992.0;                           // 1.5 * 2^47: its last place is 2^-5
     const double r = t + kMagic, f = t - (r - kMagic);
     const int k = __double2loint(r);
     // ln2^i / i!
     const double e = fma(f, fma(f, fma(f, fma(f, fma(f, 1.3333558146428443e-3, 9.618129107628477e-3), 5.550410866482158e-2), 2.402265069591007e-1), 6.931471805599453e-1), 1.0);
-    const double w = __shfl_sync(0xffffffffu, table, k & 31) * e;
+    const double w = __shfl_sync(0xffffffffu, table, k) * e;
     return __hiloint2double(__double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
   }
 };
 
-struct Partial { double above, in, below; uint32_t count, low, high, pad; };
+struct Partial { double above, in, all; uint32_t count, low, high, pad; };
 
 struct SampleShared {
   uint32_t bins[kSampleBins], total[kSampleBins];
   unsigned long long list[kSampleList];
   double weight[kSampleList];
   double warp_sums[kSampleCluster * kSampleWarps];                                   // of all warps of the cluster
-  Partial part[kSampleCluster], warp_part[kSampleWarps];
+  Partial part[2][kSampleCluster], warp_part[kSampleWarps];
+  double warp_above[kSampleWarps];                                         // of a warp's logits above the bin of the cut
   float tops[kSampleCluster], warp_top[kSampleWarps];
   uint32_t scan[kSampleWarps], listed, counts[kSampleCluster * kSampleWarps];
   double scan_d[kSampleWarps];
@@ -157,6 +159,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const int per_warp = a.slice / WARPS, its = per_warp / 32, base = rank * a.slice + warp * per_warp + lane;
   float* x = s_logits + warp * per_warp + lane;
   const auto clean = [](float v) { return v == 0.f ? 0.f : (v != v ? -INFINITY : v); };        // -0 is 0, NaN is never chosen
+  float top = -INFINITY;
   {
     constexpr int VEC = 16 / sizeof(T);
     const int first = base - lane, here = max(0, min(per_warp, a.V - first));
@@ -166,22 +169,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       done = here / VEC * VEC;
 #pragma unroll 8
       for (int i = lane * VEC; i < done; i += 32 * VEC) {
-        const uint4 u = *reinterpret_cast<const uint4*>(logits + first + i);
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(logits + first + i));
         T v[VEC];
         *reinterpret_cast<uint4*>(v) = u;
+        float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) part[i + e] = clean(load_logit(v + e));
+        for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e] = clean(load_logit(v + e)));
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(part + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
       }
     }
 #pragma unroll 16
-    for (int i = done + lane; i < per_warp; i += 32) part[i] = i < here ? clean(load_logit(logits + first + i)) : -INFINITY;
+    for (int i = done + lane; i < per_warp; i += 32) {
+      const float v = i < here ? clean(load_logit(logits + first + i)) : -INFINITY;
+      part[i] = v;
+      top = fmaxf(top, v);
+    }
     __syncwarp();
   }
   const double T_row = a.temperature ? a.temperature[row] : a.t, p = a.top_p ? a.top_p[row] : a.p, m = fmin(a.min_p ? a.min_p[row] : a.m, 1.0);
   const int k_row = a.top_k ? a.top_k[row] : a.k;
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int j = 0; j < its; ++j) top = fmaxf(top, x[32 * j]);
   float own_top = top;
   top = warp_max(top);
   if (lane == 0) s.warp_top[warp] = top;
@@ -220,12 +227,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     own_top = own_top == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
   }
-  const double c = 1.4426950408889634 / T_row;
+  const double c = fmax(1.4426950408889634 / T_row, 1e-300);
   const Weights weigh{exp2(lane / 32.0), static_cast<double>(top), c};
   const double u = a.draws64 ? static_cast<const double*>(a.draws)[row] : static_cast<double>(static_cast<const float*>(a.draws)[row]);
   const bool by_mass = p < 1.0;
   const float per_bin = fminf(static_cast<float>(c * 64.0), 1e30f);        // bins of 1/64 of a factor of two
-  const auto bin_of = [&](float v) { return v > -INFINITY ? static_cast<int>(fminf((top - v) * per_bin, static_cast<float>(kSampleBins - 1))) : kSampleBins; };
+  const auto far_of = [&](float v) { return (top - v) * per_bin; };         // in bins; -inf is beyond them all
+  const auto bin_of = [&](float v) { return v > -INFINITY ? static_cast<int>(fminf(far_of(v), static_cast<float>(kSampleBins - 1))) : kSampleBins; };
 
   // the counts of all CTAs' bins, in every CTA
   const auto merge_bins = [&]() {
@@ -233,8 +241,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const int per = (kSampleBins + C - 1) / C;
     for (int i = rank * per + tid; i < min(kSampleBins, (rank + 1) * per); i += kSampleThreads) {
       uint32_t n = 0;
-      for (int r = 0; r < C; ++r) n += cluster.map_shared_rank(s.bins, r)[i];
-      for (int r = 0; r < C; ++r) cluster.map_shared_rank(s.total, r)[i] = n;
+#pragma unroll
+      for (int r = 0; r < kSampleCluster; ++r) n += r < C ? cluster.map_shared_rank(s.bins, r)[i] : 0u;
+#pragma unroll
+      for (int r = 0; r < kSampleCluster; ++r)
+        if (r < C) cluster.map_shared_rank(s.total, r)[i] = n;
     }
     cluster.sync();
   };
@@ -256,12 +267,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return s.found;
   };
   // puts what `take` names into CTA 0's list; its length (beyond the list's end: too many), in every CTA after a cluster.sync()
-  const auto gather = [&](auto take) {
+  const auto gather = [&](auto take, auto near) {                         // `near`: a cheap test that none fails
     SampleShared* lead = cluster.map_shared_rank(&s, 0);
 #pragma unroll 4
     for (int j = 0; j < its; ++j) {
-      const uint32_t key = key_of(x[32 * j]);
-      if (key != 0 && take(x[32 * j], key, index_of(j))) {
+      const float v = x[32 * j];
+      if (!near(v)) continue;
+      const uint32_t key = key_of(v);
+      if (key != 0 && take(v, key, index_of(j))) {
         const uint32_t at = atomicAdd(&lead->listed, 1u);
         if (at < kSampleList) lead->list[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j);
       }
@@ -276,6 +289,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return size;
   };
 
+  // whether v lies in bin b, by its distance
+  const auto in_bin = [&](float v, float far, int b) { return far >= b && (far < b + 1 || b == kSampleBins - 1) && v > -INFINITY; };
+
   Place cut{1u, 0xffffffffu};                                              // keeps all
 
   // ---- top-k -------------------------------------------------------------------------------------------------------------
@@ -286,7 +302,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       if (own < kSampleBins) atomicAdd(&s.bins[own], 1u);
       merge_bins();
       const int bin = bin_reaching(k_row);                                 // none: fewer maxima than k
-      const uint32_t n = gather([&](float v, uint32_t, uint32_t) { return bin < kSampleBins && bin_of(v) <= bin; });
+      const uint32_t n = gather([&](float, uint32_t, uint32_t) { return true; }, [&](float v) { return bin < kSampleBins && bin_of(v) <= bin; });
       listed = bin < kSampleBins && n <= kSampleList;
       if (listed) {
         // ---- all that can stay lies in CTA 0's list ----------------------------------------------------------------------------
@@ -355,20 +371,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   }
 
   // One cut in the order: by the number of what stays (k), or by its weight (below p times the weight of all that the present cut keeps).
+  int cut_bin = -1;                                                        // the bin of values in which a cut by weight over all lies
   const auto select = [&](bool mass, uint32_t k) {
+    const bool whole = cut.key == 1u;                                      // nothing is cut yet
     uint32_t low = 0, high = 0xffffffffu, above_n = 0;
     double above = 0.0, aim = 0.0;
     bool first = true;
-    int shift = 0;
+    int shift = 0, turn = mass;
     uint32_t in_n;
+    int last_bin = 0;
     // bins of the present interval: by value over all, then by key
     const auto place = [&](float v, uint32_t key) { return first ? bin_of(v) : static_cast<int>((high - key) >> shift); };
     const auto inside = [&](uint32_t key, uint32_t index) { return key != 0 && key >= low && key <= high && stays(key, index, cut); };
     while (true) {
+      if (first && whole) {
+#pragma unroll 8
+        for (int j = 0; j < its; ++j) {
+          const int b = bin_of(x[32 * j]);
+          if (b < kSampleBins) atomicAdd(&s.bins[b], 1u);
+        }
+      } else {
 #pragma unroll 4
-      for (int j = 0; j < its; ++j) {
-        const uint32_t key = key_of(x[32 * j]);
-        if (inside(key, index_of(j))) atomicAdd(&s.bins[place(x[32 * j], key)], 1u);
+        for (int j = 0; j < its; ++j) {
+          const uint32_t key = key_of(x[32 * j]);
+          if (inside(key, index_of(j))) atomicAdd(&s.bins[place(x[32 * j], key)], 1u);
+        }
       }
       merge_bins();
       for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
@@ -376,28 +403,49 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       Partial all;
       // weights above, in and below a bin of the interval
       const auto weigh_bin = [&](int b) {
-        Partial q{0.0, 0.0, 0.0, 0u, 0xffffffffu, 0u, 0u};
+        Partial q{0.0, 0.0, 0.0, 0u, 0xffffffffu, 0u, 0u};            // `all` counts only over the first interval
+        const auto note = [&](uint32_t key) {
+          ++q.count;
+          q.low = min(q.low, key);
+          q.high = max(q.high, key);
+        };
+        if (mass && first && whole) {
 #pragma unroll 4
-        for (int j = 0; j < its; ++j) {
-          const uint32_t key = key_of(x[32 * j]);
-          const bool is_in = inside(key, index_of(j));
-          const int at = is_in ? place(x[32 * j], key) : 0;
-          if (mass && __any_sync(0xffffffffu, is_in)) {
-            const double w = weigh(x[32 * j] > -INFINITY ? x[32 * j] : top);
-            if (is_in) (at < b ? q.above : at == b ? q.in : q.below) += w;
+          for (int j = 0; j < its; ++j) {
+            const float v = x[32 * j];
+            const double w = weigh(v);
+            const float far = far_of(v);
+            q.all += w;
+            if (far < b) q.above += w;
+            if (in_bin(v, far, b)) {
+              q.in += w;
+              note(key_of(v));
+            }
           }
-          if (is_in && at == b) {
-            ++q.count;
-            q.low = min(q.low, key);
-            q.high = max(q.high, key);
+        } else {
+#pragma unroll 4
+          for (int j = 0; j < its; ++j) {
+            const float v = x[32 * j];
+            const uint32_t key = key_of(v);
+            const bool is_in = inside(key, index_of(j));
+            const int at = is_in ? place(v, key) : 0;
+            if (mass && __any_sync(0xffffffffu, is_in)) {
+              const double w = weigh(v);
+              if (is_in) {
+                q.all += w;
+                if (at <= b) (at < b ? q.above : q.in) += w;
+              }
+            }
+            if (is_in && at == b) note(key);
           }
         }
-        q.above = warp_sum_d(q.above), q.in = warp_sum_d(q.in), q.below = warp_sum_d(q.below);
+        q.above = warp_sum_d(q.above), q.in = warp_sum_d(q.in), q.all = warp_sum_d(q.all);
+        if (lane == 0) s.warp_above[warp] = q.above;
         q.count = __reduce_add_sync(0xffffffffu, q.count);
         q.low = __reduce_min_sync(0xffffffffu, q.low);
         q.high = __reduce_max_sync(0xffffffffu, q.high);
         const auto join = [](Partial& x, const Partial& y) {
-          x.above += y.above, x.in += y.in, x.below += y.below, x.count += y.count;
+          x.above += y.above, x.in += y.in, x.all += y.all, x.count += y.count;
           x.low = min(x.low, y.low), x.high = max(x.high, y.high);
         };
         if (lane == 0) s.warp_part[warp] = q;
@@ -405,11 +453,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         q = s.warp_part[0];
 #pragma unroll
         for (int i = 1; i < WARPS; ++i) join(q, s.warp_part[i]);
-        if (tid < C) cluster.map_shared_rank(s.part, tid)[rank] = q;
-        cluster.sync();
-        q = s.part[0];
-        for (int i = 1; i < C; ++i) join(q, s.part[i]);
-        cluster.sync();
+        turn ^= 1;
+        if (tid < C) cluster.map_shared_rank(s.part[turn], tid)[rank] = q;
+        cluster.sync();                                                    // behind it nobody reads the parts of the call before the last
+        q = s.part[turn][0];
+        for (int i = 1; i < C; ++i) join(q, s.part[turn][i]);
         return q;
       };
       if (!mass) {
@@ -430,7 +478,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
           const int b = tid * PER + i;
           const double mid = first ? static_cast<double>(top) - (b + 0.5) / static_cast<double>(per_bin)
                                    : static_cast<double>(value_of(max(low, high - min(high - low, (static_cast<uint32_t>(b) << shift) + ((1u << shift) >> 1)))));
-          est[i] = s.total[b] ? s.total[b] * exp2(fmax((mid - static_cast<double>(top)) * c, -1000.0)) : 0.0;
+          est[i] = s.total[b] * static_cast<double>(exp2f(static_cast<float>(fmax((mid - static_cast<double>(top)) * c, -140.0))));
           sum += est[i];
         }
         const double est_before = block_scan_d(sum, s.scan_d, total) - sum;
@@ -462,7 +510,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
           __syncthreads();
           const double est_above = s.scan_d[0];
           all = weigh_bin(bin);
-          if (first) aim = fmax(p * (all.above + all.in + all.below), 1e-300);
+          if (first) aim = fmax(p * all.all, 1e-300);
           const double goal = aim - above;
           if (goal <= all.above && bin > least) most = bin - 1;             // the cut lies further up ...
           else if (goal > all.above + all.in && bin < most) least = bin + 1;     // ... or down
@@ -472,16 +520,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         above += all.above;
       }
       in_n = all.count;
+      last_bin = bin;
       low = all.low;
       high = all.high;
-      if (low >= high || in_n <= kSampleList) break;
+      if (low >= high || in_n <= kSampleList) {
+        if (mass && first && whole) cut_bin = bin;
+        break;
+      }
       first = false;
       shift = 0;
       while (((high - low) >> shift) >= static_cast<uint32_t>(kSampleBins)) ++shift;
     }
     const auto member = [&](uint32_t key, uint32_t index) { return key >= low && key <= high && stays(key, index, cut); };
     if (in_n <= kSampleList) {
-      const uint32_t n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); });
+      const bool by_bin = first && whole;
+      const uint32_t n = gather([&](float v, uint32_t key, uint32_t index) { return by_bin || member(key, index); }, [&](float v) { return !by_bin || in_bin(v, far_of(v), last_bin); });
       if (rank == 0) {
         block_sort(s.list, list_power(n));
         int last;                                                          // the last of the list that stays
@@ -540,24 +593,47 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     cluster.sync();
     cut = s.cut;
-    if (tid == 0) s.listed = 0;
-    cluster.sync();
+    if (!mass) {                                                           // the list may be wanted once more
+      if (tid == 0) s.listed = 0;
+      cluster.sync();
+    }
   };
   if (k_row > 0 && k_row < a.V) select(false, k_row);
   if (by_mass) select(true, 0);
 
   // ---- the draw ------------------------------------------------------------------------------------------------------------
+  const float low_m = m > 0.0 ? static_cast<float>(top + log2(m) / c - 1e-6 * (fabs(top) + fabs(log2(m) / c))) : -INFINITY;      // no weight below it reaches min_p
   const auto weight_of = [&](int j) {
-    const uint32_t key = key_of(x[32 * j]);
-    const bool in = key != 0 && stays(key, index_of(j), cut);
+    const float v = x[32 * j];
+    const uint32_t key = key_of(v);
+    const bool in = key != 0 && v >= low_m && stays(key, index_of(j), cut);
     if (!__any_sync(0xffffffffu, in)) return 0.0;
-    const double w = weigh(in ? x[32 * j] : top);
+    const double w = weigh(v);
     return in && w >= m ? w : 0.0;
   };
   double sum = 0.0;
+  if (cut.key == 1u && m <= 0.0) {
 #pragma unroll 4
-  for (int j = 0; j < its; ++j) sum += weight_of(j);
-  sum = warp_sum_d(sum);
+    for (int j = 0; j < its; ++j) sum += weigh(x[32 * j]);
+    sum = warp_sum_d(sum);
+    if (sum < 1e-200) sum = 0.0;                                           // nothing but what is never chosen
+  } else if (cut_bin >= 0 && m <= 0.0) {
+    // what lies above the cut's bin has been summed up
+#pragma unroll 4
+    for (int j = 0; j < its; ++j) {
+      const float v = x[32 * j];
+      const bool in = in_bin(v, far_of(v), cut_bin);
+      if (__any_sync(0xffffffffu, in)) {
+        const double w = weigh(v);
+        if (in && stays(key_of(v), index_of(j), cut)) sum += w;
+      }
+    }
+    sum = warp_sum_d(sum) + s.warp_above[warp];
+  } else {
+#pragma unroll 4
+    for (int j = 0; j < its; ++j) sum += weight_of(j);
+    sum = warp_sum_d(sum);
+  }
   if (lane < C) cluster.map_shared_rank(s.warp_sums, lane)[rank * WARPS + warp] = sum;
   cluster.sync();
   // the warp in which the cumulative weight passes the aim, else the last that holds any
@@ -580,14 +656,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   before_at = __shfl_sync(0xffffffffu, first_past == 0xffffffffu ? before_last : before_at, at / each);
   if (at == rank * WARPS + warp) {
     double upto = before_at;
-    uint32_t chosen = 0, found = 0;
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) {
-      const double w = weight_of(j), c_j = upto + warp_scan_d(w, lane);
-      const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0), past = __ballot_sync(0xffffffffu, w > 0.0 && c_j > aim);
-      if (!found && any) chosen = __shfl_sync(0xffffffffu, index_of(j), past ? __ffs(past) - 1 : 31 - __clz(any));
-      found |= past;
-      upto = __shfl_sync(0xffffffffu, c_j, 31);
+    uint32_t chosen = 0;
+    bool found = false;
+    for (int j0 = 0; j0 < its && !found; j0 += 4) {                        // four at a time hide each other's latency
+      double w[4], of[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = j0 + i < its ? weight_of(j0 + i) : 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) of[i] = warp_sum_d(w[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (found || !(of[i] > 0.0)) continue;
+        const double c_i = upto + warp_scan_d(w[i], lane);
+        const uint32_t any = __ballot_sync(0xffffffffu, w[i] > 0.0), past = __ballot_sync(0xffffffffu, w[i] > 0.0 && c_i > aim);
+        chosen = __shfl_sync(0xffffffffu, index_of(j0 + i), past ? __ffs(past) - 1 : 31 - __clz(any));
+        found = past != 0;
+        upto += of[i];
+      }
     }
     if (lane == 0) a.token[row] = chosen;
   }
