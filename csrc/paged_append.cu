@@ -42,8 +42,7 @@ template <> struct Pair<__half> {
 };
 
 template <typename T>
-__device__ __forceinline__ void pa_load8(const T* p, float (&f)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void pa_unpack8(const uint4& u, float (&f)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -51,6 +50,9 @@ __device__ __forceinline__ void pa_load8(const T* p, float (&f)[8]) {
     f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
 }
+__device__ __forceinline__ uint4 pa_raw8(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+template <typename T>
+__device__ __forceinline__ void pa_load8(const T* p, float (&f)[8]) { pa_unpack8<T>(pa_raw8(p), f); }
 template <typename T>
 __device__ __forceinline__ void pa_store8(T* p, const float (&f)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::put(f[0], f[1]), Pair<T>::put(f[2], f[3]), Pair<T>::put(f[4], f[5]), Pair<T>::put(f[6], f[7]));
@@ -225,8 +227,10 @@ __device__ __forceinline__ int pa_step_of(int n, long long x, F bound) {
 // Units of a call's pages: sequence b has those from starts[b] / P + 2 b on; its rows touch at most (n - 2) / P + 2 pages.
 __device__ __forceinline__ long long pa_first_unit(const PagedAppendArgs& a, int b) { return static_cast<long long>(a.starts[b]) / a.P + 2LL * b; }
 
+constexpr int kQueryHeads = 8;             // of a row that D / 8 lanes take, four at a time: the rotation is read once for them
+
 // One block per (page, head, keys or values) holds the page's new rows in registers between the maximum and the codes, IT vectors a thread; after the
-// `page_units` of them, blocks of 8 rows for the queries.
+// `page_units` of them, blocks for the queries.
 template <typename T, bool F8, int IT>
 __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int page_units) {
   pdl_entry();
@@ -234,26 +238,30 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
   const int groups = blockDim.x / hl.lanes, group = threadIdx.x / hl.lanes;
   __shared__ uint32_t s_max[16];
   if (static_cast<int>(blockIdx.x) >= page_units) {
-    const int row0 = (static_cast<int>(blockIdx.x) - page_units) * 8;
-    int b = pa_step_of(a.B, row0, [&](int i) { return static_cast<long long>(a.starts[i]); });
-    int at = -1;
-    NewRows nr{0, 0, 0};
-    for (int i = group; i < 8 * a.H; i += groups) {
-      const int row = row0 + i / a.H, h = i % a.H;
-      if (row >= a.rows) break;
-      if (row != at) {
-        at = row;
-        while (b + 1 < a.B && a.starts[b + 1] <= row) ++b;
-        nr = pa_new_rows(a, b);
-        if (row >= nr.row && row < nr.row + nr.n) hl.turns(a, nr.first + row - nr.row);
+    const int chunks = (a.H + kQueryHeads - 1) / kQueryHeads;
+    const long long item0 = (static_cast<long long>(blockIdx.x) - page_units) * groups, item = item0 + group;
+    const int row = static_cast<int>(item / chunks), h0 = static_cast<int>(item % chunks) * kQueryHeads;
+    int b = pa_step_of(a.B, item0 / chunks, [&](int i) { return static_cast<long long>(a.starts[i]); });
+    if (row >= a.rows) return;
+    while (b + 1 < a.B && a.starts[b + 1] <= row) ++b;
+    const NewRows nr = pa_new_rows(a, b);
+    const bool there = row >= nr.row && row < nr.row + nr.n;
+    if (there) hl.turns(a, nr.first + row - nr.row);
+    const T* src = static_cast<const T*>(a.q) + row * a.q_row + hl.l8;
+    T* dst = static_cast<T*>(a.q_out) + static_cast<long long>(row) * a.H * a.D + hl.l8;
+#pragma unroll
+    for (int h = h0; h < h0 + kQueryHeads; h += 4) {
+      uint4 raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = there && h + i < a.H ? pa_raw8(src + (h + i) * a.q_head) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (h + i >= a.H) break;
+        float f[8];
+        pa_unpack8<T>(raw[i], f);
+        if (there) hl.finish(a, static_cast<const T*>(a.q_weight), f);
+        pa_store8(dst + (h + i) * a.D, f);
       }
-      T* q_out = static_cast<T*>(a.q_out) + (static_cast<long long>(row) * a.H + h) * a.D + hl.l8;
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row >= nr.row && row < nr.row + nr.n) {
-        pa_load8(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head + hl.l8, f);
-        hl.finish(a, static_cast<const T*>(a.q_weight), f);
-      }
-      pa_store8(q_out, f);
     }
     return;
   }
@@ -271,14 +279,17 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
   const int slot0 = lo - static_cast<int>(j) * a.P, row0 = nr.row + lo - nr.first, n = hi - lo;
   float f[IT][8];
   uint32_t m = 0;
+  const T* src = is_v ? static_cast<const T*>(a.v) + row0 * a.v_row + hd * a.v_head + hl.l8 : static_cast<const T*>(a.k) + row0 * a.k_row + hd * a.k_head + hl.l8;
+  const long long step = is_v ? a.v_row : a.k_row;
+  uint4 raw[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) raw[it] = it * groups + group < n ? pa_raw8(src + (it * groups + group) * step) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int i = it * groups + group;
+    pa_unpack8<T>(raw[it], f[it]);
     if (i < n) {
-      if (is_v) {
-        pa_load8(static_cast<const T*>(a.v) + (row0 + i) * a.v_row + hd * a.v_head + hl.l8, f[it]);
-      } else {
-        pa_load8(static_cast<const T*>(a.k) + (row0 + i) * a.k_row + hd * a.k_head + hl.l8, f[it]);
+      if (!is_v) {
         hl.turns(a, lo + i);
         hl.finish(a, static_cast<const T*>(a.k_weight), f[it]);
       }
@@ -326,11 +337,11 @@ int paged_append_launch(const PagedAppendArgs& a, cudaStream_t stream) {
     const long long units = static_cast<long long>(a.B) * (a.H + 2 * a.G);
     return (int)launch_dependent(paged_append_step_kernel<T, F8>, dim3(static_cast<unsigned>((units * lanes + 127) / 128)), dim3(128), 0, stream, a);
   }
-  // every sequence takes rows / P + 2 units at most, and no more pages are touched than there are rows
+  // every sequence takes rows / P + 2 units at most
+  const int vectors = a.P * lanes, threads = vectors > 2048 ? 512 : vectors > 128 ? 256 : 128;
   const long long units = (static_cast<long long>(a.rows) / a.P + 2LL * a.B) * 2 * a.G;
-  const long long blocks = units + (a.q ? (a.rows + 7) / 8 : 0);
+  const long long queries = a.q ? static_cast<long long>(a.rows) * ((a.H + kQueryHeads - 1) / kQueryHeads) : 0, blocks = units + (queries + threads / lanes - 1) / (threads / lanes);
   if (blocks > 0x7fffffffLL) return -5;
-  const int vectors = a.P * lanes, threads = vectors > 2048 ? 512 : vectors > 128 ? 256 : vectors < 64 ? 64 : 128;
   const dim3 grid(static_cast<unsigned>(blocks)), block(threads);
   const int u = static_cast<int>(units);
   switch ((vectors + threads - 1) / threads) {

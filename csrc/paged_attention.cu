@@ -37,11 +37,12 @@ struct PagedAttnArgs {
   const void *k_pages, *v_pages;               // [pages, G, P, D]
   const float *k_scale, *v_scale;              // [pages, G] (null: 16-bit pages)
   const int *table, *lengths, *starts;         // [B, width], [B], [B + 1] (nullable)
-  float* part;                                 // workspace (see part_floats)
+  float* part;                                 // workspace (see part_stats)
   int* err;
   long long q_row, q_head, table_row;
   int rows, B, H, G, D, P, pages, width, window, whole;
   float scale;
+  int ctas;                                    // shares of the work that `part` has room for (not read where shares are whole items)
 };
 static_assert(sizeof(PagedAttnArgs) == 160, "as ops/paged_cache.py packs it");
 
@@ -212,8 +213,7 @@ __device__ __forceinline__ float pt_exp2(float x) {
   return y;
 }
 
-// Floats of the workspace for `ctas` shares: heads of split items, then two pieces a share of ROWS rows: {m, l, M, -} and D sums each.
-__host__ __device__ inline long long part_floats(int ctas, int rows, int D) { return static_cast<long long>(ctas) * (8 + 2LL * rows * (4 + D)); }
+// The workspace holds, for each of `ctas` shares, the head of its split item (8 floats) and two pieces of ROWS rows: {m, l, M, -} and D sums each.
 __device__ __forceinline__ float* part_stats(const PagedAttnArgs& a, int ctas, int rows, int piece) { return a.part + ctas * 8LL + static_cast<long long>(piece) * rows * 4; }
 __device__ __forceinline__ float* part_sums(const PagedAttnArgs& a, int ctas, int rows, int piece) {
   return a.part + ctas * 8LL + 2LL * ctas * rows * 4 + static_cast<long long>(piece) * rows * a.D;
@@ -746,87 +746,79 @@ int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
   return r == CUDA_SUCCESS ? 0 : 4000 + static_cast<int>(r);
 }
 
-template <typename T, bool F8, int D, int ROWS, int NR>
-struct PagedLaunch {
-  using TL = Tile<F8, D>;
-  static constexpr int kSmem = 1024 + TL::kStages * (2 * TL::kSize + 32 + 16) + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * D * 4 : 0);
-  // CTAs that the device holds at once
-  static int resident() {
-    static const int n = [] {
-      const auto kernel = paged_attention_kernel<T, F8, D, ROWS, NR>;
-      int per = 0, dev = 0, sms = 0;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return 0;
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, (kWarps + 1) * 32, kSmem) != cudaSuccess) return 0;
-      if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-      return per * sms;
-    }();
-    return n;
-  }
-  static int ctas(const PagedAttnArgs& a) {
-    const int R = a.H / a.G;
-    const long long row_tiles = a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS);
-    const long long tiles = a.whole ? 1 : (static_cast<long long>(a.width) * a.P + kKeys - 1) / kKeys;
-    const long long most = row_tiles * a.G * tiles, n = resident();
-    return static_cast<int>(most < n ? most : n);
-  }
-  static int run(const PagedAttnArgs& a, cudaStream_t stream) {
-    CUtensorMap mk, mv;
-    int r = page_map<F8, D>(&mk, a.k_pages, a);
-    if (r == 0) r = page_map<F8, D>(&mv, a.v_pages, a);
-    if (r != 0) return r;
-    const int n = ctas(a);
-    if (n <= 0) return -21;
-    cudaError_t e = launch_dependent(paged_attention_kernel<T, F8, D, ROWS, NR>, dim3(n), dim3((kWarps + 1) * 32), kSmem, stream, a, mk, mv);
-    if (e != cudaSuccess || a.whole) return static_cast<int>(e);
-    const int R = a.H / a.G, rows = a.starts ? 16 : (R < ROWS ? R : ROWS);
-    return static_cast<int>(launch_dependent(paged_attention_join_kernel<T, ROWS>, dim3(n, rows), dim3(128), 0, stream, a, n));
-  }
+// What to do with a form of the kernel: launch it, or say how many of its CTAs the device holds at once.
+struct PagedCall {
+  const PagedAttnArgs* a;
+  cudaStream_t stream;
 };
 
-// Floats of workspace (`floats` given) or the launches.
-template <typename T, bool F8, int D>
-int paged_form(const PagedAttnArgs& a, int rows, cudaStream_t stream, long long* floats) {
+template <typename T, bool F8, int D, int ROWS, int NR>
+int paged_form(const PagedCall& call) {
+  using TL = Tile<F8, D>;
+  constexpr int kSmem = 1024 + TL::kStages * (2 * TL::kSize + 32 + 16) + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * D * 4 : 0);
+  const auto kernel = paged_attention_kernel<T, F8, D, ROWS, NR>;
+  static const cudaError_t ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (ready != cudaSuccess) return -30;
+  if (call.a == nullptr) {
+    int per = 0, dev = 0, sms = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, (kWarps + 1) * 32, kSmem) != cudaSuccess) return -31;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -32;
+    return per * sms;
+  }
+  const PagedAttnArgs& a = *call.a;
+  CUtensorMap mk, mv;
+  int r = page_map<F8, D>(&mk, a.k_pages, a);
+  if (r == 0) r = page_map<F8, D>(&mv, a.v_pages, a);
+  if (r != 0) return r;
   const int R = a.H / a.G;
-  if (rows == 64) {
-    using L = PagedLaunch<T, F8, D, 64, 2>;
-    if (floats) return *floats = part_floats(L::ctas(a), 64, D), 0;
-    return L::run(a, stream);
-  }
-  if (a.starts == nullptr && R <= 8) {
-    using L = PagedLaunch<T, F8, D, 16, 1>;
-    if (floats) return *floats = part_floats(L::ctas(a), 16, D), 0;
-    return L::run(a, stream);
-  }
-  using L = PagedLaunch<T, F8, D, 16, 2>;
-  if (floats) return *floats = part_floats(L::ctas(a), 16, D), 0;
-  return L::run(a, stream);
+  const long long items = (a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS)) * a.G;
+  // whole items are dealt out evenly too
+  const int n = a.whole ? static_cast<int>(items < 148 * 8 ? items : 148 * 8) : a.ctas;
+  if (n <= 0) return -21;
+  const cudaError_t e = launch_dependent(kernel, dim3(n), dim3((kWarps + 1) * 32), kSmem, call.stream, a, mk, mv);
+  if (e != cudaSuccess || a.whole) return static_cast<int>(e);
+  return static_cast<int>(launch_dependent(paged_attention_join_kernel<T, ROWS>, dim3(n, a.starts ? 16 : (R < ROWS ? R : ROWS)), dim3(128), 0, call.stream, a, n));
+}
+
+template <typename T, bool F8, int D>
+int paged_rows(const PagedCall& call, int rows, bool few) {
+  if (rows == 64) return paged_form<T, F8, D, 64, 2>(call);
+  return few ? paged_form<T, F8, D, 16, 1>(call) : paged_form<T, F8, D, 16, 2>(call);
 }
 template <typename T, bool F8>
-int paged_dim(const PagedAttnArgs& a, int rows, cudaStream_t stream, long long* floats) {
-  switch (a.D) {
-    case 64: return paged_form<T, F8, 64>(a, rows, stream, floats);
-    case 128: return paged_form<T, F8, 128>(a, rows, stream, floats);
-    case 256: return paged_form<T, F8, 256>(a, rows, stream, floats);
+int paged_dim(const PagedCall& call, int D, int rows, bool few) {
+  switch (D) {
+    case 64: return paged_rows<T, F8, 64>(call, rows, few);
+    case 128: return paged_rows<T, F8, 128>(call, rows, few);
+    case 256: return paged_rows<T, F8, 256>(call, rows, few);
   }
   return -2;
+}
+int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool few) {
+  if (rows != 16 && rows != 64) return -3;
+  if (dtype == 0) return f8 ? paged_dim<__nv_bfloat16, true>(call, D, rows, few) : paged_dim<__nv_bfloat16, false>(call, D, rows, few);
+  if (dtype == 1) return f8 ? paged_dim<__half, true>(call, D, rows, few) : paged_dim<__half, false>(call, D, rows, few);
+  return -6;
 }
 
 }  // namespace tyr
 
 using namespace tyr;
 
-// dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows: 16 or 64 of a tile.  With `floats` only the workspace is asked for.
-extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int rows, void* stream, long long* floats) {
+// dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows: 16 or 64 of a tile.
+extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int rows, void* stream) {
   const PagedAttnArgs& a = *static_cast<const PagedAttnArgs*>(packed);
   if (a.rows <= 0 || a.B <= 0 || a.H <= 0 || a.G <= 0 || a.H % a.G != 0 || a.pages <= 0 || a.width <= 0 || a.window < 0) return -1;
   if (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) return -2;
-  if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64)) return -3;
+  if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64) || (!a.whole && (a.part == nullptr || a.ctas <= 0))) return -3;
   // a sequence's work and the pages' rows are counted in 32 bits
   const long long tiles = (static_cast<long long>(a.width) * a.P + kKeys - 1) / kKeys;
   if ((static_cast<long long>(a.rows) * (a.H / a.G) / rows + 1) * a.G * tiles > 0x7fffffffLL || static_cast<long long>(a.pages) * a.G > 0x7fffffffLL) return -4;
   if (static_cast<long long>(a.width) * a.P > 0x7fffffffLL || static_cast<long long>(a.rows) * a.H > 0x7fffffffLL) return -5;
-  const bool f8 = a.k_scale != nullptr;
-  if (dtype == 0) return f8 ? paged_dim<__nv_bfloat16, true>(a, rows, (cudaStream_t)stream, floats) : paged_dim<__nv_bfloat16, false>(a, rows, (cudaStream_t)stream, floats);
-  if (dtype == 1) return f8 ? paged_dim<__half, true>(a, rows, (cudaStream_t)stream, floats) : paged_dim<__half, false>(a, rows, (cudaStream_t)stream, floats);
-  return -6;
+  return paged_type(PagedCall{&a, (cudaStream_t)stream}, dtype, a.k_scale != nullptr, a.D, rows, a.starts == nullptr && a.H / a.G <= 8);
+}
+
+// CTAs of a form that the current device holds at once (few: at most 8 rows in a tile of 16); negative: an error.
+extern "C" TYR_EXPORT int tyr_paged_attention_resident(int dtype, int f8, int D, int rows, int few) {
+  return paged_type(PagedCall{nullptr, nullptr}, dtype, f8 != 0, D, rows, few != 0);
 }

@@ -9,6 +9,7 @@ from tyr_b200.ops import paged_cache as pc
 from tyr_b200.ops.paged_cache import PagedStore, paged_append, paged_attention
 
 F64 = torch.float64
+FIELDS = ("k", "v", "k_scale", "v_scale")
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24, torch.float8_e4m3fn: 2.0 ** -4}
 
 
@@ -64,10 +65,10 @@ class Batch:
         to = lambda t: None if t is None else t.to(dev)
         self.q, self.k, self.v, self.table, starts = to(self.q), to(self.k), to(self.v), to(self.table), to(starts)
         self.args = (self.table, torch.tensor(self.lens, dtype=torch.int32, device=dev), starts)
-        self.store = PagedStore(*(to(getattr(self.store, n)) for n in PagedStore.__slots__))
+        self.store = PagedStore(*(to(getattr(self.store, n)) for n in FIELDS))
 
     def copy(self):
-        return PagedStore(*(None if getattr(self.store, n) is None else getattr(self.store, n).clone() for n in PagedStore.__slots__))
+        return PagedStore(*(None if getattr(self.store, n) is None else getattr(self.store, n).clone() for n in FIELDS))
 
     def sequence(self, b, store=None):
         """(keys, values) [G, length, D] of sequence b in 64 bits."""

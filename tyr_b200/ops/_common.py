@@ -23,7 +23,7 @@ def ptr(t):
 def cur_stream(device=None):
     """Current torch stream of ``device`` as a raw handle.  Also binds that device to the calling
     host thread inside the kernel library (autograd worker threads start without one)."""
-    idx = torch.device(device).index if device is not None else None
+    idx = None if device is None else device.index if type(device) is torch.device else torch.device(device).index
     if idx is None:
         idx = torch.cuda.current_device()
     rc = kernels().tyr_bind_device(idx)
@@ -40,7 +40,7 @@ def check(rc: int, what: str):
 
 def err_word(device) -> torch.Tensor:
     """Per-device int32[4] record {code, block, detail, spare} written by kernels on a timeout."""
-    idx = torch.device(device).index
+    idx = device.index if type(device) is torch.device else torch.device(device).index
     if idx is None:
         idx = torch.cuda.current_device()
     w = _err_words.get(idx)

@@ -11,6 +11,7 @@ On the GPU, operands that do not go together (a page outside the cache, a length
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import List, Optional, Tuple
@@ -18,7 +19,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from .._native import register_signatures
-from ._common import check, cur_stream, err_word, lib, ptr
+from ._common import check, cur_stream, err_word, lib
 
 E4M3 = torch.float8_e4m3fn
 LARGEST = 448.0                     # of e4m3
@@ -36,32 +37,33 @@ def _sigs(lib_):
     if hasattr(lib_, "tyr_paged_append"):
         lib_.tyr_paged_append.argtypes, lib_.tyr_paged_append.restype = [P, I, P], I
     if hasattr(lib_, "tyr_paged_attention"):
-        lib_.tyr_paged_attention.argtypes, lib_.tyr_paged_attention.restype = [P, I, I, P, ctypes.POINTER(ctypes.c_longlong)], I
+        lib_.tyr_paged_attention.argtypes, lib_.tyr_paged_attention.restype = [P, I, I, P], I
+        lib_.tyr_paged_attention_resident.argtypes, lib_.tyr_paged_attention_resident.restype = [I] * 5, I
 
 
 # the kernels' argument blocks, as csrc/paged_append.cu and csrc/paged_attention.cu declare them
 _APPEND = struct.Struct("@16Q7q11if0q")
-_ATTEND = struct.Struct("@11Q3q10if0q")
+_ATTEND = struct.Struct("@11Q3q10ifi0q")
 
 
 class PagedStore:
     """The pages of one layer: ``k`` and ``v`` [pages, kv heads, page, head size] in e4m3, bf16 or fp16, and the scales [pages, kv heads] of e4m3 pages."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "shape", "index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
-        shape, dtype = k.shape, k.dtype
-        if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.device != k.device or not (k.is_contiguous() and v.is_contiguous()):
+        shape, dtype, dev = k.shape, k.dtype, k.get_device()
+        if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.get_device() != dev or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("paged store: k and v are contiguous [pages, kv heads, page, head size] of one type and device")
         if (dtype == E4M3) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
             raise ValueError("paged store: e4m3 pages need k_scale and v_scale, other pages have none")
         if k_scale is not None:
             for s in (k_scale, v_scale):
-                if s.shape != shape[:2] or s.dtype != torch.float32 or not s.is_contiguous() or s.device != k.device:
+                if s.shape != shape[:2] or s.dtype != torch.float32 or not s.is_contiguous() or s.get_device() != dev:
                     raise ValueError("paged store: scales are contiguous fp32 [pages, kv heads] beside the pages")
-        elif dtype not in (torch.bfloat16, torch.float16) and k.is_cuda or not dtype.is_floating_point:
+        elif dev >= 0 and dtype not in _DTYPES or not dtype.is_floating_point:
             raise ValueError(f"paged store: pages in {dtype} are not supported")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale, self.shape, self.index = k, v, k_scale, v_scale, tuple(shape), dev
 
     @staticmethod
     def allocate(pages: int, kv_heads: int, page: int, head_dim: int, device, dtype: torch.dtype = E4M3) -> "PagedStore":
@@ -74,7 +76,7 @@ class PagedStore:
 
     @property
     def page(self) -> int:
-        return self.k.shape[2]
+        return self.shape[2]
 
     def values(self, pages: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """What these pages hold, fp32 [len(pages), kv heads, page, head size] of the keys and of the values."""
@@ -87,25 +89,29 @@ class PagedStore:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
 
-def _together(what: str, store: PagedStore, rows: int, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor]) -> None:
-    B = lengths.shape[0]
-    if lengths.dim() != 1 or B == 0 or lengths.dtype != torch.int32 or lengths.stride(0) != 1:
+def _together(what: str, store: PagedStore, rows: int, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor]) -> Tuple[int, int, int]:
+    """(sequences, pages of a row of the table, elements between its rows)."""
+    shape, stride, size = table.shape, table.stride(), lengths.shape
+    if len(size) != 1 or size[0] == 0 or lengths.dtype != torch.int32 or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths are contiguous int32 [sequences]")
-    if table.dim() != 2 or table.shape[0] != B or table.shape[1] == 0 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+    B = size[0]
+    if len(shape) != 2 or shape[0] != B or shape[1] == 0 or table.dtype != torch.int32 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what}: the table is int32 [sequences, pages] with contiguous rows")
     if starts is None:
         if rows != B:
             raise ValueError(f"{what}: {rows} rows for {B} sequences need starts")
-    elif starts.dim() != 1 or starts.shape[0] != B + 1 or starts.dtype != torch.int32 or starts.stride(0) != 1:
+    elif starts.shape != (B + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous():
         raise ValueError(f"{what}: starts are contiguous int32 [sequences + 1]")
-    dev = store.k.device
-    if table.device != dev or lengths.device != dev or (starts is not None and starts.device != dev):
+    dev = store.index
+    if table.get_device() != dev or lengths.get_device() != dev or (starts is not None and starts.get_device() != dev):
         raise ValueError(f"{what}: store, table, lengths and starts lie on different devices")
+    return B, shape[1], stride[0]
 
 
 def _on_gpu(what: str, store: PagedStore, dtype: torch.dtype) -> int:
     """The kernels' number of the operands' type; refuses what they do not serve."""
-    D, P, number = store.k.shape[3], store.k.shape[2], _DTYPES.get(dtype)
+    _, _, P, D = store.shape
+    number = _DTYPES.get(dtype)
     if number is None or (store.k_scale is None and store.k.dtype != dtype):
         raise ValueError(f"{what}: operands in {dtype} over pages in {store.k.dtype} are not supported")
     if D not in HEAD_SIZES or P not in PAGE_SIZES:
@@ -117,7 +123,8 @@ def _on_gpu(what: str, store: PagedStore, dtype: torch.dtype) -> int:
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, heads, D] as the kernels read it: whole heads, 16-byte aligned."""
-    return t if t.stride(2) == 1 and (t.stride(0) | t.stride(1)) & 7 == 0 and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
+    row, head, one = t.stride()
+    return t if one == 1 and (row | head) & 7 == 0 and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -205,48 +212,61 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     e4m3 pages: the scale of a (page, head) is the smallest power of two, 2^-100 at least, that keeps its largest magnitude within 448.  It grows with later tokens of
     the page, whose older codes are rescaled (exactly, unless they leave e4m3's normal range); the first slot of a page starts it anew.  A value that is not finite
     makes it NaN until then, and so the attention of all that sees the page."""
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != store.k.shape[1] or k.shape[2] != store.k.shape[3] or k.shape[0] == 0:
-        raise ValueError(f"paged_append: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit pages {tuple(store.k.shape)}")
-    rows, G, D = k.shape
-    dev = store.k.device
-    if k.device != dev or v.device != dev:
+    pages, G, P, D = store.shape
+    shape, dtype, dev = k.shape, k.dtype, store.index
+    if len(shape) != 3 or v.shape != shape or v.dtype != dtype or shape[1] != G or shape[2] != D or shape[0] == 0:
+        raise ValueError(f"paged_append: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit pages {store.shape}")
+    rows = shape[0]
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("paged_append: k, v and the store lie on different devices")
-    _together("paged_append", store, rows, table, lengths, starts)
-    if q is not None and (q.dim() != 3 or q.shape[0] != rows or q.shape[2] != D or q.shape[1] == 0 or q.dtype != k.dtype or q.device != dev):
-        raise ValueError(f"paged_append: queries {tuple(q.shape)} do not fit keys {tuple(k.shape)}")
+    B, width, table_row = _together("paged_append", store, rows, table, lengths, starts)
+    H = 0
+    if q is not None:
+        size = q.shape
+        if len(size) != 3 or size[0] != rows or size[2] != D or size[1] == 0 or q.dtype != dtype or q.get_device() != dev:
+            raise ValueError(f"paged_append: queries {tuple(size)} do not fit keys {tuple(shape)}")
+        H = size[1]
     if (cos is None) != (sin is None):
         raise ValueError("paged_append: cos and sin go together")
-    half = 0
+    half = positions = 0
     if cos is not None:
-        half = cos.shape[-1]
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] == 0 or half == 0 or 2 * half > D or cos.device != dev or sin.device != dev:
-            raise ValueError(f"paged_append: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} do not fit heads of {D}")
+        size = cos.shape
+        if len(size) != 2 or sin.shape != size or size[0] == 0 or size[1] == 0 or 2 * size[1] > D or cos.get_device() != dev or sin.get_device() != dev:
+            raise ValueError(f"paged_append: cos {tuple(size)} and sin {tuple(sin.shape)} do not fit heads of {D}")
+        positions, half = size
     for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (D,) or w.device != dev):
+        if w is not None and (w.shape != (D,) or w.get_device() != dev):
             raise ValueError(f"paged_append: norm weights are [{D}] beside the pages")
-    if not k.is_cuda:
+    if dev < 0:
         return _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w)
-    number = _on_gpu("paged_append", store, k.dtype)
+    number = _on_gpu("paged_append", store, dtype)
     if half % 8:
         raise ValueError(f"paged_append: the rotation turns a multiple of 16 channels, got {2 * half}")
     k, v = _rows_of(k), _rows_of(v)
-    tables, weights = (), (None, None)
     if half:
-        tables = tuple(t if t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() & 15 == 0 else _aligned(t.float()) for t in (cos, sin))
-    if q_weight is not None or k_weight is not None:
-        weights = tuple(None if w is None else _aligned(w.to(k.dtype)) for w in (q_weight, k_weight))
-    out, H, q_at, out_at, q_row, q_head = None, 0, 0, 0, 0, 0
+        cos, sin = (t if t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() & 15 == 0 else _aligned(t.float()) for t in (cos, sin))
+    q_weight, k_weight = (None if w is None else _aligned(w.to(dtype)) for w in (q_weight, k_weight))
+    device, out, q_stride = k.device, None, (0, 0)
     if q is not None:
-        q, H = _rows_of(q), q.shape[1]
-        out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
-        q_at, out_at, q_row, q_head = q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1)
+        q = _rows_of(q)
+        out, q_stride = torch.empty((rows, H, D), dtype=dtype, device=device), q.stride()
+    k_stride, v_stride = k.stride(), v.stride()
     at = lambda t: 0 if t is None else t.data_ptr()
-    packed = _APPEND.pack(q_at, k.data_ptr(), v.data_ptr(), out_at, store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(),
-                          lengths.data_ptr(), at(starts), tables[0].data_ptr() if half else 0, tables[1].data_ptr() if half else 0, at(weights[0]), at(weights[1]),
-                          err_word(dev).data_ptr(), q_row, q_head, k.stride(0), k.stride(1), v.stride(0), v.stride(1), table.stride(0),
-                          rows, lengths.shape[0], H, G, D, store.k.shape[2], store.k.shape[0], table.shape[1], cos.shape[0] if half else 0, half, int(one_plus_w), eps)
-    check(lib().tyr_paged_append(packed, number, cur_stream(dev)), "paged_append")
+    packed = _APPEND.pack(at(q), k.data_ptr(), v.data_ptr(), at(out), store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(),
+                          lengths.data_ptr(), at(starts), at(cos), at(sin), at(q_weight), at(k_weight), err_word(device).data_ptr(), q_stride[0], q_stride[1], k_stride[0],
+                          k_stride[1], v_stride[0], v_stride[1], table_row, rows, B, H, G, D, P, pages, width, positions, half, one_plus_w, eps)
+    check(lib().tyr_paged_append(packed, number, cur_stream(device)), "paged_append")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _resident(index: int, number: int, f8: bool, D: int, tile: int, few: bool) -> int:
+    """CTAs of a form of the kernel that device ``index`` holds at once: the shares that a call's work is cut into."""
+    cur_stream(torch.device("cuda", index))
+    n = lib().tyr_paged_attention_resident(number, f8, D, tile, few)
+    if n <= 0:
+        raise RuntimeError(f"tyr_b200 native call paged_attention_resident failed with code {n}")
+    return n
 
 
 def _attend_ref(q, store, table, lengths, starts, window, scale):
@@ -270,32 +290,31 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
                     window: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
     """Attention of the new tokens' queries ``[rows, heads, D]`` over their sequences' pages, which hold the new tokens already -> ``[rows, heads, D]``; rows of no
     sequence come back as zeros.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
-    if q.dim() != 3 or q.shape[0] == 0 or q.shape[2] != store.k.shape[3] or q.shape[1] == 0 or q.shape[1] % store.k.shape[1] or q.device != store.k.device:
-        raise ValueError(f"paged_attention: queries {tuple(q.shape)} on {q.device} do not fit pages {tuple(store.k.shape)} on {store.k.device}")
-    rows, H, D = q.shape
+    pages, G, P, D = store.shape
+    shape = q.shape
+    if len(shape) != 3 or shape[0] == 0 or shape[2] != D or shape[1] == 0 or shape[1] % G or q.get_device() != store.index:
+        raise ValueError(f"paged_attention: queries {tuple(shape)} on {q.device} do not fit pages {store.shape} on {store.k.device}")
+    rows, H, _ = shape
     if window is not None and window <= 0:
         raise ValueError(f"paged_attention: the window must be positive, got {window}")
-    _together("paged_attention", store, rows, table, lengths, starts)
+    B, width, table_row = _together("paged_attention", store, rows, table, lengths, starts)
     scale = 1.0 / math.sqrt(D) if scale is None else scale
-    if not q.is_cuda:
+    if store.index < 0:
         return _attend_ref(q, store, table, lengths, starts, window, scale)
-    number = _on_gpu("paged_attention", store, q.dtype)
-    q, B = _rows_of(q), lengths.shape[0]
-    pages, G, P, _ = store.k.shape
-    dev, width = q.device, table.shape[1]
-    out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
-    tile = 64 if starts is not None and rows * (H // G) > 16 * B else 16
+    dtype, device = q.dtype, q.device
+    number = _on_gpu("paged_attention", store, dtype)
+    q, f8 = _rows_of(q), store.k_scale is not None
+    stride, R = q.stride(), H // G
+    out = torch.empty((rows, H, D), dtype=dtype, device=device)
+    tile = 64 if starts is not None and rows * R > 16 * B else 16
     whole = width * P <= WHOLE_MAX_KEYS
-    at = lambda t: 0 if t is None else t.data_ptr()
-    tail = (rows, B, H, G, D, P, pages, width, min(window or 0, 2 ** 30), int(whole), scale)
-    head = (q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(), lengths.data_ptr(), at(starts))
-    mid = (err_word(dev).data_ptr(), q.stride(0), q.stride(1), table.stride(0))
-    stream = cur_stream(dev)
-    work, floats = None, ctypes.c_longlong(0)
+    work = None
     if not whole:
-        rc = lib().tyr_paged_attention(_ATTEND.pack(*head, 0, *mid, *tail), number, tile, stream, ctypes.byref(floats))
-        if rc != 0:
-            raise RuntimeError(f"tyr_b200 native call paged_attention failed with code {rc}")
-        work = torch.empty(floats.value, dtype=torch.float32, device=dev)
-    check(lib().tyr_paged_attention(_ATTEND.pack(*head, at(work), *mid, *tail), number, tile, stream, None), "paged_attention")
+        row_tiles = rows * R // tile + B if starts is not None else B * -(-R // tile)
+        ctas = min(row_tiles * G * -(-width * P // 64), _resident(store.index, number, f8, D, tile, starts is None and R <= 8))
+        work = torch.empty(ctas * (8 + 2 * tile * (4 + D)), dtype=torch.float32, device=device)
+    packed = _ATTEND.pack(q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), store.k_scale.data_ptr() if f8 else 0, store.v_scale.data_ptr() if f8 else 0,
+                          table.data_ptr(), lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if whole else work.data_ptr(), err_word(device).data_ptr(),
+                          stride[0], stride[1], table_row, rows, B, H, G, D, P, pages, width, min(window or 0, 2 ** 30), whole, scale, 0 if whole else ctas)
+    check(lib().tyr_paged_attention(packed, number, tile, cur_stream(device)), "paged_attention")
     return out

@@ -28,11 +28,11 @@ def _sigs(lib_):
         lib_.tyr_sample.argtypes, lib_.tyr_sample.restype = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p], ctypes.c_int
 
 
-def _setting(name: str, v, logits: torch.Tensor, dtype: torch.dtype, least: float):
+def _setting(name: str, v, rows: int, dev: int, dtype: torch.dtype, least: float):
     """(address, number) of a setting: a tensor with one number a row, or one for all."""
     if isinstance(v, torch.Tensor):
-        if v.shape != logits.shape[:1] or v.dtype != dtype or not v.is_contiguous() or v.device != logits.device:
-            raise ValueError(f"sample: {name} is a number or contiguous {dtype} [{logits.shape[0]}] beside the logits")
+        if v.shape != (rows,) or v.dtype != dtype or not v.is_contiguous() or v.get_device() != dev:
+            raise ValueError(f"sample: {name} is a number or contiguous {dtype} [{rows}] beside the logits")
         return v.data_ptr(), 0
     if not v >= least:
         raise ValueError(f"sample: {name} must be at least {least}, got {v}")
@@ -73,28 +73,30 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
 
     A temperature of 0 takes the largest logit, the lowest index among equals.  -inf and NaN are never chosen, infinite logits share the draw; a row with nothing to
     choose from gives -1.  Every setting is a number or holds one for each row (fp32; ``top_k`` int32), on the logits' device."""
-    if logits.dim() != 2 or logits.shape[0] == 0 or logits.shape[1] == 0:
-        raise ValueError(f"sample: logits are [rows, vocabulary], got {tuple(logits.shape)}")
-    B, V = logits.shape
-    if draws.shape != (B,) or draws.dtype not in (torch.float32, torch.float64) or draws.device != logits.device:
+    shape, dev = logits.shape, logits.get_device()
+    if len(shape) != 2 or shape[0] == 0 or shape[1] == 0:
+        raise ValueError(f"sample: logits are [rows, vocabulary], got {tuple(shape)}")
+    B, V = shape
+    if draws.shape != (B,) or draws.dtype not in (torch.float32, torch.float64) or draws.get_device() != dev:
         raise ValueError(f"sample: draws are fp32 or fp64 [{B}] beside the logits")
     top_k = 0 if top_k is None else top_k
-    t_at, t = _setting("temperature", temperature, logits, torch.float32, 0.0)
-    k_at, k = _setting("top_k", top_k, logits, torch.int32, 0)
-    p_at, p = _setting("top_p", top_p, logits, torch.float32, 0.0)
-    m_at, m = _setting("min_p", min_p, logits, torch.float32, 0.0)
-    if not logits.is_cuda:
+    t_at, t = _setting("temperature", temperature, B, dev, torch.float32, 0.0)
+    k_at, k = _setting("top_k", top_k, B, dev, torch.int32, 0)
+    p_at, p = _setting("top_p", top_p, B, dev, torch.float32, 0.0)
+    m_at, m = _setting("min_p", min_p, B, dev, torch.float32, 0.0)
+    if dev < 0:
         if not logits.is_floating_point():
             raise ValueError(f"sample: logits in {logits.dtype} are not supported")
         return _sample_ref(logits, draws, temperature, top_k, top_p, min_p)
     number = _DTYPES.get(logits.dtype)
     if number is None or V > MAX_VOCAB:
         raise ValueError(f"sample: {V} logits in {logits.dtype} are not supported (bf16, fp16 or fp32, up to {MAX_VOCAB})")
-    if logits.stride(1) != 1 and V > 1:
-        logits = logits.contiguous()
-    draws = draws.contiguous()
-    token = torch.empty(B, dtype=torch.int64, device=logits.device)
-    packed = _ARGS.pack(logits.data_ptr(), draws.data_ptr(), t_at, p_at, m_at, k_at, token.data_ptr(), logits.stride(0), t, p, m, B, V, 0, draws.dtype == torch.float64,
+    row, one = logits.stride()
+    if one != 1 and V > 1:
+        logits, row = logits.contiguous(), V
+    draws, device = draws.contiguous(), logits.device
+    token = torch.empty(B, dtype=torch.int64, device=device)
+    packed = _ARGS.pack(logits.data_ptr(), draws.data_ptr(), t_at, p_at, m_at, k_at, token.data_ptr(), row, t, p, m, B, V, 0, draws.dtype == torch.float64,
                         min(int(k), V), 0)
-    check(lib().tyr_sample(packed, number, cur_stream(logits.device)), "sample")
+    check(lib().tyr_sample(packed, number, cur_stream(device)), "sample")
     return token
