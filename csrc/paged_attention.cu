@@ -153,13 +153,28 @@ struct Tile {
   static constexpr int kSize = kKeys * D * kBytes;                          // of the keys, and of the values
   static constexpr int kChunks = D * kBytes / 16;
   static constexpr int kRun = F8 && D >= 128 ? 16 : 8;                      // channels of a box that a lane takes of a value row
-  static constexpr int kStages = kSize <= 4096 ? 6 : (kSize <= 8192 ? 4 : (kSize <= 16384 ? 3 : 2));
   // 16-byte piece c of row r
   static __device__ __forceinline__ uint32_t at(uint32_t base, int r, int c) {
     constexpr int per = kRow / 16;
     const int swizzle = kRow == 128 ? r & 7 : (r >> 1) & 3;
     return base + (c / per) * (kKeys * kRow) + r * kRow + (((c % per) ^ swizzle) << 4);
   }
+};
+
+// Registers and shared memory of a form.  A CTA has five warps, and each quarter of an SM 16384 registers: three CTAs fit with 128 a thread, two with 168, one
+// with more; the fewer stages that many CTAs leave are enough while there are two.
+template <bool F8, int D, int ROWS, int NR>
+struct Form {
+  using TL = Tile<F8, D>;
+  static constexpr int kSlice = D < 128 ? D : 128;                          // channels that the warps join at a time
+  static constexpr int kExtra = 1024 + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * kSlice * 4 : 0);
+  static constexpr int stages(int ctas) { return ((227 * 1024) / ctas - 1024 - kExtra) / (2 * TL::kSize + 48); }
+  static constexpr int kWanted = D == 64 ? (ROWS == 16 ? 3 : 2) : (ROWS == 64 ? 1 : NR == 1 ? (D == 128 ? 3 : 2) : (D == 128 ? 2 : 1));
+  static constexpr int kCtas = stages(kWanted) >= 2 ? kWanted : (kWanted > 1 && stages(kWanted - 1) >= 2 ? kWanted - 1 : 1);
+  static constexpr int kStages = stages(kCtas) < 6 ? stages(kCtas) : 6;
+  static constexpr int kSmem = kExtra + kStages * (2 * TL::kSize + 48);
+  static constexpr int kBound = kCtas == 3 ? 256 : (kCtas == 2 ? 192 : 160);      // threads of which two CTAs (or one) share the registers
+  static constexpr int kAtOnce = kCtas == 1 ? 1 : 2;
 };
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -226,11 +241,12 @@ __device__ __forceinline__ void write4(T* p, float4 v) {
 
 // T: type of the queries, the results and 16-bit pages; NR: rows of a lane (1: at most 8 rows in a tile of 16).
 template <typename T, bool F8, int D, int ROWS, int NR>
-__global__ void __launch_bounds__((kWarps + 1) * 32) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROWS, NR>::kAtOnce) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                                                                            const __grid_constant__ CUtensorMap map_v) {
   using TL = Tile<F8, D>;
   using M = typename std::conditional<F8, __half, T>::type;                 // operands of the products
-  constexpr int STAGES = TL::kStages, KSTEPS = D / 16, NTILES = D / 8;
+  using FM = Form<F8, D, ROWS, NR>;
+  constexpr int STAGES = FM::kStages, KSTEPS = D / 16, NTILES = D / 8;
   constexpr int GROUPS = ROWS == 16 ? 1 : kKeys / 16;                       // runs of 16 keys a warp takes of a tile
   constexpr bool QREG = D <= 128;                                           // the queries' fragments stay in registers
   constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end; in e4m3 pages it meets the codes' 2^-8
@@ -242,7 +258,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32) paged_attention_kernel(cons
   uint64_t* empty = full + STAGES;
   float* s_stats = reinterpret_cast<float*>(empty + STAGES);                // [4][16][4], joining warps (ROWS 16)
   uint4* s_q = reinterpret_cast<uint4*>(s_stats + 256);                     // fragments of the queries, QREG false: [warps that differ][KSTEPS][32]
-  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][D] (ROWS 16)
+  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][kSlice] (ROWS 16)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -598,49 +614,52 @@ __global__ void __launch_bounds__((kWarps + 1) * 32) paged_attention_kernel(cons
     const long long first_row = sh.s.row;
     // channels c * 8 kRun + 2 t kRun + (0 .. 2 kRun - 1) of rows g and g + 8: o[c kRun + i][e] is the one at e kRun + i
     if constexpr (ROWS == 16) {
-      asm volatile("bar.sync 1, 128;" ::: "memory");                        // the last piece's sums are no longer read
+      constexpr int SLICE = FM::kSlice, TILES = SLICE / 8;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        if (t == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + g + 8 * r) * 4) = make_float4(m[r], l[r], top[r], 0.f);
-        float* dst = s_sum + (warp * 8 * NR + g + 8 * r) * D;
+      for (int part = 0; part < D / SLICE; ++part) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");                      // the last sums are no longer read
 #pragma unroll
-        for (int c = 0; c < NTILES / TL::kRun; ++c)
+        for (int r = 0; r < NR; ++r) {
+          if (t == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + g + 8 * r) * 4) = make_float4(m[r], l[r], top[r], 0.f);
+          float* dst = s_sum + (warp * 8 * NR + g + 8 * r) * SLICE;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int c = 0; c < TILES / TL::kRun; ++c)
 #pragma unroll
-            for (int i = 0; i < TL::kRun; i += 4)
-              *reinterpret_cast<float4*>(dst + c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i) =
-                  make_float4(o[c * TL::kRun + i][2 * r + e], o[c * TL::kRun + i + 1][2 * r + e], o[c * TL::kRun + i + 2][2 * r + e], o[c * TL::kRun + i + 3][2 * r + e]);
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int i = tid * 4; i < used * D; i += kWarps * 32 * 4) {
-        const int r = i / D, d = i % D;
-        float mm = -INFINITY, tt = -INFINITY;
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
-          mm = fmaxf(mm, st.x);
-          tt = fmaxf(tt, st.z);
+              for (int i = 0; i < TL::kRun; i += 4) {
+                const int k = part * TILES + c * TL::kRun + i;
+                *reinterpret_cast<float4*>(dst + c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i) = make_float4(o[k][2 * r + e], o[k + 1][2 * r + e], o[k + 2][2 * r + e], o[k + 3][2 * r + e]);
+              }
         }
-        float ll = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = tid * 4; i < used * SLICE; i += kWarps * 32 * 4) {
+          const int r = i / SLICE, d = part * SLICE + i % SLICE;
+          float mm = -INFINITY, tt = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
-          if (st.x != -INFINITY) ll += st.y * pt_exp2(st.x - mm);
-          if (st.z != -INFINITY) {
-            const float f = pt_exp2(st.z - tt);
-            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * D + d);
+          for (int w = 0; w < kWarps; ++w) {
+            const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
+            mm = fmaxf(mm, st.x);
+            tt = fmaxf(tt, st.z);
+          }
+          float ll = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
+            if (st.x != -INFINITY || st.y != 0.f) ll += st.y * (st.x == -INFINITY ? 1.f : pt_exp2(st.x - mm));
+            const float f = st.z == -INFINITY ? (st.y != st.y ? 1.f : 0.f) : pt_exp2(st.z - tt);
+            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * SLICE + i % SLICE);
             v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
           }
-        }
-        if (done) {
-          const int row = sh.row_tile * ROWS + r;
-          const float f = ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(tt - mm) : 1.f) / ll : 0.f;
-          write4(static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
-        } else {
-          *reinterpret_cast<float4*>(part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(r) * D + d) = make_float4(v.x * kUndo, v.y * kUndo, v.z * kUndo, v.w * kUndo);
-          if (d == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + r * 4) = make_float4(mm, ll, tt, 0.f);
+          if (done) {
+            const int row = sh.row_tile * ROWS + r;
+            const float f = ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(tt - mm) : 1.f) / ll : 0.f;
+            write4(static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+          } else {
+            *reinterpret_cast<float4*>(part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(r) * D + d) = make_float4(v.x * kUndo, v.y * kUndo, v.z * kUndo, v.w * kUndo);
+            if (d == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + r * 4) = make_float4(mm, ll, tt, 0.f);
+          }
         }
       }
     } else {
@@ -700,11 +719,9 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
       const int piece = piece_of(i);
       const float4 st = *reinterpret_cast<const float4*>(part_stats(a, ctas, ROWS, piece) + r * 4);
       const float4 x = *reinterpret_cast<const float4*>(part_sums(a, ctas, ROWS, piece) + static_cast<long long>(r) * a.D + d);
-      if (st.x != -INFINITY) l += st.y * pt_exp2(st.x - m);
-      if (st.z != -INFINITY) {
-        const float f = pt_exp2(st.z - top);
-        v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
-      }
+      if (st.x != -INFINITY || st.y != 0.f) l += st.y * (st.x == -INFINITY ? 1.f : pt_exp2(st.x - m));
+      const float f = st.z == -INFINITY ? (st.y != st.y ? 1.f : 0.f) : pt_exp2(st.z - top);
+      v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
     }
     s_v[threadIdx.x] = v;
     s_l[threadIdx.x] = l;
@@ -754,8 +771,7 @@ struct PagedCall {
 
 template <typename T, bool F8, int D, int ROWS, int NR>
 int paged_form(const PagedCall& call) {
-  using TL = Tile<F8, D>;
-  constexpr int kSmem = 1024 + TL::kStages * (2 * TL::kSize + 32 + 16) + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * D * 4 : 0);
+  constexpr int kSmem = Form<F8, D, ROWS, NR>::kSmem;
   const auto kernel = paged_attention_kernel<T, F8, D, ROWS, NR>;
   static const cudaError_t ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (ready != cudaSuccess) return -30;
