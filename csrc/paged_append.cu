@@ -57,7 +57,8 @@ template <typename T>
 __device__ __forceinline__ void pa_store8(T* p, const float (&f)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::put(f[0], f[1]), Pair<T>::put(f[2], f[3]), Pair<T>::put(f[4], f[5]), Pair<T>::put(f[6], f[7]));
 }
-__device__ __forceinline__ uint2 pa_codes8(const float (&f)[8], float inv) {
+__device__ __forceinline__ uint2 pa_codes8(const float (&f)[8], float inv) {      // zeros for a scale that is NaN (inv 0): codes are numbers always
+  if (inv == 0.f) return make_uint2(0u, 0u);
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);

@@ -7,18 +7,17 @@
 //
 // Bound: the keys and values are read once, 2 D bytes a (key, head) in e4m3, for 4 R D operations; up to some hundred operations a byte the memory bounds it.
 //
-// One producer warp copies tiles of 64 keys and values by TMA into a ring of stages (page by page, 128-byte swizzle), four consumer warps multiply with
-// mma.sync m16n8k16: either every warp takes 16 keys of the tile for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
-// memory), or 16 of 64 rows for all keys (ROWS 64: several new tokens).
+// One producer warp copies tiles of keys and values by TMA into a ring of stages (page by page, 128-byte swizzle), four consumer warps multiply with
+// mma.sync m16n8k16: either every warp takes tiles of 32 keys of its own for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
+// memory), or 16 of 64 rows for all tiles of 64 keys (ROWS 64: several new tokens).
 //
 // Every operand comes from shared memory in 16-byte pieces: the order of the channels within a product's sum is free as long as the queries follow it, and so is
 // the order of the keys as long as the values follow it.  A lane (g, t) reads bytes 16 t .. 16 t + 15 (and every 64 on) of key row pi(g), pi(n) = n for even n
 // and n ^ 4 for odd n, and channels 16 g .. 16 g + 15 of the four value rows that its probabilities belong to; with the swizzle neither conflicts.
 //
-// e4m3 to f16 takes three operations for two numbers: the code's seven low bits at bit 7 of a half are the number times 2^-8, subnormals too, and no code gives
-// an infinity or NaN, so that keys past a sequence's end need no care beside their zero probabilities.  Queries in bf16 are scaled by a power of two for each row
-// into f16's range.  With M = max (s + log2 v_scale) beside m, the probabilities times the page's value scale stay within f16 whatever the scales: 2^(s + log2
-// v_scale - M), and the result is taken times 2^(M - m) / l.
+// e4m3 becomes f16 two codes at a time (64 lanes a clock an SM, as the byte permutes that pair the values' rows; done by masks and shifts it took three operations
+// and bound the kernel).  Queries in bf16 are scaled by a power of two for each row into f16's range.  With M = max (s + log2 v_scale) beside m, the probabilities
+// times the page's value scale stay within f16 whatever the scales: 2^(s + log2 v_scale - M), and the result is taken times 2^(M - m) / l.
 //
 // Work is cut into equal shares of tiles, one for each resident CTA, whatever the lengths: a share may begin and end inside a (sequence, head).  Such pieces go to
 // a workspace of the call, and a second launch joins them in the order of the keys.
@@ -28,7 +27,7 @@
 
 namespace tyr {
 
-constexpr int kKeys = 64;                      // keys of a tile
+__host__ __device__ constexpr int tile_keys(int rows) { return rows == 16 ? 32 : 64; }
 constexpr int kWarps = 4;                      // consumer warps
 
 struct PagedAttnArgs {
@@ -62,8 +61,9 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
     s.n = 0;
   }
   const int first = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
-  s.tile0 = first / kKeys;
-  s.tiles = s.n == 0 ? 0 : (s.len + kKeys - 1) / kKeys - s.tile0;
+  constexpr int KEYS = tile_keys(ROWS);
+  s.tile0 = first / KEYS;
+  s.tiles = s.n == 0 ? 0 : (s.len + KEYS - 1) / KEYS - s.tile0;
   s.row_tiles = s.n == 0 ? 0 : (s.n * (a.H / a.G) + ROWS - 1) / ROWS;
   return s;
 }
@@ -135,8 +135,8 @@ struct Share {
     // tiles that the piece's rows see
     const int R = a.H / a.G, held = s.len - s.n, i0 = row_tile * ROWS / R, i1 = min(s.n, (row_tile * ROWS + ROWS - 1) / R + 1) - 1;
     const int lo = a.window > 0 ? max(0, held + i0 - a.window + 1) : 0;
-    first = lo / kKeys;
-    last = (held + i1) / kKeys + 1;
+    first = lo / tile_keys(ROWS);
+    last = (held + i1) / tile_keys(ROWS) + 1;
     if (!a.whole) {
       first = max(first, s.tile0 + x0);
       last = min(last, s.tile0 + x1);
@@ -145,19 +145,19 @@ struct Share {
   }
 };
 
-template <bool F8, int D>
+template <bool F8, int D, int KEYS>
 struct Tile {
   static constexpr int kBytes = F8 ? 1 : 2;
   static constexpr int kRow = D * kBytes < 128 ? D * kBytes : 128;          // bytes of a row in a box
   static constexpr int kBoxes = D * kBytes / kRow;
-  static constexpr int kSize = kKeys * D * kBytes;                          // of the keys, and of the values
+  static constexpr int kSize = KEYS * D * kBytes;                          // of the keys, and of the values
   static constexpr int kChunks = D * kBytes / 16;
   static constexpr int kRun = F8 && D >= 128 ? 16 : 8;                      // channels of a box that a lane takes of a value row
   // 16-byte piece c of row r
   static __device__ __forceinline__ uint32_t at(uint32_t base, int r, int c) {
     constexpr int per = kRow / 16;
     const int swizzle = kRow == 128 ? r & 7 : (r >> 1) & 3;
-    return base + (c / per) * (kKeys * kRow) + r * kRow + (((c % per) ^ swizzle) << 4);
+    return base + (c / per) * (KEYS * kRow) + r * kRow + (((c % per) ^ swizzle) << 4);
   }
 };
 
@@ -165,13 +165,14 @@ struct Tile {
 // with more; the fewer stages that many CTAs leave are enough while there are two.
 template <bool F8, int D, int ROWS, int NR>
 struct Form {
-  using TL = Tile<F8, D>;
+  using TL = Tile<F8, D, tile_keys(ROWS)>;
   static constexpr int kSlice = D < 128 ? D : 128;                          // channels that the warps join at a time
   static constexpr int kExtra = 1024 + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * kSlice * 4 : 0);
   static constexpr int stages(int ctas) { return ((227 * 1024) / ctas - 1024 - kExtra) / (2 * TL::kSize + 48); }
+  static constexpr int kFew = ROWS == 16 ? 4 : 2;                           // stages that keep the consumers busy
   static constexpr int kWanted = D == 64 ? (ROWS == 16 ? 3 : 2) : (ROWS == 64 ? 1 : NR == 1 ? (D == 128 ? 3 : 2) : (D == 128 ? 2 : 1));
-  static constexpr int kCtas = stages(kWanted) >= 2 ? kWanted : (kWanted > 1 && stages(kWanted - 1) >= 2 ? kWanted - 1 : 1);
-  static constexpr int kStages = stages(kCtas) < 6 ? stages(kCtas) : 6;
+  static constexpr int kCtas = stages(kWanted) >= kFew ? kWanted : (kWanted > 1 && stages(kWanted - 1) >= kFew ? kWanted - 1 : 1);
+  static constexpr int kStages = stages(kCtas) < 12 ? stages(kCtas) : 12;
   static constexpr int kSmem = kExtra + kStages * (2 * TL::kSize + 48);
   static constexpr int kBound = kCtas == 3 ? 256 : (kCtas == 2 ? 192 : 160);      // threads of which two CTAs (or one) share the registers
   static constexpr int kAtOnce = kCtas == 1 ? 1 : 2;
@@ -192,8 +193,12 @@ __device__ __forceinline__ uint32_t pt_prmt(uint32_t x, uint32_t y, uint32_t sel
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(sel));
   return r;
 }
-// codes in bytes 1 and 3 -> two halves, times 2^-8; bytes 0 and 2 do not matter
-__device__ __forceinline__ uint32_t halves_of_codes(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
+// the two codes in a word's lower half -> two halves
+__device__ __forceinline__ uint32_t halves_of_codes(uint32_t w) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(w)));
+  return r;
+}
 
 template <typename T> struct Num;
 template <> struct Num<__nv_bfloat16> {
@@ -243,13 +248,14 @@ __device__ __forceinline__ void write4(T* p, float4 v) {
 template <typename T, bool F8, int D, int ROWS, int NR>
 __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROWS, NR>::kAtOnce) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                                                                            const __grid_constant__ CUtensorMap map_v) {
-  using TL = Tile<F8, D>;
+  constexpr int KEYS = tile_keys(ROWS);
+  using TL = Tile<F8, D, KEYS>;
   using M = typename std::conditional<F8, __half, T>::type;                 // operands of the products
   using FM = Form<F8, D, ROWS, NR>;
   constexpr int STAGES = FM::kStages, KSTEPS = D / 16, NTILES = D / 8;
-  constexpr int GROUPS = ROWS == 16 ? 1 : kKeys / 16;                       // runs of 16 keys a warp takes of a tile
+  constexpr int GROUPS = KEYS / 16;                                         // runs of 16 keys
   constexpr bool QREG = D <= 128;                                           // the queries' fragments stay in registers
-  constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end; in e4m3 pages it meets the codes' 2^-8
+  constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* extra = smem + STAGES * 2 * TL::kSize;
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, kWarps);
+      mbar_init(empty + i, ROWS == 16 ? 1 : kWarps);
     }
     mbar_fence_init();
     tma_prefetch_desc(&map_k);
@@ -275,19 +281,19 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   pdl_wait();
   const int R = a.H / a.G;
   Share<ROWS> sh(a, lane);
-  int stage = 0;
-  uint32_t phase = 0;
+  uint32_t turn = 0;                                                        // tiles before this one: its stage and the parity of the stage's use
 
   if (warp == kWarps) {
     // ---- producer ---------------------------------------------------------------------------------------------------
-    const int page_rows = min(a.P, kKeys), per_tile = kKeys / page_rows;
+    const int page_rows = min(a.P, KEYS), per_tile = KEYS / page_rows;
     while (sh.next()) {
       const int last_page = (sh.s.len - 1) / a.P;
       const int* table = a.table + sh.b * a.table_row;
       int batch = -1, id = 0;                       // pages 32 batch .. of the sequence, one a lane
       float2 scale = make_float2(1.f, 0.f);
-      for (int tile = sh.first; tile < sh.last; ++tile) {
-        const int p0 = tile * kKeys / a.P;
+      for (int tile = sh.first; tile < sh.last; ++tile, ++turn) {
+        const int stage = turn % STAGES, phase = turn / STAGES & 1;
+        const int p0 = tile * KEYS / a.P;
         if (p0 >> 5 != batch) {
           batch = p0 >> 5;
           const int p = batch * 32 + lane;
@@ -308,16 +314,12 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         __syncwarp();
         if (lane < n) {
           uint8_t* dst = smem + stage * 2 * TL::kSize + lane * page_rows * TL::kRow;
-          const int row = (tile * kKeys) % a.P, z = page * a.G + sh.head;
+          const int row = (tile * KEYS) % a.P, z = page * a.G + sh.head;
 #pragma unroll
           for (int c = 0; c < TL::kBoxes; ++c) {
-            tma_load_3d(dst + c * kKeys * TL::kRow, &map_k, full + stage, c * (TL::kRow / TL::kBytes), row, z);
-            tma_load_3d(dst + TL::kSize + c * kKeys * TL::kRow, &map_v, full + stage, c * (TL::kRow / TL::kBytes), row, z);
+            tma_load_3d(dst + c * KEYS * TL::kRow, &map_k, full + stage, c * (TL::kRow / TL::kBytes), row, z);
+            tma_load_3d(dst + TL::kSize + c * KEYS * TL::kRow, &map_v, full + stage, c * (TL::kRow / TL::kBytes), row, z);
           }
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
         }
       }
     }
@@ -327,6 +329,13 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   // ---- consumers ------------------------------------------------------------------------------------------------------
   const int g = lane >> 2, t = lane & 3, pi = g & 1 ? g ^ 4 : g;
   const int tid = threadIdx.x;
+  // this lane's pieces of a tile: rows 8 apart and boxes lie the same way
+  constexpr int PIECES_BOX = TL::kRow / 64;                                 // of a key row in a box
+  uint32_t k_at[PIECES_BOX], v_at[2];
+#pragma unroll
+  for (int c = 0; c < PIECES_BOX; ++c) k_at[c] = TL::at(0, pi, t + 4 * c);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v_at[i] = F8 && D == 64 ? TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g >> 1) + (g & 1) * 8 : TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g);
   // rows of no sequence
   for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps) {
     const bool none = a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0;
@@ -378,9 +387,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
           up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
           factor[r] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         }
-        factor[r] *= 256.f;                                                  // of the keys' codes
         const uint32_t* flat = &raw[0][0];
-        // channels {0, 2} and {1, 3} of every four, as the codes' even and odd bytes come out
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
           uint32_t x = flat[2 * ks], y = flat[2 * ks + 1];
@@ -389,14 +396,13 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             x = Num<__half>::pack(u.x * up, u.y * up);
             y = Num<__half>::pack(v.x * up, v.y * up);
           }
-          const uint32_t even = pt_prmt(x, y, 0x5410), odd = pt_prmt(x, y, 0x7632);
           if constexpr (QREG) {
-            qa[ks][r] = even;
-            qa[ks][NR + r] = odd;
+            qa[ks][r] = x;
+            qa[ks][NR + r] = y;
           } else if (ROWS != 16 || warp == 0) {
             uint32_t* dst = reinterpret_cast<uint32_t*>(s_q + ((ROWS == 16 ? 0 : warp) * KSTEPS + ks) * 32 + lane);
-            dst[r] = even;
-            dst[NR + r] = odd;
+            dst[r] = x;
+            dst[NR + r] = y;
           }
         }
       } else {
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");
     // every key of tiles from `clear0` to before `clear1` is seen by all rows of the piece
     const int p_first = held + sh.row_tile * ROWS / R, p_last = held + (sh.row_tile * ROWS + used - 1) / R;
-    const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + kKeys - 1) / kKeys : 0, clear1 = (p_first + 1) / kKeys;
+    const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + KEYS - 1) / KEYS : 0, clear1 = (p_first + 1) / KEYS;
 
     float m[NR], l[NR], top[NR], o[NTILES][2 * NR];
 #pragma unroll
@@ -427,10 +433,14 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
 #pragma unroll
       for (int e = 0; e < 2 * NR; ++e) o[i][e] = 0.f;
 
-    for (int tile = sh.first; tile < sh.last; ++tile) {
-      if (!mbar_wait(full + stage, phase, a.err, 2)) return;
+    // ROWS 16: every fourth tile
+    const int skip = ROWS == 16 ? warp : 0, step = ROWS == 16 ? kWarps : 1;
+    const uint32_t first_turn = turn;
+    for (int tile = sh.first + skip; tile < sh.last; tile += step) {
+      turn = first_turn + (tile - sh.first);
+      const int stage = turn % STAGES;
+      if (!mbar_wait(full + stage, turn / STAGES & 1, a.err, 2)) return;
       const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
-      const int group0 = ROWS == 16 ? warp : 0;
       // ---- scores ------------------------------------------------------------------------------------------------------
       float s[GROUPS][2][2 * NR];
 #pragma unroll
@@ -463,11 +473,11 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint4 u = lds128(TL::at(kb, 16 * (group0 + j) + 8 * h + pi, t + 4 * c));
+            const uint4 u = lds128(kb + k_at[c % PIECES_BOX] + (c / PIECES_BOX) * (KEYS * TL::kRow) + (16 * j + 8 * h) * TL::kRow);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
             if constexpr (F8) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) mma<M, NR>(s[j][h], qs[i], halves_of_codes(w[i] << 8), halves_of_codes(w[i]));
+              for (int i = 0; i < 4; ++i) mma<M, NR>(s[j][h], qs[i], halves_of_codes(w[i]), halves_of_codes(w[i] >> 16));
             } else {
               mma<M, NR>(s[j][h], qs[0], w[0], w[1]);
               mma<M, NR>(s[j][h], qs[1], w[2], w[3]);
@@ -475,7 +485,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
           }
       }
       // ---- running maxima --------------------------------------------------------------------------------------------------
-      const int key0 = tile * kKeys;
+      const int key0 = tile * KEYS;
       const bool masked = tile < clear0 || tile >= clear1;
       float mx[NR], mt[NR], lv[GROUPS];
 #pragma unroll
@@ -485,7 +495,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         float ks = 1.f;
         lv[j] = 0.f;
         if constexpr (F8) {
-          const int at = a.P >= kKeys ? 0 : 16 * (group0 + j) / a.P;
+          const int at = a.P >= KEYS ? 0 : 16 * j / a.P;
           const float2 sc = s_scale[stage * 4 + at];
           ks = sc.y == sc.y ? sc.x : sc.y;                                   // a page whose values hold no numbers shows at the keys that are seen
           lv[j] = sc.y == sc.y ? sc.y : 0.f;
@@ -500,7 +510,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             for (int e = 0; e < 2; ++e) {
               float v = s[j][h][2 * r + e] * f;
               if (masked) {
-                const int key = key0 + 16 * (group0 + j) + 8 * h + (e == 0 ? 2 * t : (2 * t + 1) ^ 4);
+                const int key = key0 + 16 * j + 8 * h + (e == 0 ? 2 * t : (2 * t + 1) ^ 4);
                 if (key > pos[r] || (a.window > 0 && key <= pos[r] - a.window)) v = -INFINITY;
               }
               s[j][h][2 * r + e] = v;
@@ -554,39 +564,40 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             pa[h * NR + r] = Num<M>::pack(p0 * by, p1 * by);
           }
         }
-        const int row = 16 * (group0 + j) + 2 * t, row1 = 16 * (group0 + j) + ((2 * t + 1) ^ 4);
-        const int left = F8 || !masked ? 16 : sh.s.len - (key0 + 16 * (group0 + j));      // 16-bit pages: what lies past the end may be no number
+        // what lies past the sequence's end may be no number, and nothing times that neither
+        const int left = masked ? sh.s.len - (key0 + 16 * j) : 16;
+        const uint32_t v0 = vb + v_at[0] + 16 * j * TL::kRow, v1 = vb + v_at[1] + 16 * j * TL::kRow;
+        // codes e of two words -> two halves
+        const auto pair = [](uint32_t x, uint32_t y, int e) { return halves_of_codes(pt_prmt(x, y, (4 + e) << 4 | e)); };
         if constexpr (F8 && D == 64) {
-          const uint32_t at = (g & 1) * 8;
-          const uint2 x = lds64(TL::at(vb, row, g >> 1) + at), y = lds64(TL::at(vb, row1, g >> 1) + at);
-          const uint2 z = lds64(TL::at(vb, row + 8, g >> 1) + at), u = lds64(TL::at(vb, row1 + 8, g >> 1) + at);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = i & 3;
-            const uint32_t sel = (4 + e) << 12 | e << 4;
-            mma<M, NR>(o[i], pa, halves_of_codes(pt_prmt(i < 4 ? x.x : x.y, i < 4 ? y.x : y.y, sel)), halves_of_codes(pt_prmt(i < 4 ? z.x : z.y, i < 4 ? u.x : u.y, sel)));
+          uint2 x = lds64(v0), y = lds64(v1), z = lds64(v0 + 8 * TL::kRow), u = lds64(v1 + 8 * TL::kRow);
+          if (left < 16) {
+            if (2 * t >= left) x = make_uint2(0u, 0u);
+            if (((2 * t + 1) ^ 4) >= left) y = make_uint2(0u, 0u);
+            if (2 * t + 8 >= left) z = make_uint2(0u, 0u);
+            if (((2 * t + 1) ^ 4) + 8 >= left) u = make_uint2(0u, 0u);
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            mma<M, NR>(o[i], pa, pair(i < 4 ? x.x : x.y, i < 4 ? y.x : y.y, i & 3), pair(i < 4 ? z.x : z.y, i < 4 ? u.x : u.y, i & 3));
         } else {
 #pragma unroll
           for (int c = 0; c < TL::kBoxes; ++c) {
-            const uint4 xs = lds128(TL::at(vb, row, 8 * c + g)), ys = lds128(TL::at(vb, row1, 8 * c + g));
-            const uint4 zs = lds128(TL::at(vb, row + 8, 8 * c + g)), us = lds128(TL::at(vb, row1 + 8, 8 * c + g));
-            uint32_t x[4] = {xs.x, xs.y, xs.z, xs.w}, y[4] = {ys.x, ys.y, ys.z, ys.w}, z[4] = {zs.x, zs.y, zs.z, zs.w}, u[4] = {us.x, us.y, us.z, us.w};
+            const uint32_t at = c * KEYS * TL::kRow;
+            uint4 xs = lds128(v0 + at), ys = lds128(v1 + at), zs = lds128(v0 + at + 8 * TL::kRow), us = lds128(v1 + at + 8 * TL::kRow);
+            if (left < 16) {
+              if (2 * t >= left) xs = make_uint4(0u, 0u, 0u, 0u);
+              if (((2 * t + 1) ^ 4) >= left) ys = make_uint4(0u, 0u, 0u, 0u);
+              if (2 * t + 8 >= left) zs = make_uint4(0u, 0u, 0u, 0u);
+              if (((2 * t + 1) ^ 4) + 8 >= left) us = make_uint4(0u, 0u, 0u, 0u);
+            }
+            const uint32_t x[4] = {xs.x, xs.y, xs.z, xs.w}, y[4] = {ys.x, ys.y, ys.z, ys.w}, z[4] = {zs.x, zs.y, zs.z, zs.w}, u[4] = {us.x, us.y, us.z, us.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               if constexpr (F8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t sel = (4 + e) << 12 | e << 4;
-                  mma<M, NR>(o[c * 16 + 4 * w + e], pa, halves_of_codes(pt_prmt(x[w], y[w], sel)), halves_of_codes(pt_prmt(z[w], u[w], sel)));
-                }
+                for (int e = 0; e < 4; ++e) mma<M, NR>(o[c * 16 + 4 * w + e], pa, pair(x[w], y[w], e), pair(z[w], u[w], e));
               } else {
-                if (left < 16) {
-                  if (2 * t >= left) x[w] = 0u;
-                  if (((2 * t + 1) ^ 4) >= left) y[w] = 0u;
-                  if (2 * t + 8 >= left) z[w] = 0u;
-                  if (((2 * t + 1) ^ 4) + 8 >= left) u[w] = 0u;
-                }
                 mma<M, NR>(o[c * 8 + 2 * w], pa, pt_prmt(x[w], y[w], 0x5410), pt_prmt(z[w], u[w], 0x5410));
                 mma<M, NR>(o[c * 8 + 2 * w + 1], pa, pt_prmt(x[w], y[w], 0x7632), pt_prmt(z[w], u[w], 0x7632));
               }
@@ -596,13 +607,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + stage);
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1;
-      }
     }
+    turn = first_turn + max(0, sh.last - sh.first);
     // ---- the piece's result: in units of 2^top where the keys have scales, l over the lanes of a row ----------------------------------
-    constexpr float kUndo = !F8 && __is_same(M, __half) ? 1.f / 256.f : 1.f;
+    constexpr float kUndo = __is_same(M, __half) ? 1.f / 256.f : 1.f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -743,8 +751,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
 typedef CUresult (*PagedEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Pages as [pages * G, P, D]; boxes of 128 bytes (a whole row where it is shorter) of min(P, 64) tokens of one page and head.
-template <bool F8, int D>
+// Pages as [pages * G, P, D]; boxes of 128 bytes (a whole row where it is shorter) of min(P, KEYS) tokens of one page and head.
+template <bool F8, int D, int KEYS>
 int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
   static const PagedEncodeFn encode = [] {
     void* ptr = nullptr;
@@ -753,10 +761,10 @@ int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
                ? reinterpret_cast<PagedEncodeFn>(ptr) : nullptr;
   }();
   if (encode == nullptr) return -20;
-  using TL = Tile<F8, D>;
+  using TL = Tile<F8, D, KEYS>;
   const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(a.P), static_cast<cuuint64_t>(a.pages) * a.G};
   const cuuint64_t strides[2] = {D * TL::kBytes, static_cast<cuuint64_t>(a.P) * D * TL::kBytes};
-  const cuuint32_t box[3] = {TL::kRow / TL::kBytes, static_cast<cuuint32_t>(a.P < kKeys ? a.P : kKeys), 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {TL::kRow / TL::kBytes, static_cast<cuuint32_t>(a.P < KEYS ? a.P : KEYS), 1}, step[3] = {1, 1, 1};
   const CUresult r = encode(map, F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, TL::kRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -783,8 +791,8 @@ int paged_form(const PagedCall& call) {
   }
   const PagedAttnArgs& a = *call.a;
   CUtensorMap mk, mv;
-  int r = page_map<F8, D>(&mk, a.k_pages, a);
-  if (r == 0) r = page_map<F8, D>(&mv, a.v_pages, a);
+  int r = page_map<F8, D, tile_keys(ROWS)>(&mk, a.k_pages, a);
+  if (r == 0) r = page_map<F8, D, tile_keys(ROWS)>(&mv, a.v_pages, a);
   if (r != 0) return r;
   const int R = a.H / a.G;
   const long long items = (a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS)) * a.G;
@@ -828,7 +836,7 @@ extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int
   if (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) return -2;
   if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64) || (!a.whole && (a.part == nullptr || a.ctas <= 0))) return -3;
   // a sequence's work and the pages' rows are counted in 32 bits
-  const long long tiles = (static_cast<long long>(a.width) * a.P + kKeys - 1) / kKeys;
+  const long long tiles = (static_cast<long long>(a.width) * a.P + tile_keys(rows) - 1) / tile_keys(rows);
   if ((static_cast<long long>(a.rows) * (a.H / a.G) / rows + 1) * a.G * tiles > 0x7fffffffLL || static_cast<long long>(a.pages) * a.G > 0x7fffffffLL) return -4;
   if (static_cast<long long>(a.width) * a.P > 0x7fffffffLL || static_cast<long long>(a.rows) * a.H > 0x7fffffffLL) return -5;
   return paged_type(PagedCall{&a, (cudaStream_t)stream}, dtype, a.k_scale != nullptr, a.D, rows, a.starts == nullptr && a.H / a.G <= 8);

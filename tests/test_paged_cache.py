@@ -265,6 +265,7 @@ def broken(dev, decode):
         y[0, 1, 5] = bad
         put(2, y)
         assert float(store.k_scale[1, 0]) == 2.0 ** -8 and math.isnan(store.k_scale[1, 1]) and math.isnan(store.v_scale[1, 1])
+        assert not store.k[1, 1, 1].float().any() and not store.v[1, 1, 1].float().any()      # codes are numbers always
         put(3, x)
         assert math.isnan(store.k_scale[1, 1]) and float(store.v_scale[1, 0]) == 2.0 ** -8
         put(1, x)
