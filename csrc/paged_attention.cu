@@ -8,11 +8,12 @@
 // Bound: the keys and values are read once, 2 D bytes a (key, head) in e4m3, for 4 R D operations; up to some hundred operations a byte the memory bounds it.
 //
 // One producer warp copies tiles of keys and values by TMA into a ring of stages (page by page, 128-byte swizzle), four consumer warps multiply with
-// mma.sync m16n8k16: either every warp takes tiles of 32 keys of its own for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
+// mma.sync m16n8k16: either every warp takes tiles of its own (32 keys of 128 bytes) for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
 // memory), or 16 of 64 rows for all tiles of 64 keys (ROWS 64: several new tokens).
 //
 // Every operand comes from shared memory in 16-byte pieces: the order of the channels within a product's sum is free as long as the queries follow it, and so is
-// the order of the keys as long as the values follow it.  A lane (g, t) reads bytes 16 t .. 16 t + 15 (and every 64 on) of key row pi(g), pi(n) = n for even n
+// the order of the keys as long as the values follow it.  The keys and the values are the products' first operands (16 of them, or 16 channels, by 8 rows; a second
+// 8 rows where there are more), so that few rows leave nothing idle but columns.  A lane (g, t) reads bytes 16 t .. 16 t + 15 (and every 64 on) of key row pi(g), pi(n) = n for even n
 // and n ^ 4 for odd n, and channels 16 g .. 16 g + 15 of the four value rows that its probabilities belong to; with the swizzle neither conflicts.
 //
 // e4m3 becomes f16 two codes at a time (64 lanes a clock an SM, as the byte permutes that pair the values' rows; done by masks and shifts it took three operations
@@ -27,7 +28,8 @@
 
 namespace tyr {
 
-__host__ __device__ constexpr int tile_keys(int rows) { return rows == 16 ? 32 : 64; }
+// keys of a tile: while decoding some 8 KB of keys and values, a warp's own
+__host__ __device__ constexpr int tile_keys(int rows, int row_bytes) { return rows == 64 ? 64 : row_bytes <= 128 ? 32 : 16; }
 constexpr int kWarps = 4;                      // consumer warps
 
 struct PagedAttnArgs {
@@ -50,7 +52,7 @@ struct PartHead { int row, heads, used, last, slot, pad[3]; };      // a (sequen
 struct Seq { int row, n, len, tile0, tiles, row_tiles; };
 
 // Rows, keys and tiles of sequence b; none where the operands do not go together (recorded).
-template <int ROWS>
+template <int ROWS, int KEYS>
 __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   Seq s;
   s.len = a.lengths[b];
@@ -61,7 +63,6 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
     s.n = 0;
   }
   const int first = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
-  constexpr int KEYS = tile_keys(ROWS);
   s.tile0 = first / KEYS;
   s.tiles = s.n == 0 ? 0 : (s.len + KEYS - 1) / KEYS - s.tile0;
   s.row_tiles = s.n == 0 ? 0 : (s.n * (a.H / a.G) + ROWS - 1) / ROWS;
@@ -76,7 +77,7 @@ __device__ __forceinline__ long long warp_sum64(long long v) {
 }
 
 // This CTA's share of the work, walked piece by piece: a piece is a run of tiles of one (sequence, head, row tile).  Every warp walks it for itself.
-template <int ROWS>
+template <int ROWS, int KEYS>
 struct Share {
   const PagedAttnArgs& a;
   long long at, end, before, per;              // in tiles (items where shares are whole items); `before`: work of the sequences before b
@@ -88,7 +89,7 @@ struct Share {
 
   __device__ __forceinline__ Share(const PagedAttnArgs& args, int lane_) : a(args), lane(lane_) {
     long long sum = 0;
-    for (int i = lane; i < a.B; i += 32) sum += seq_work(a, seq_of<ROWS>(a, i));
+    for (int i = lane; i < a.B; i += 32) sum += seq_work(a, seq_of<ROWS, KEYS>(a, i));
     const long long total = warp_sum64(sum);
     per = (total + gridDim.x - 1) / gridDim.x;
     at = min(static_cast<long long>(blockIdx.x) * per, total);
@@ -97,7 +98,7 @@ struct Share {
     b = 0;
     if (at >= end) return;
     for (int base = 0; base < a.B; base += 32) {
-      const long long mine = base + lane < a.B ? seq_work(a, seq_of<ROWS>(a, base + lane)) : 0;
+      const long long mine = base + lane < a.B ? seq_work(a, seq_of<ROWS, KEYS>(a, base + lane)) : 0;
       long long upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -113,14 +114,14 @@ struct Share {
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    s = seq_of<ROWS>(a, b);
+    s = seq_of<ROWS, KEYS>(a, b);
   }
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
     while (at - before >= seq_work(a, s)) {
       before += seq_work(a, s);
       if (++b >= a.B) return false;
-      s = seq_of<ROWS>(a, b);
+      s = seq_of<ROWS, KEYS>(a, b);
     }
     const int off = static_cast<int>(at - before), unit = a.whole ? 1 : s.tiles, item = off / unit;
     head = item / s.row_tiles;
@@ -135,8 +136,8 @@ struct Share {
     // tiles that the piece's rows see
     const int R = a.H / a.G, held = s.len - s.n, i0 = row_tile * ROWS / R, i1 = min(s.n, (row_tile * ROWS + ROWS - 1) / R + 1) - 1;
     const int lo = a.window > 0 ? max(0, held + i0 - a.window + 1) : 0;
-    first = lo / tile_keys(ROWS);
-    last = (held + i1) / tile_keys(ROWS) + 1;
+    first = lo / KEYS;
+    last = (held + i1) / KEYS + 1;
     if (!a.whole) {
       first = max(first, s.tile0 + x0);
       last = min(last, s.tile0 + x1);
@@ -165,14 +166,20 @@ struct Tile {
 // with more; the fewer stages that many CTAs leave are enough while there are two.
 template <bool F8, int D, int ROWS, int NR>
 struct Form {
-  using TL = Tile<F8, D, tile_keys(ROWS)>;
-  static constexpr int kSlice = D < 128 ? D : 128;                          // channels that the warps join at a time
-  static constexpr int kExtra = 1024 + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * kSlice * 4 : 0);
-  static constexpr int stages(int ctas) { return ((227 * 1024) / ctas - 1024 - kExtra) / (2 * TL::kSize + 48); }
-  static constexpr int kFew = ROWS == 16 ? 4 : 2;                           // stages that keep the consumers busy
+  static constexpr int kKeys = tile_keys(ROWS, D * (F8 ? 1 : 2));
+  using TL = Tile<F8, D, kKeys>;
+  static constexpr int kExtra = 1024 + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * 32 * 4 : 0);
+  // ROWS 16: a multiple of the warps, so that a stage is always the same warp's.  A warp that waits for a stage's next use has then seen its last one, and one bit
+  // tells them apart.
+  static constexpr int stages(int ctas) {
+    const int n = ((227 * 1024) / ctas - 1024 - kExtra) / (2 * TL::kSize + 48);
+    return ROWS == 16 ? n / kWarps * kWarps : n;
+  }
+  static constexpr int kFew = ROWS == 16 ? 2 * kWarps : 2;                  // one in use and one on its way
   static constexpr int kWanted = D == 64 ? (ROWS == 16 ? 3 : 2) : (ROWS == 64 ? 1 : NR == 1 ? (D == 128 ? 3 : 2) : (D == 128 ? 2 : 1));
   static constexpr int kCtas = stages(kWanted) >= kFew ? kWanted : (kWanted > 1 && stages(kWanted - 1) >= kFew ? kWanted - 1 : 1);
   static constexpr int kStages = stages(kCtas) < 12 ? stages(kCtas) : 12;
+  static_assert(kStages >= kFew, "shared memory");
   static constexpr int kSmem = kExtra + kStages * (2 * TL::kSize + 48);
   static constexpr int kBound = kCtas == 3 ? 256 : (kCtas == 2 ? 192 : 160);      // threads of which two CTAs (or one) share the registers
   static constexpr int kAtOnce = kCtas == 1 ? 1 : 2;
@@ -212,19 +219,22 @@ template <> struct Num<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
-// c (rows g and, with NR 2, g + 8) += a b; M is the operands' type.
-template <typename M, int NR>
-__device__ __forceinline__ void mma(float (&c)[2 * NR], const uint32_t (&x)[2 * NR], uint32_t b0, uint32_t b1) {
-  float z0 = 0.f, z1 = 0.f;
-  float &c2 = NR == 2 ? c[2 * NR - 2] : z0, &c3 = NR == 2 ? c[2 * NR - 1] : z1;
-  const uint32_t a0 = x[0], a2 = x[NR], a1 = NR == 2 ? x[1] : 0u, a3 = NR == 2 ? x[2 * NR - 1] : 0u;
-  if constexpr (sizeof(M) == 2 && __is_same(M, __half)) {
+// c [16, 8] += a [16, 16] b [16, 8]; M is the operands' type.
+template <typename M>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (__is_same(M, __half)) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c2), "+f"(c3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   } else {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c2), "+f"(c3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+}
+// An 8 x 8 matrix of 16-bit numbers, a lane (g, t) holding row g's 2 t and 2 t + 1, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
 __device__ __forceinline__ float pt_exp2(float x) {
@@ -248,11 +258,11 @@ __device__ __forceinline__ void write4(T* p, float4 v) {
 template <typename T, bool F8, int D, int ROWS, int NR>
 __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROWS, NR>::kAtOnce) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                                                                            const __grid_constant__ CUtensorMap map_v) {
-  constexpr int KEYS = tile_keys(ROWS);
+  constexpr int KEYS = Form<F8, D, ROWS, NR>::kKeys;
   using TL = Tile<F8, D, KEYS>;
   using M = typename std::conditional<F8, __half, T>::type;                 // operands of the products
   using FM = Form<F8, D, ROWS, NR>;
-  constexpr int STAGES = FM::kStages, KSTEPS = D / 16, NTILES = D / 8;
+  constexpr int STAGES = FM::kStages, KSTEPS = D / 16, TILES = D / 16;
   constexpr int GROUPS = KEYS / 16;                                         // runs of 16 keys
   constexpr bool QREG = D <= 128;                                           // the queries' fragments stay in registers
   constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end
@@ -264,7 +274,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   uint64_t* empty = full + STAGES;
   float* s_stats = reinterpret_cast<float*>(empty + STAGES);                // [4][16][4], joining warps (ROWS 16)
   uint4* s_q = reinterpret_cast<uint4*>(s_stats + 256);                     // fragments of the queries, QREG false: [warps that differ][KSTEPS][32]
-  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][kSlice] (ROWS 16)
+  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][32] (ROWS 16)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -280,7 +290,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   __syncthreads();
   pdl_wait();
   const int R = a.H / a.G;
-  Share<ROWS> sh(a, lane);
+  Share<ROWS, KEYS> sh(a, lane);
   uint32_t turn = 0;                                                        // tiles before this one: its stage and the parity of the stage's use
 
   if (warp == kWarps) {
@@ -344,20 +354,18 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   }
   PartHead head{0, 0, 0, -1, 0, {0, 0, 0}};
   if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
-  bool first_piece = true;
+  bool first_piece = true, lost = false;
   while (sh.next()) {
     const int held = sh.s.len - sh.s.n, used = min(ROWS, sh.s.n * R - sh.row_tile * ROWS);         // rows of this tile
     const int warp_row = ROWS == 16 ? 0 : warp * 16;
-    // ---- queries: this lane's rows, their places and their fragments -------------------------------------------------
+    // ---- queries: row g (and g + 8) in fragments; the scores' rows are 2 t and 2 t + 1 (and 8 further) ----------------------------
     uint32_t qa[QREG ? KSTEPS : 1][2 * NR];
     float factor[NR];
-    int pos[NR];
     if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");                // the last piece's fragments are no longer read
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int in_tile = warp_row + g + 8 * r, row = sh.row_tile * ROWS + in_tile, i = row / R;
       const bool there = in_tile < used;
-      pos[r] = there ? held + i : -1;
       const T* src = static_cast<const T*>(a.q) + (there ? (sh.s.row + i) * a.q_row + (sh.head * R + row % R) * a.q_head : 0);
       constexpr int PIECES = TL::kChunks / 4;                                // 16-byte pieces of a key row that a lane takes
       constexpr int PER = F8 ? 16 : 8;                                       // channels of one
@@ -421,34 +429,51 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       }
     }
     if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");
+    float by_row[NR][2];                                                     // of the scores' rows
+    int pos[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int in_tile = warp_row + 8 * r + 2 * t + e;
+        by_row[r][e] = __shfl_sync(0xffffffffu, factor[r], (2 * t + e) * 4);
+        pos[r][e] = in_tile < used ? held + (sh.row_tile * ROWS + in_tile) / R : -1;
+      }
     // every key of tiles from `clear0` to before `clear1` is seen by all rows of the piece
     const int p_first = held + sh.row_tile * ROWS / R, p_last = held + (sh.row_tile * ROWS + used - 1) / R;
     const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + KEYS - 1) / KEYS : 0, clear1 = (p_first + 1) / KEYS;
 
-    float m[NR], l[NR], top[NR], o[NTILES][2 * NR];
+    float m[NR][2], l[NR][2], top[NR][2], o[TILES][NR][4];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) m[r] = top[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int i = 0; i < NTILES; ++i)
+      for (int e = 0; e < 2; ++e) m[r][e] = top[r][e] = -INFINITY, l[r][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2 * NR; ++e) o[i][e] = 0.f;
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][r][e] = 0.f;
 
-    // ROWS 16: every fourth tile
-    const int skip = ROWS == 16 ? warp : 0, step = ROWS == 16 ? kWarps : 1;
+    // ROWS 16: every fourth tile of all
     const uint32_t first_turn = turn;
+    const int skip = ROWS == 16 ? static_cast<int>((warp - first_turn) & (kWarps - 1)) : 0, step = ROWS == 16 ? kWarps : 1;
     for (int tile = sh.first + skip; tile < sh.last; tile += step) {
       turn = first_turn + (tile - sh.first);
       const int stage = turn % STAGES;
-      if (!mbar_wait(full + stage, turn / STAGES & 1, a.err, 2)) return;
+      if (lost || !mbar_wait(full + stage, turn / STAGES & 1, a.err, 2)) {
+        lost = true;                                                        // recorded; the warps still meet at their barriers
+        break;
+      }
       const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
-      // ---- scores ------------------------------------------------------------------------------------------------------
-      float s[GROUPS][2][2 * NR];
+      // ---- scores: keys pi(g) and pi(g) + 8 of every 16, rows 2 t and 2 t + 1 --------------------------------------------------
+      float s[GROUPS][NR][4];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 2 * NR; ++e) s[j][h][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[j][r][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < TL::kChunks / 4; ++c) {
         constexpr int STEPS = F8 ? 4 : 2;
@@ -470,26 +495,29 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
           }
         }
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j)
+        for (int j = 0; j < GROUPS; ++j) {
+          const uint32_t at = kb + k_at[c % PIECES_BOX] + (c / PIECES_BOX) * (KEYS * TL::kRow) + 16 * j * TL::kRow;
+          const uint4 us = lds128(at), vs = lds128(at + 8 * TL::kRow);
+          const uint32_t u[4] = {us.x, us.y, us.z, us.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 u = lds128(kb + k_at[c % PIECES_BOX] + (c / PIECES_BOX) * (KEYS * TL::kRow) + (16 * j + 8 * h) * TL::kRow);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          for (int i = 0; i < STEPS; ++i) {
+            uint32_t x[4];
             if constexpr (F8) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) mma<M, NR>(s[j][h], qs[i], halves_of_codes(w[i]), halves_of_codes(w[i] >> 16));
+              x[0] = halves_of_codes(u[i]); x[1] = halves_of_codes(v[i]); x[2] = halves_of_codes(u[i] >> 16); x[3] = halves_of_codes(v[i] >> 16);
             } else {
-              mma<M, NR>(s[j][h], qs[0], w[0], w[1]);
-              mma<M, NR>(s[j][h], qs[1], w[2], w[3]);
+              x[0] = u[2 * i]; x[1] = v[2 * i]; x[2] = u[2 * i + 1]; x[3] = v[2 * i + 1];
             }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) mma<M>(s[j][r], x[0], x[1], x[2], x[3], qs[i][r], qs[i][NR + r]);
           }
+        }
       }
       // ---- running maxima --------------------------------------------------------------------------------------------------
       const int key0 = tile * KEYS;
       const bool masked = tile < clear0 || tile >= clear1;
-      float mx[NR], mt[NR], lv[GROUPS];
+      float mx[NR][2], mt[NR][2], lv[GROUPS];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) mx[r] = mt[r] = -INFINITY;
+      for (int r = 0; r < NR; ++r) mx[r][0] = mx[r][1] = mt[r][0] = mt[r][1] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         float ks = 1.f;
@@ -501,72 +529,81 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
           lv[j] = sc.y == sc.y ? sc.y : 0.f;
         }
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float f = factor[r] * ks;
-          float top_j = -INFINITY;
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = s[j][h][2 * r + e] * f;
-              if (masked) {
-                const int key = key0 + 16 * j + 8 * h + (e == 0 ? 2 * t : (2 * t + 1) ^ 4);
-                if (key > pos[r] || (a.window > 0 && key <= pos[r] - a.window)) v = -INFINITY;
-              }
-              s[j][h][2 * r + e] = v;
-              top_j = fmaxf(top_j, v);
+          for (int e = 0; e < 2; ++e) {
+            const float f = by_row[r][e] * ks;
+            float v = s[j][r][e] * f, w = s[j][r][2 + e] * f;
+            if (masked) {
+              const int key = key0 + 16 * j + pi, p = pos[r][e];
+              if (key > p || (a.window > 0 && key <= p - a.window)) v = -INFINITY;
+              if (key + 8 > p || (a.window > 0 && key + 8 <= p - a.window)) w = -INFINITY;
             }
-          mx[r] = fmaxf(mx[r], top_j);
-          if (F8) mt[r] = fmaxf(mt[r], top_j + lv[j]);
-        }
+            s[j][r][e] = v;
+            s[j][r][2 + e] = w;
+            const float top_j = fmaxf(v, w);
+            mx[r][e] = fmaxf(mx[r][e], top_j);
+            if (F8) mt[r][e] = fmaxf(mt[r][e], top_j + lv[j]);
+          }
       }
       bool grew = false;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        if (F8) {
-          mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xffffffffu, mt[r], 1));
-          mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xffffffffu, mt[r], 2));
-        } else {
-          mt[r] = mx[r];
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          grew |= mx[r][e] > m[r][e];
+          if (F8) grew |= mt[r][e] > top[r][e];
         }
-        grew |= mx[r] > m[r] || mt[r] > top[r];
-      }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float m_new = fmaxf(m[r], mx[r]), t_new = fmaxf(top[r], mt[r]);
-          l[r] *= m[r] == m_new ? 1.f : pt_exp2(m[r] - m_new);
-          const float f = top[r] == t_new ? 1.f : pt_exp2(top[r] - t_new);
-          m[r] = m_new;
-          top[r] = t_new;
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int i = 0; i < NTILES; ++i) {
-            o[i][2 * r] *= f;
-            o[i][2 * r + 1] *= f;
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              mx[r][e] = fmaxf(mx[r][e], __shfl_xor_sync(0xffffffffu, mx[r][e], x));
+              if (F8) mt[r][e] = fmaxf(mt[r][e], __shfl_xor_sync(0xffffffffu, mt[r][e], x));
+            }
+            const float m_new = fmaxf(m[r][e], mx[r][e]), t_new = F8 ? fmaxf(top[r][e], mt[r][e]) : m_new;
+            l[r][e] *= m[r][e] == m_new ? 1.f : pt_exp2(m[r][e] - m_new);
+            const float f = top[r][e] == t_new ? 1.f : pt_exp2(top[r][e] - t_new);
+            m[r][e] = m_new;
+            top[r][e] = t_new;
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+              o[i][r][e] *= f;
+              o[i][r][2 + e] *= f;
+            }
           }
-        }
       }
-      // ---- probabilities and their product with the values --------------------------------------------------------------------
+      // ---- probabilities, turned so that a lane holds row g's keys 2 t and 2 t + 1, and their product with the values ----------------
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
-        uint32_t pa[2 * NR];
+        uint32_t pb[NR][2];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          const float ref = m[r] == -INFINITY ? 0.f : m[r];
-          // 16-bit pages: no scales, top == m
-          const float by = F8 ? (lv[j] == -INFINITY ? 0.f : pt_exp2(fminf(lv[j] + ref - top[r], 100.f) + kShift)) : (__is_same(M, __half) ? 256.f : 1.f);
+          float p[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p0 = pt_exp2(s[j][h][2 * r] - ref), p1 = pt_exp2(s[j][h][2 * r + 1] - ref);
-            l[r] += p0 + p1;
-            pa[h * NR + r] = Num<M>::pack(p0 * by, p1 * by);
+          for (int e = 0; e < 2; ++e) {
+            const float ref = m[r][e] == -INFINITY ? 0.f : m[r][e];
+            // 16-bit pages: no scales, top == m
+            const float by = F8 ? (lv[j] == -INFINITY ? 0.f : pt_exp2(fminf(lv[j] + ref - top[r][e], 100.f) + kShift)) : (__is_same(M, __half) ? 256.f : 1.f);
+            p[e] = pt_exp2(s[j][r][e] - ref);
+            p[2 + e] = pt_exp2(s[j][r][2 + e] - ref);
+            l[r][e] += p[e] + p[2 + e];
+            p[e] *= by;
+            p[2 + e] *= by;
           }
+          pb[r][0] = transposed(Num<M>::pack(p[0], p[1]));
+          pb[r][1] = transposed(Num<M>::pack(p[2], p[3]));
         }
         // what lies past the sequence's end may be no number, and nothing times that neither
         const int left = masked ? sh.s.len - (key0 + 16 * j) : 16;
         const uint32_t v0 = vb + v_at[0] + 16 * j * TL::kRow, v1 = vb + v_at[1] + 16 * j * TL::kRow;
+        const auto times = [&](int tile_of, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) mma<M>(o[tile_of][r], a0, a1, a2, a3, pb[r][0], pb[r][1]);
+        };
         // codes e of two words -> two halves
         const auto pair = [](uint32_t x, uint32_t y, int e) { return halves_of_codes(pt_prmt(x, y, (4 + e) << 4 | e)); };
         if constexpr (F8 && D == 64) {
@@ -578,8 +615,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             if (((2 * t + 1) ^ 4) + 8 >= left) u = make_uint2(0u, 0u);
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mma<M, NR>(o[i], pa, pair(i < 4 ? x.x : x.y, i < 4 ? y.x : y.y, i & 3), pair(i < 4 ? z.x : z.y, i < 4 ? u.x : u.y, i & 3));
+          for (int e = 0; e < 4; e += 2) {
+            times(e / 2, pair(x.x, y.x, e), pair(x.x, y.x, e + 1), pair(z.x, u.x, e), pair(z.x, u.x, e + 1));
+            times(2 + e / 2, pair(x.y, y.y, e), pair(x.y, y.y, e + 1), pair(z.y, u.y, e), pair(z.y, u.y, e + 1));
+          }
         } else {
 #pragma unroll
           for (int c = 0; c < TL::kBoxes; ++c) {
@@ -596,10 +635,9 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             for (int w = 0; w < 4; ++w) {
               if constexpr (F8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma<M, NR>(o[c * 16 + 4 * w + e], pa, pair(x[w], y[w], e), pair(z[w], u[w], e));
+                for (int e = 0; e < 4; e += 2) times(c * 8 + 2 * w + e / 2, pair(x[w], y[w], e), pair(x[w], y[w], e + 1), pair(z[w], u[w], e), pair(z[w], u[w], e + 1));
               } else {
-                mma<M, NR>(o[c * 8 + 2 * w], pa, pt_prmt(x[w], y[w], 0x5410), pt_prmt(z[w], u[w], 0x5410));
-                mma<M, NR>(o[c * 8 + 2 * w + 1], pa, pt_prmt(x[w], y[w], 0x7632), pt_prmt(z[w], u[w], 0x7632));
+                times(c * 4 + w, pt_prmt(x[w], y[w], 0x5410), pt_prmt(x[w], y[w], 0x7632), pt_prmt(z[w], u[w], 0x5410), pt_prmt(z[w], u[w], 0x7632));
               }
             }
           }
@@ -612,37 +650,39 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     // ---- the piece's result: in units of 2^top where the keys have scales, l over the lanes of a row ----------------------------------
     constexpr float kUndo = __is_same(M, __half) ? 1.f / 256.f : 1.f;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (!F8) top[r] = m[r];
-    }
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], x);
+        if (!F8) top[r][e] = m[r][e];
+      }
     const bool done = sh.begins && sh.ends;
     const int slot = first_piece ? 0 : 1, piece = 2 * blockIdx.x + slot;
     const long long first_row = sh.s.row;
-    // channels c * 8 kRun + 2 t kRun + (0 .. 2 kRun - 1) of rows g and g + 8: o[c kRun + i][e] is the one at e kRun + i
+    // channels 8 kRun c + kRun g + 4 q .. + 3 of row (r, e)
+    const auto four = [&](int r, int e, int c, int q, float f) {
+      const int k = c * (TL::kRun / 2) + 2 * q;
+      return make_float4(o[k][r][e] * f, o[k][r][2 + e] * f, o[k + 1][r][e] * f, o[k + 1][r][2 + e] * f);
+    };
     if constexpr (ROWS == 16) {
-      constexpr int SLICE = FM::kSlice, TILES = SLICE / 8;
+      // 32 channels at a time: four of each of a box's eight runs
 #pragma unroll
-      for (int part = 0; part < D / SLICE; ++part) {
+      for (int part = 0; part < D / 32; ++part) {
+        const int c = part / (TL::kRun / 4), q = part % (TL::kRun / 4);
         asm volatile("bar.sync 1, 128;" ::: "memory");                      // the last sums are no longer read
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          if (t == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + g + 8 * r) * 4) = make_float4(m[r], l[r], top[r], 0.f);
-          float* dst = s_sum + (warp * 8 * NR + g + 8 * r) * SLICE;
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int c = 0; c < TILES / TL::kRun; ++c)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int i = 0; i < TL::kRun; i += 4) {
-                const int k = part * TILES + c * TL::kRun + i;
-                *reinterpret_cast<float4*>(dst + c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i) = make_float4(o[k][2 * r + e], o[k + 1][2 * r + e], o[k + 2][2 * r + e], o[k + 3][2 * r + e]);
-              }
-        }
+          for (int e = 0; e < 2; ++e) {
+            const int row = 8 * r + 2 * t + e;
+            if (part == 0 && g == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + row) * 4) = make_float4(m[r][e], l[r][e], top[r][e], 0.f);
+            *reinterpret_cast<float4*>(s_sum + (warp * 8 * NR + row) * 32 + 4 * g) = four(r, e, c, q, 1.f);
+          }
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        for (int i = tid * 4; i < used * SLICE; i += kWarps * 32 * 4) {
-          const int r = i / SLICE, d = part * SLICE + i % SLICE;
+        const int r = tid >> 3;
+        if (r < used) {
+          const int d = (8 * c + (tid & 7)) * TL::kRun + 4 * q;
           float mm = -INFINITY, tt = -INFINITY;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
@@ -657,7 +697,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
             if (st.x != -INFINITY || st.y != 0.f) ll += st.y * (st.x == -INFINITY ? 1.f : pt_exp2(st.x - mm));
             const float f = st.z == -INFINITY ? (st.y != st.y ? 1.f : 0.f) : pt_exp2(st.z - tt);
-            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * SLICE + i % SLICE);
+            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * 32 + 4 * (tid & 7));
             v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
           }
           if (done) {
@@ -672,26 +712,25 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const int in_tile = warp_row + g + 8 * r, row = sh.row_tile * ROWS + in_tile;
-        if (in_tile >= used) continue;
-        const float f = !done ? kUndo : l[r] > 0.f || l[r] != l[r] ? kUndo * (F8 ? pt_exp2(top[r] - m[r]) : 1.f) / l[r] : 0.f;
-        T* dst = static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D;
-        float* sums = part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(in_tile) * D;
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int c = 0; c < NTILES / TL::kRun; ++c)
+        for (int e = 0; e < 2; ++e) {
+          const int in_tile = warp_row + 8 * r + 2 * t + e, row = sh.row_tile * ROWS + in_tile;
+          if (in_tile >= used) continue;
+          const float ll = l[r][e], f = !done ? kUndo : ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(top[r][e] - m[r][e]) : 1.f) / ll : 0.f;
+          T* dst = static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D;
+          float* sums = part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(in_tile) * D;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int c = 0; c < D / (8 * TL::kRun); ++c)
 #pragma unroll
-            for (int i = 0; i < TL::kRun; i += 4) {
-              const int d = c * 8 * TL::kRun + (2 * t + e) * TL::kRun + i;
-              const float4 v = make_float4(o[c * TL::kRun + i][2 * r + e] * f, o[c * TL::kRun + i + 1][2 * r + e] * f, o[c * TL::kRun + i + 2][2 * r + e] * f,
-                                           o[c * TL::kRun + i + 3][2 * r + e] * f);
+            for (int q = 0; q < TL::kRun / 4; ++q) {
+              const int d = (8 * c + g) * TL::kRun + 4 * q;
+              const float4 v = four(r, e, c, q, f);
               if (done) write4(dst + d, v);
               else *reinterpret_cast<float4*>(sums + d) = v;
             }
-        if (!done && t == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + in_tile * 4) = make_float4(m[r], l[r], top[r], 0.f);
-      }
+          if (!done && g == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + in_tile * 4) = make_float4(m[r][e], ll, top[r][e], 0.f);
+        }
     }
     if (sh.begins && !sh.ends) head = {sh.s.row, sh.head, used, static_cast<int>((sh.item_end - 1) / sh.per), slot, {sh.row_tile, 0, 0}};
     first_piece = false;
@@ -791,8 +830,8 @@ int paged_form(const PagedCall& call) {
   }
   const PagedAttnArgs& a = *call.a;
   CUtensorMap mk, mv;
-  int r = page_map<F8, D, tile_keys(ROWS)>(&mk, a.k_pages, a);
-  if (r == 0) r = page_map<F8, D, tile_keys(ROWS)>(&mv, a.v_pages, a);
+  int r = page_map<F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mk, a.k_pages, a);
+  if (r == 0) r = page_map<F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mv, a.v_pages, a);
   if (r != 0) return r;
   const int R = a.H / a.G;
   const long long items = (a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS)) * a.G;
@@ -836,7 +875,8 @@ extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int
   if (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) return -2;
   if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64) || (!a.whole && (a.part == nullptr || a.ctas <= 0))) return -3;
   // a sequence's work and the pages' rows are counted in 32 bits
-  const long long tiles = (static_cast<long long>(a.width) * a.P + tile_keys(rows) - 1) / tile_keys(rows);
+  const int keys = tile_keys(rows, a.D * (a.k_scale ? 1 : 2));
+  const long long tiles = (static_cast<long long>(a.width) * a.P + keys - 1) / keys;
   if ((static_cast<long long>(a.rows) * (a.H / a.G) / rows + 1) * a.G * tiles > 0x7fffffffLL || static_cast<long long>(a.pages) * a.G > 0x7fffffffLL) return -4;
   if (static_cast<long long>(a.width) * a.P > 0x7fffffffLL || static_cast<long long>(a.rows) * a.H > 0x7fffffffLL) return -5;
   return paged_type(PagedCall{&a, (cudaStream_t)stream}, dtype, a.k_scale != nullptr, a.D, rows, a.starts == nullptr && a.H / a.G <= 8);

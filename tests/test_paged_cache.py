@@ -335,6 +335,22 @@ def test_attention_gpu(case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R, P, D, cache", ((5, 16, 128, pc.E4M3), (6, 32, 256, pc.E4M3), (12, 64, 128, pc.E4M3), (8, 16, 64, pc.E4M3), (4, 32, 128, torch.bfloat16), (2, 128, 256, torch.bfloat16)))
+def test_repeated_steps_agree(R, P, D, cache):
+    """Whatever order the copies of a step's tiles arrive in: every one of many repetitions gives the same bits."""
+    lens = [37 * n % 2900 + 1 for n in range(60)]
+    batch = Batch(held=lens, new=[1] * 60, G=4, R=R, P=P, D=D, dtype=torch.bfloat16, cache=cache, dev="cuda", decode=True, strided=False)
+    want = paged_attention(batch.q, batch.store, *batch.args)
+    check_attention(batch, want)
+    flush = torch.empty(2 ** 26, device="cuda")
+    for i in range(150):
+        if i % 5 == 0:
+            flush.zero_()                                      # the pages come from memory again
+        assert torch.equal(paged_attention(batch.q, batch.store, *batch.args), want)
+    _common.raise_on_device_error()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("decode", (True, False))
 def test_value_scales_of_any_spread(decode):
     """Values of one page 2^60 times another's, the large ones where the scores are least; and pages of nothing but zeros."""

@@ -311,7 +311,7 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     work = None
     if not whole:
         row_tiles = rows * R // tile + B if starts is not None else B * -(-R // tile)
-        ctas = min(row_tiles * G * -(-width * P // (32 if tile == 16 else 64)), _resident(store.index, number, f8, D, tile, starts is None and R <= 8))
+        ctas = min(row_tiles * G * -(-width * P // 16), _resident(store.index, number, f8, D, tile, starts is None and R <= 8))
         work = torch.empty(ctas * (8 + 2 * tile * (4 + D)), dtype=torch.float32, device=device)
     packed = _ATTEND.pack(q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), store.k_scale.data_ptr() if f8 else 0, store.v_scale.data_ptr() if f8 else 0,
                           table.data_ptr(), lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if whole else work.data_ptr(), err_word(device).data_ptr(),
