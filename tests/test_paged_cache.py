@@ -401,7 +401,7 @@ def test_operands_reach_the_kernels_aligned():
     for t in (x, x.transpose(0, 1), torch.arange(4 * 3 * 65, dtype=torch.bfloat16).view(4, 3, 65)[..., 1:], torch.arange(4 * 200, dtype=torch.bfloat16).view(4, 200)[:, 8:].unflatten(1, (3, 64))):
         y = pc._rows_of(t)
         assert torch.equal(y, t) and y.data_ptr() % 16 == 0 and y.stride(2) == 1 and all(s % 8 == 0 for s in y.stride()[:2])
-    w = pc._aligned(x[0, 0])
+    w = pc._aligned(x[0, 0], torch.bfloat16)
     assert torch.equal(w, x[0, 0]) and w.data_ptr() % 16 == 0
     assert pc._rows_of(y) is y
 

@@ -29,6 +29,8 @@ PAGE_SIZES = (16, 32, 64, 128)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 # capacity up to which the keys of a (sequence, head) are not cut into pieces
 WHOLE_MAX_KEYS = 256
+# tiles of 16 keys that a share of the work has at least: two for each warp
+LEAST_TILES = 8
 
 
 @register_signatures
@@ -127,7 +129,9 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if one == 1 and (row | head) & 7 == 0 and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
+def _aligned(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if t.dtype != dtype:
+        t = t.to(dtype)
     return t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -243,18 +247,29 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     if half % 8:
         raise ValueError(f"paged_append: the rotation turns a multiple of 16 channels, got {2 * half}")
     k, v = _rows_of(k), _rows_of(v)
+    (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
+    cos_at = sin_at = q_weight_at = k_weight_at = q_at = out_at = q_row = q_head = 0
     if half:
-        cos, sin = (t if t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() & 15 == 0 else _aligned(t.float()) for t in (cos, sin))
-    q_weight, k_weight = (None if w is None else _aligned(w.to(dtype)) for w in (q_weight, k_weight))
-    device, out, q_stride = k.device, None, (0, 0)
+        cos, sin = _aligned(cos, torch.float32), _aligned(sin, torch.float32)
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+    if k_weight is not None:
+        k_weight = _aligned(k_weight, dtype)
+        k_weight_at = k_weight.data_ptr()
+    out = None
     if q is not None:
+        if q_weight is not None:
+            q_weight = _aligned(q_weight, dtype)
+            q_weight_at = q_weight.data_ptr()
         q = _rows_of(q)
-        out, q_stride = torch.empty((rows, H, D), dtype=dtype, device=device), q.stride()
-    k_stride, v_stride = k.stride(), v.stride()
-    at = lambda t: 0 if t is None else t.data_ptr()
-    packed = _APPEND.pack(at(q), k.data_ptr(), v.data_ptr(), at(out), store.k.data_ptr(), store.v.data_ptr(), at(store.k_scale), at(store.v_scale), table.data_ptr(),
-                          lengths.data_ptr(), at(starts), at(cos), at(sin), at(q_weight), at(k_weight), err_word(device).data_ptr(), q_stride[0], q_stride[1], k_stride[0],
-                          k_stride[1], v_stride[0], v_stride[1], table_row, rows, B, H, G, D, P, pages, width, positions, half, one_plus_w, eps)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_at, out_at, (q_row, q_head, _) = q.data_ptr(), out.data_ptr(), q.stride()
+    k_scale_at = v_scale_at = 0
+    if store.k_scale is not None:
+        k_scale_at, v_scale_at = store.k_scale.data_ptr(), store.v_scale.data_ptr()
+    device = k.device
+    packed = _APPEND.pack(q_at, k.data_ptr(), v.data_ptr(), out_at, store.k.data_ptr(), store.v.data_ptr(), k_scale_at, v_scale_at, table.data_ptr(), lengths.data_ptr(),
+                          0 if starts is None else starts.data_ptr(), cos_at, sin_at, q_weight_at, k_weight_at, err_word(device).data_ptr(), q_row, q_head, k_row, k_head,
+                          v_row, v_head, table_row, rows, B, H, G, D, P, pages, width, positions, half, one_plus_w, eps)
     check(lib().tyr_paged_append(packed, number, cur_stream(device)), "paged_append")
     return out
 
@@ -305,13 +320,13 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     number = _on_gpu("paged_attention", store, dtype)
     q, f8 = _rows_of(q), store.k_scale is not None
     stride, R = q.stride(), H // G
-    out = torch.empty((rows, H, D), dtype=dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     tile = 64 if starts is not None and rows * R > 16 * B else 16
     whole = width * P <= WHOLE_MAX_KEYS
     work = None
     if not whole:
         row_tiles = rows * R // tile + B if starts is not None else B * -(-R // tile)
-        ctas = min(row_tiles * G * -(-width * P // 16), _resident(store.index, number, f8, D, tile, starts is None and R <= 8))
+        ctas = min(-(-row_tiles * G * -(-width * P // 16) // LEAST_TILES), _resident(store.index, number, f8, D, tile, starts is None and R <= 8))
         work = torch.empty(ctas * (8 + 2 * tile * (4 + D)), dtype=torch.float32, device=device)
     packed = _ATTEND.pack(q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), store.k_scale.data_ptr() if f8 else 0, store.v_scale.data_ptr() if f8 else 0,
                           table.data_ptr(), lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if whole else work.data_ptr(), err_word(device).data_ptr(),
