@@ -41,6 +41,7 @@ template <> struct Pair<__half> {
   }
 };
 
+// Eight channels of a lane are two runs of four: `raw` holds them as they lie in memory.
 template <typename T>
 __device__ __forceinline__ void pa_unpack8(const uint4& u, float (&f)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -49,13 +50,6 @@ __device__ __forceinline__ void pa_unpack8(const uint4& u, float (&f)[8]) {
     const float2 t = Pair<T>::get(w[i]);
     f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
-}
-__device__ __forceinline__ uint4 pa_raw8(const void* p) { return *reinterpret_cast<const uint4*>(p); }
-template <typename T>
-__device__ __forceinline__ void pa_load8(const T* p, float (&f)[8]) { pa_unpack8<T>(pa_raw8(p), f); }
-template <typename T>
-__device__ __forceinline__ void pa_store8(T* p, const float (&f)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::put(f[0], f[1]), Pair<T>::put(f[2], f[3]), Pair<T>::put(f[4], f[5]), Pair<T>::put(f[6], f[7]));
 }
 __device__ __forceinline__ uint2 pa_codes8(const float (&f)[8], float inv) {      // zeros for a scale that is NaN (inv 0): codes are numbers always
   if (inv == 0.f) return make_uint2(0u, 0u);
@@ -91,24 +85,41 @@ __device__ __forceinline__ float pa_scale(uint32_t bits) {
 __device__ __forceinline__ float pa_joined(float want, float old) { return want != want || old != old ? __uint_as_float(0x7fffffffu) : fmaxf(want, old); }
 __device__ __forceinline__ float pa_inverse(float scale) { return scale == scale ? 1.f / scale : 0.f; }
 
-// Eight channels of a head on each of D / 8 neighbouring lanes, all of whose rows are at `pos`.
+// A head on D / 8 neighbouring lanes, all of whose rows are at one position.  Of the rotated part a lane has four channels and the four that they turn with, so that
+// the rotation needs no other lane; of the rest eight in a row.
 struct HeadLanes {
-  int lane, lanes, l8, half;
+  int lane, lanes, lo, hi;                     // channels lo .. lo + 3 and hi .. hi + 3
+  bool turned;
   uint32_t mask;
-  float c[8], s[8];
+  float4 c, s;
   __device__ __forceinline__ HeadLanes(const PagedAppendArgs& a, int thread)
-      : lanes(a.D >> 3), half(a.half), mask(a.D == 256 ? 0xffffffffu : ((1u << (a.D >> 3)) - 1u) << ((threadIdx.x & 31) & ~((a.D >> 3) - 1))) {
+      : lanes(a.D >> 3), mask(a.D == 256 ? 0xffffffffu : ((1u << (a.D >> 3)) - 1u) << ((threadIdx.x & 31) & ~((a.D >> 3) - 1))) {
     lane = thread & (lanes - 1);
-    l8 = lane * 8;
+    const int pairs = a.half >> 2;
+    turned = lane < pairs;
+    lo = turned ? 4 * lane : 2 * a.half + 8 * (lane - pairs);
+    hi = turned ? a.half + lo : lo + 4;
+  }
+  template <typename T>
+  __device__ __forceinline__ uint4 raw(const T* head) const {
+    const uint2 x = *reinterpret_cast<const uint2*>(head + lo), y = *reinterpret_cast<const uint2*>(head + hi);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* head, const float (&f)[8]) const {
+    *reinterpret_cast<uint2*>(head + lo) = make_uint2(Pair<T>::put(f[0], f[1]), Pair<T>::put(f[2], f[3]));
+    *reinterpret_cast<uint2*>(head + hi) = make_uint2(Pair<T>::put(f[4], f[5]), Pair<T>::put(f[6], f[7]));
+  }
+  __device__ __forceinline__ void store_codes(uint8_t* head, const float (&f)[8], float inv) const {
+    const uint2 u = pa_codes8(f, inv);
+    *reinterpret_cast<uint32_t*>(head + lo) = u.x;
+    *reinterpret_cast<uint32_t*>(head + hi) = u.y;
   }
   __device__ __forceinline__ void turns(const PagedAppendArgs& a, int pos) {
-    if (l8 >= 2 * half) return;
-    const long long at = static_cast<long long>(pos) * half + (l8 < half ? l8 : l8 - half);
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(a.cos + at + i);
-      *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(a.sin + at + i);
-    }
+    if (!turned) return;
+    const long long at = static_cast<long long>(pos) * a.half + lo;
+    c = *reinterpret_cast<const float4*>(a.cos + at);
+    s = *reinterpret_cast<const float4*>(a.sin + at);
   }
   // norm and rotation of the lanes' channels, in 32 bits throughout
   template <typename T>
@@ -120,17 +131,17 @@ struct HeadLanes {
       for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
       const float r = rsqrtf(ss / a.D + a.eps);
       float w[8];
-      pa_load8(weight + l8, w);
+      pa_unpack8<T>(raw(weight), w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = f[i] * r * (a.one_plus_w ? 1.f + w[i] : w[i]);
     }
-    if (half > 0) {
-      const bool turned = l8 < 2 * half;
-      const int other = turned ? (l8 < half ? lane + (half >> 3) : lane - (half >> 3)) : lane;
+    if (turned) {
+      const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = __shfl_sync(mask, f[i], other, lanes);
-        if (turned) f[i] = l8 < half ? f[i] * c[i] - w * s[i] : f[i] * c[i] + w * s[i];
+      for (int i = 0; i < 4; ++i) {
+        const float x = f[i], y = f[4 + i];
+        f[i] = x * cs[i] - y * sn[i];
+        f[4 + i] = x * sn[i] + y * cs[i];
       }
     }
   }
@@ -172,11 +183,12 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const __grid_con
   const T* src = is_q ? static_cast<const T*>(a.q) + b * a.q_row + hd * a.q_head
                       : (is_v ? static_cast<const T*>(a.v) + b * a.v_row + hd * a.v_head : static_cast<const T*>(a.k) + b * a.k_row + hd * a.k_head);
   float f[8];
-  pa_load8(src + hl.l8, f);
+  pa_unpack8<T>(hl.raw(src), f);
   const NewRows nr = pa_new_rows(a, b);
-  T* q_out = static_cast<T*>(a.q_out) + (static_cast<long long>(b) * a.H + hd) * a.D + hl.l8;
+  T* q_out = static_cast<T*>(a.q_out) + (static_cast<long long>(b) * a.H + hd) * a.D;
   if (nr.n == 0) {
-    if (is_q) *reinterpret_cast<uint4*>(q_out) = make_uint4(0u, 0u, 0u, 0u);
+    const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (is_q) hl.store(q_out, none);
     return;
   }
   const int page = is_q ? 0 : pa_page(a, b, nr.first / a.P);
@@ -190,7 +202,7 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const __grid_con
     hl.finish(a, static_cast<const T*>(is_q ? a.q_weight : a.k_weight), f);
   }
   if (is_q) {
-    pa_store8(q_out, f);
+    hl.store(q_out, f);
     return;
   }
   void* pages = is_v ? a.v_pages : a.k_pages;
@@ -207,10 +219,10 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const __grid_con
         *reinterpret_cast<uint4*>(tile + i) = u;
       }
     }
-    *reinterpret_cast<uint2*>(tile + slot * a.D + hl.l8) = pa_codes8(f, pa_inverse(scale));
+    hl.store_codes(tile + slot * a.D, f, pa_inverse(scale));
     if (hl.lane == 0) scales[at] = scale;
   } else {
-    pa_store8(static_cast<T*>(pages) + (at * a.P + slot) * a.D + hl.l8, f);
+    hl.store(static_cast<T*>(pages) + (at * a.P + slot) * a.D, f);
   }
 }
 
@@ -233,7 +245,7 @@ constexpr int kQueryHeads = 8;             // of a row that D / 8 lanes take, fo
 // One block per (page, head, keys or values) holds the page's new rows in registers between the maximum and the codes, IT vectors a thread; after the
 // `page_units` of them, blocks for the queries.
 template <typename T, bool F8, int IT>
-__global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int page_units) {
+__global__ void __launch_bounds__(IT == 8 ? 512 : 256, IT == 8 ? 1 : 4) paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int page_units) {
   pdl_entry();
   HeadLanes hl(a, threadIdx.x);
   const int groups = blockDim.x / hl.lanes, group = threadIdx.x / hl.lanes;
@@ -248,20 +260,20 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
     const NewRows nr = pa_new_rows(a, b);
     const bool there = row >= nr.row && row < nr.row + nr.n;
     if (there) hl.turns(a, nr.first + row - nr.row);
-    const T* src = static_cast<const T*>(a.q) + row * a.q_row + hl.l8;
-    T* dst = static_cast<T*>(a.q_out) + static_cast<long long>(row) * a.H * a.D + hl.l8;
+    const T* src = static_cast<const T*>(a.q) + row * a.q_row;
+    T* dst = static_cast<T*>(a.q_out) + static_cast<long long>(row) * a.H * a.D;
 #pragma unroll
     for (int h = h0; h < h0 + kQueryHeads; h += 4) {
       uint4 raw[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = there && h + i < a.H ? pa_raw8(src + (h + i) * a.q_head) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 4; ++i) raw[i] = there && h + i < a.H ? hl.raw(src + (h + i) * a.q_head) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (h + i >= a.H) break;
         float f[8];
         pa_unpack8<T>(raw[i], f);
         if (there) hl.finish(a, static_cast<const T*>(a.q_weight), f);
-        pa_store8(dst + (h + i) * a.D, f);
+        hl.store(dst + (h + i) * a.D, f);
       }
     }
     return;
@@ -280,11 +292,11 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
   const int slot0 = lo - static_cast<int>(j) * a.P, row0 = nr.row + lo - nr.first, n = hi - lo;
   float f[IT][8];
   uint32_t m = 0;
-  const T* src = is_v ? static_cast<const T*>(a.v) + row0 * a.v_row + hd * a.v_head + hl.l8 : static_cast<const T*>(a.k) + row0 * a.k_row + hd * a.k_head + hl.l8;
+  const T* src = is_v ? static_cast<const T*>(a.v) + row0 * a.v_row + hd * a.v_head : static_cast<const T*>(a.k) + row0 * a.k_row + hd * a.k_head;
   const long long step = is_v ? a.v_row : a.k_row;
   uint4 raw[IT];
 #pragma unroll
-  for (int it = 0; it < IT; ++it) raw[it] = it * groups + group < n ? pa_raw8(src + (it * groups + group) * step) : make_uint4(0u, 0u, 0u, 0u);
+  for (int it = 0; it < IT; ++it) raw[it] = it * groups + group < n ? hl.raw(src + (it * groups + group) * step) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int i = it * groups + group;
@@ -318,7 +330,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int i = it * groups + group;
-      if (i < n) *reinterpret_cast<uint2*>(tile + (slot0 + i) * a.D + hl.l8) = pa_codes8(f[it], inv);
+      if (i < n) hl.store_codes(tile + (slot0 + i) * a.D, f[it], inv);
     }
     if (threadIdx.x == 0) scales[at] = scale;
   } else {
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int i = it * groups + group;
-      if (i < n) pa_store8(tile + (slot0 + i) * a.D + hl.l8, f[it]);
+      if (i < n) hl.store(tile + (slot0 + i) * a.D, f[it]);
     }
   }
 }
@@ -363,7 +375,7 @@ extern "C" TYR_EXPORT int tyr_paged_append(const void* packed, int dtype, void* 
   const PagedAppendArgs& a = *static_cast<const PagedAppendArgs*>(packed);
   if (a.rows <= 0 || a.B <= 0 || a.H < 0 || a.G <= 0 || a.pages <= 0 || a.width <= 0) return -1;
   if ((a.D != 64 && a.D != 128 && a.D != 256) || (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128)) return -2;
-  if (a.half < 0 || a.half % 8 != 0 || 2 * a.half > a.D || (a.half > 0 && (a.cos == nullptr || a.sin == nullptr))) return -3;
+  if (a.half < 0 || a.half % 4 != 0 || 2 * a.half > a.D || (a.half > 0 && (a.cos == nullptr || a.sin == nullptr))) return -3;
   if ((a.q != nullptr) != (a.q_out != nullptr) || (a.k_scale != nullptr) != (a.v_scale != nullptr)) return -4;
   const bool f8 = a.k_scale != nullptr;
   if (dtype == 0) return f8 ? paged_append_launch<__nv_bfloat16, true>(a, (cudaStream_t)stream) : paged_append_launch<__nv_bfloat16, false>(a, (cudaStream_t)stream);

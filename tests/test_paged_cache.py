@@ -198,6 +198,8 @@ APPENDS = [
     (RAGGED, False, 4, 2, 64, 128, torch.float16, pc.E4M3, 16, False),
     (RAGGED, False, 2, 1, 128, 256, torch.bfloat16, pc.E4M3, 128, True),
     (RAGGED, False, 2, 2, 64, 64, torch.bfloat16, torch.bfloat16, None, True),
+    (STEPS, True, 2, 3, 16, 128, torch.bfloat16, pc.E4M3, 12, True),
+    (RAGGED, False, 2, 1, 32, 64, torch.float16, pc.E4M3, 20, True),
     (dict(held=[0], new=[1000]), False, 8, 6, 64, 128, torch.bfloat16, pc.E4M3, 64, False),
     (dict(held=[3] * 300, new=[n % 3 for n in range(300)]), False, 1, 2, 16, 64, torch.float16, pc.E4M3, 32, True),
 ]
@@ -449,7 +451,7 @@ def test_refusals_gpu():
     low = small("cuda", cache=torch.float16, dtype=torch.float16)
     for call in (
         lambda: paged_append(b.store, b.k.float(), b.v.float(), table, lens), lambda: paged_append(b.store, cpu.k, cpu.v, table, lens), lambda: paged_append(b.store, b.k, b.v, cpu.table, lens),
-        lambda: paged_append(b.store, b.k, b.v, table, lens, **turns(30, 12, "cuda")), lambda: paged_append(b.store, b.k, b.v, table, lens, **turns(30, 16, "cpu")),
+        lambda: paged_append(b.store, b.k, b.v, table, lens, **turns(30, 10, "cuda")), lambda: paged_append(b.store, b.k, b.v, table, lens, **turns(30, 16, "cpu")),
         lambda: paged_append(odd.store, odd.k, odd.v, *odd.args), lambda: paged_append(page.store, page.k, page.v, *page.args),
         lambda: paged_append(low.store, b.k, b.v, table, lens), lambda: paged_attention(b.q, low.store, table, lens), lambda: paged_attention(b.q.float(), b.store, table, lens),
         lambda: paged_attention(cpu.q, b.store, table, lens), lambda: paged_attention(odd.q, odd.store, *odd.args), lambda: paged_attention(page.q, page.store, *page.args),

@@ -244,8 +244,8 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     if dev < 0:
         return _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w)
     number = _on_gpu("paged_append", store, dtype)
-    if half % 8:
-        raise ValueError(f"paged_append: the rotation turns a multiple of 16 channels, got {2 * half}")
+    if half % 4:
+        raise ValueError(f"paged_append: the rotation turns a multiple of 8 channels, got {2 * half}")
     k, v = _rows_of(k), _rows_of(v)
     (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
     cos_at = sin_at = q_weight_at = k_weight_at = q_at = out_at = q_row = q_head = 0
