@@ -9,7 +9,7 @@
 //
 // One producer warp copies tiles of keys and values by TMA into a ring of stages (page by page, 128-byte swizzle), four consumer warps multiply with
 // mma.sync m16n8k16: either every warp takes tiles of its own (32 keys of 128 bytes) for the same 16 rows (ROWS 16: decoding, the warps' results are joined through shared
-// memory), or 16 of 64 rows for all tiles of 64 keys (ROWS 64: several new tokens).
+// memory), or 16 of 128 rows (of 64 with heads of 256) for all tiles of 64 keys (several new tokens).
 //
 // Every operand comes from shared memory in 16-byte pieces: the order of the channels within a product's sum is free as long as the queries follow it, and so is
 // the order of the keys as long as the values follow it.  The keys and the values are the products' first operands (16 of them, or 16 channels, by 8 rows; a second
@@ -29,8 +29,9 @@
 namespace tyr {
 
 // keys of a tile: while decoding some 8 KB of keys and values, a warp's own
-__host__ __device__ constexpr int tile_keys(int rows, int row_bytes) { return rows == 64 ? 64 : row_bytes <= 128 ? 32 : 16; }
-constexpr int kWarps = 4;                      // consumer warps
+__host__ __device__ constexpr int tile_keys(int rows, int row_bytes) { return rows > 16 ? 64 : row_bytes <= 128 ? 32 : 16; }
+// Consumer warps of a form: 16 rows each, or four with the same 16.
+__host__ __device__ constexpr int warps_of(int rows) { return rows == 16 ? 4 : rows / 16; }
 
 struct PagedAttnArgs {
   const void* q;                               // [rows, H, D]; element strides below
@@ -162,13 +163,15 @@ struct Tile {
   }
 };
 
-// Registers and shared memory of a form.  A CTA has five warps, and each quarter of an SM 16384 registers: three CTAs fit with 128 a thread, two with 168, one
-// with more; the fewer stages that many CTAs leave are enough while there are two.
+// Registers and shared memory of a form.  A CTA has five warps, and each quarter of an SM 16384 registers: three CTAs fit with 128 a thread, two (or one of nine
+// warps) with 168, one with more; the fewer stages that many CTAs leave are enough while there are two.
 template <bool F8, int D, int ROWS, int NR>
 struct Form {
   static constexpr int kKeys = tile_keys(ROWS, D * (F8 ? 1 : 2));
   using TL = Tile<F8, D, kKeys>;
-  static constexpr int kExtra = 1024 + 1024 + (D <= 128 ? 0 : (ROWS == 16 ? 1 : 4) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * 32 * 4 : 0);
+  static constexpr int kWarps = warps_of(ROWS), kThreads = (kWarps + 1) * 32;
+  static constexpr bool kQueriesInRegisters = D == 64 || (D == 128 && ROWS == 16);
+  static constexpr int kExtra = 1024 + 1024 + (kQueriesInRegisters ? 0 : (ROWS == 16 ? 1 : kWarps) * (D / 16) * 512) + (ROWS == 16 ? kWarps * 8 * NR * 32 * 4 : 0);
   // ROWS 16: a multiple of the warps, so that a stage is always the same warp's.  A warp that waits for a stage's next use has then seen its last one, and one bit
   // tells them apart.
   static constexpr int stages(int ctas) {
@@ -176,12 +179,12 @@ struct Form {
     return ROWS == 16 ? n / kWarps * kWarps : n;
   }
   static constexpr int kFew = ROWS == 16 ? 2 * kWarps : 2;                  // one in use and one on its way
-  static constexpr int kWanted = D == 64 ? (ROWS == 16 ? 3 : 2) : (ROWS == 64 ? 1 : NR == 1 ? (D == 128 ? 3 : 2) : (D == 128 ? 2 : 1));
+  static constexpr int kWanted = ROWS > 16 ? 1 : D == 64 ? 3 : (NR == 1 ? (D == 128 ? 3 : 2) : (D == 128 ? 2 : 1));
   static constexpr int kCtas = stages(kWanted) >= kFew ? kWanted : (kWanted > 1 && stages(kWanted - 1) >= kFew ? kWanted - 1 : 1);
   static constexpr int kStages = stages(kCtas) < 12 ? stages(kCtas) : 12;
   static_assert(kStages >= kFew, "shared memory");
   static constexpr int kSmem = kExtra + kStages * (2 * TL::kSize + 48);
-  static constexpr int kBound = kCtas == 3 ? 256 : (kCtas == 2 ? 192 : 160);      // threads of which two CTAs (or one) share the registers
+  static constexpr int kBound = kWarps == 8 ? 384 : kCtas == 3 ? 256 : (kCtas == 2 ? 192 : 160);      // threads of which two CTAs (or one) share the registers
   static constexpr int kAtOnce = kCtas == 1 ? 1 : 2;
 };
 
@@ -262,9 +265,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   using TL = Tile<F8, D, KEYS>;
   using M = typename std::conditional<F8, __half, T>::type;                 // operands of the products
   using FM = Form<F8, D, ROWS, NR>;
+  constexpr int kWarps = FM::kWarps, kSync = kWarps * 32;                   // threads that meet at the consumers' barrier
   constexpr int STAGES = FM::kStages, KSTEPS = D / 16, TILES = D / 16;
   constexpr int GROUPS = KEYS / 16;                                         // runs of 16 keys
-  constexpr bool QREG = D <= 128;                                           // the queries' fragments stay in registers
+  constexpr bool QREG = FM::kQueriesInRegisters;                                           // the queries' fragments stay in registers
   constexpr float kShift = 8.f;                                             // probabilities times 2^8: further from f16's small end
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   uint64_t* empty = full + STAGES;
   float* s_stats = reinterpret_cast<float*>(empty + STAGES);                // [4][16][4], joining warps (ROWS 16)
   uint4* s_q = reinterpret_cast<uint4*>(s_stats + 256);                     // fragments of the queries, QREG false: [warps that differ][KSTEPS][32]
-  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : 4) * KSTEPS * 32));   // [4][8 NR][32] (ROWS 16)
+  float* s_sum = reinterpret_cast<float*>(s_q + (QREG ? 0 : (ROWS == 16 ? 1 : kWarps) * KSTEPS * 32));   // [4][8 NR][32] (ROWS 16)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     // ---- queries: row g (and g + 8) in fragments; the scores' rows are 2 t and 2 t + 1 (and 8 further) ----------------------------
     uint32_t qa[QREG ? KSTEPS : 1][2 * NR];
     float factor[NR];
-    if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");                // the last piece's fragments are no longer read
+    if (!QREG) asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");                // the last piece's fragments are no longer read
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int in_tile = warp_row + g + 8 * r, row = sh.row_tile * ROWS + in_tile, i = row / R;
@@ -428,7 +432,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         }
       }
     }
-    if (!QREG) asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (!QREG) asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");
     float by_row[NR][2];                                                     // of the scores' rows
     int pos[NR][2];
 #pragma unroll
@@ -442,6 +446,8 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     // every key of tiles from `clear0` to before `clear1` is seen by all rows of the piece
     const int p_first = held + sh.row_tile * ROWS / R, p_last = held + (sh.row_tile * ROWS + used - 1) / R;
     const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + KEYS - 1) / KEYS : 0, clear1 = (p_first + 1) / KEYS;
+
+    const int p_warp = held + (sh.row_tile * ROWS + min(used, warp_row + 16) - 1) / R;
 
     float m[NR][2], l[NR][2], top[NR][2], o[TILES][NR][4];
 #pragma unroll
@@ -464,6 +470,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       if (lost || !mbar_wait(full + stage, turn / STAGES & 1, a.err, 2)) {
         lost = true;                                                        // recorded; the warps still meet at their barriers
         break;
+      }
+      if (ROWS > 16 && (warp_row >= used || tile * KEYS > p_warp)) {        // nothing that this warp's rows see
+        if (lane == 0) mbar_arrive(empty + stage);
+        continue;
       }
       const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
       // ---- scores: keys pi(g) and pi(g) + 8 of every 16, rows 2 t and 2 t + 1 --------------------------------------------------
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
 #pragma unroll
       for (int part = 0; part < D / 32; ++part) {
         const int c = part / (TL::kRun / 4), q = part % (TL::kRun / 4);
-        asm volatile("bar.sync 1, 128;" ::: "memory");                      // the last sums are no longer read
+        asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");                      // the last sums are no longer read
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -679,7 +689,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             if (part == 0 && g == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + row) * 4) = make_float4(m[r][e], l[r][e], top[r][e], 0.f);
             *reinterpret_cast<float4*>(s_sum + (warp * 8 * NR + row) * 32 + 4 * g) = four(r, e, c, q, 1.f);
           }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");
         const int r = tid >> 3;
         if (r < used) {
           const int d = (8 * c + (tid & 7)) * TL::kRun + 4 * q;
@@ -824,7 +834,7 @@ int paged_form(const PagedCall& call) {
   if (ready != cudaSuccess) return -30;
   if (call.a == nullptr) {
     int per = 0, dev = 0, sms = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, (kWarps + 1) * 32, kSmem) != cudaSuccess) return -31;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, Form<F8, D, ROWS, NR>::kThreads, kSmem) != cudaSuccess) return -31;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -32;
     return per * sms;
   }
@@ -838,14 +848,14 @@ int paged_form(const PagedCall& call) {
   // whole items are dealt out evenly too
   const int n = a.whole ? static_cast<int>(items < 148 * 8 ? items : 148 * 8) : a.ctas;
   if (n <= 0) return -21;
-  const cudaError_t e = launch_dependent(kernel, dim3(n), dim3((kWarps + 1) * 32), kSmem, call.stream, a, mk, mv);
+  const cudaError_t e = launch_dependent(kernel, dim3(n), dim3(Form<F8, D, ROWS, NR>::kThreads), kSmem, call.stream, a, mk, mv);
   if (e != cudaSuccess || a.whole) return static_cast<int>(e);
-  return static_cast<int>(launch_dependent(paged_attention_join_kernel<T, ROWS>, dim3(n, a.starts ? 16 : (R < ROWS ? R : ROWS)), dim3(128), 0, call.stream, a, n));
+  return static_cast<int>(launch_dependent(paged_attention_join_kernel<T, ROWS>, dim3(n, ROWS > 16 ? ROWS / 2 : a.starts ? 16 : (R < 16 ? R : 16)), dim3(128), 0, call.stream, a, n));
 }
 
 template <typename T, bool F8, int D>
 int paged_rows(const PagedCall& call, int rows, bool few) {
-  if (rows == 64) return paged_form<T, F8, D, 64, 2>(call);
+  if (rows > 16) return paged_form<T, F8, D, D == 256 ? 64 : 128, 2>(call);
   return few ? paged_form<T, F8, D, 16, 1>(call) : paged_form<T, F8, D, 16, 2>(call);
 }
 template <typename T, bool F8>
@@ -858,7 +868,7 @@ int paged_dim(const PagedCall& call, int D, int rows, bool few) {
   return -2;
 }
 int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool few) {
-  if (rows != 16 && rows != 64) return -3;
+  if (rows != 16 && rows != (D == 256 ? 64 : 128)) return -3;
   if (dtype == 0) return f8 ? paged_dim<__nv_bfloat16, true>(call, D, rows, few) : paged_dim<__nv_bfloat16, false>(call, D, rows, few);
   if (dtype == 1) return f8 ? paged_dim<__half, true>(call, D, rows, few) : paged_dim<__half, false>(call, D, rows, few);
   return -6;
@@ -868,12 +878,12 @@ int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool 
 
 using namespace tyr;
 
-// dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows: 16 or 64 of a tile.
+// dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows of a tile: 16, or 128 (64 of heads of 256).
 extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int rows, void* stream) {
   const PagedAttnArgs& a = *static_cast<const PagedAttnArgs*>(packed);
   if (a.rows <= 0 || a.B <= 0 || a.H <= 0 || a.G <= 0 || a.H % a.G != 0 || a.pages <= 0 || a.width <= 0 || a.window < 0) return -1;
   if (a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) return -2;
-  if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (rows != 16 && rows != 64) || (!a.whole && (a.part == nullptr || a.ctas <= 0))) return -3;
+  if ((a.k_scale != nullptr) != (a.v_scale != nullptr) || (!a.whole && (a.part == nullptr || a.ctas <= 0))) return -3;
   // a sequence's work and the pages' rows are counted in 32 bits
   const int keys = tile_keys(rows, a.D * (a.k_scale ? 1 : 2));
   const long long tiles = (static_cast<long long>(a.width) * a.P + keys - 1) / keys;

@@ -321,7 +321,7 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     q, f8 = _rows_of(q), store.k_scale is not None
     stride, R = q.stride(), H // G
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    tile = 64 if starts is not None and rows * R > 16 * B else 16
+    tile = (64 if D == 256 else 128) if starts is not None and rows * R > 16 * B else 16
     whole = width * P <= WHOLE_MAX_KEYS
     work = None
     if not whole:
