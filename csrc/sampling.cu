@@ -82,11 +82,12 @@ struct SampleShared {
   uint32_t bins[kSampleBins], total[kSampleBins];
   unsigned long long list[kSampleList];
   double weight[kSampleList];
-  double warp_sums[kSampleCluster * kSampleWarps];                                   // of all warps of the cluster
+  double warp_sums[kSampleWarps], cta_sums[kSampleCluster], run_sums[kSampleLargest / kSampleThreads];
   Partial part[2][kSampleCluster], warp_part[kSampleWarps];
   double warp_above[kSampleWarps];                                         // of a warp's logits above the bin of the cut
   float tops[kSampleCluster], warp_top[kSampleWarps];
-  uint32_t scan[kSampleWarps], listed, counts[kSampleCluster * kSampleWarps];
+  unsigned long long own[kSampleList];                                     // of the bin of the cut, this CTA's
+  uint32_t scan[kSampleWarps], listed, collected, counts[kSampleCluster * kSampleWarps];
   double scan_d[kSampleWarps];
   Place cut;
   int found, flag;
@@ -126,20 +127,42 @@ __device__ __forceinline__ double block_scan_d(double v, double* s, double& tota
   }
   return v + before;
 }
-// n items of a power of two, largest first
+// n items (a power of two, 64 at least), largest first: a bitonic network over two neighbouring items a thread.  Exchanges within a warp's 64 items take no shared
+// memory and no barrier, which leaves one exchange in ten for 64 items more, two for 128 and so on.
 __device__ __forceinline__ void block_sort(unsigned long long* v, int n) {
-  for (int size = 2; size <= n; size <<= 1)
+  __syncthreads();
+  const int at = 2 * threadIdx.x;
+  const bool on = at < n;                                                  // whole warps
+  unsigned long long x = on ? v[at] : 0, y = on ? v[at + 1] : 0;
+  for (int size = 2; size <= n; size <<= 1) {
     for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
-        const int a = 2 * i - (i & (step - 1)), b = a + step;
-        const unsigned long long x = v[a], y = v[b];
-        if ((x < y) == ((a & size) == 0)) {
-          v[a] = y;
-          v[b] = x;
+      const bool down = (at & size) == 0;                                  // largest first in this run
+      if (step >= 64) {
+        __syncthreads();
+        if (on) v[at] = x, v[at + 1] = y;
+        __syncthreads();
+        if (on) {
+          const bool upper = (at & step) == 0;
+          const unsigned long long p = v[at ^ step], q = v[(at + 1) ^ step];
+          x = upper == down ? max(x, p) : min(x, p);
+          y = upper == down ? max(y, q) : min(y, q);
+        }
+      } else if (on) {
+        if (step == 1) {
+          const unsigned long long p = max(x, y), q = min(x, y);
+          x = down ? p : q;
+          y = down ? q : p;
+        } else {
+          const bool upper = (at & step) == 0;
+          const unsigned long long p = __shfl_xor_sync(0xffffffffu, x, step >> 1), q = __shfl_xor_sync(0xffffffffu, y, step >> 1);
+          x = upper == down ? max(x, p) : min(x, p);
+          y = upper == down ? max(y, q) : min(y, q);
         }
       }
     }
+  }
+  __syncthreads();
+  if (on) v[at] = x, v[at + 1] = y;
   __syncthreads();
 }
 
@@ -283,7 +306,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return lead->listed;
   };
   const auto list_power = [&](int n) {
-    int size = 2;
+    int size = 64;
     while (size < n) size <<= 1;
     for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
     return size;
@@ -379,7 +402,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     bool first = true;
     int shift = 0, turn = mass;
     uint32_t in_n;
-    int last_bin = 0;
+    int last_turn = 0;
     // bins of the present interval: by value over all, then by key
     const auto place = [&](float v, uint32_t key) { return first ? bin_of(v) : static_cast<int>((high - key) >> shift); };
     const auto inside = [&](uint32_t key, uint32_t index) { return key != 0 && key >= low && key <= high && stays(key, index, cut); };
@@ -410,6 +433,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
           q.high = max(q.high, key);
         };
         if (mass && first && whole) {
+          if (tid == 0) s.collected = 0;
+          __syncthreads();
 #pragma unroll 4
           for (int j = 0; j < its; ++j) {
             const float v = x[32 * j];
@@ -418,8 +443,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             q.all += w;
             if (far < b) q.above += w;
             if (in_bin(v, far, b)) {
+              const uint32_t key = key_of(v);
               q.in += w;
-              note(key_of(v));
+              note(key);
+              const uint32_t at = atomicAdd(&s.collected, 1u);
+              if (at < kSampleList) s.own[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j);
             }
           }
         } else {
@@ -520,7 +548,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         above += all.above;
       }
       in_n = all.count;
-      last_bin = bin;
+      last_turn = turn;
       low = all.low;
       high = all.high;
       if (low >= high || in_n <= kSampleList) {
@@ -533,8 +561,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     const auto member = [&](uint32_t key, uint32_t index) { return key >= low && key <= high && stays(key, index, cut); };
     if (in_n <= kSampleList) {
-      const bool by_bin = first && whole;
-      const uint32_t n = gather([&](float v, uint32_t key, uint32_t index) { return by_bin || member(key, index); }, [&](float v) { return !by_bin || in_bin(v, far_of(v), last_bin); });
+      uint32_t n;
+      if (mass && first && whole) {                                        // collected beside the sums
+        uint32_t before = 0;
+        n = 0;
+        for (int r = 0; r < C; ++r) {
+          if (r < rank) before += s.part[last_turn][r].count;
+          n += s.part[last_turn][r].count;
+        }
+        SampleShared* lead = cluster.map_shared_rank(&s, 0);
+        for (int i = tid; i < static_cast<int>(s.part[last_turn][rank].count); i += kSampleThreads) lead->list[before + i] = s.own[i];
+        cluster.sync();
+      } else {
+        n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); }, [](float) { return true; });
+      }
       if (rank == 0) {
         block_sort(s.list, list_power(n));
         int last;                                                          // the last of the list that stays
@@ -634,48 +674,60 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     for (int j = 0; j < its; ++j) sum += weight_of(j);
     sum = warp_sum_d(sum);
   }
-  if (lane < C) cluster.map_shared_rank(s.warp_sums, lane)[rank * WARPS + warp] = sum;
+  // the CTA in which the cumulative weight passes the aim, else the last that holds any; then the warp in it, then the run of 32
+  if (lane == 0) s.warp_sums[warp] = sum;
+  __syncthreads();
+  if (tid < C) {
+    double own = 0.0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) own += s.warp_sums[i];
+    cluster.map_shared_rank(s.cta_sums, tid)[rank] = own;
+  }
   cluster.sync();
-  // the warp in which the cumulative weight passes the aim, else the last that holds any
-  const int n = C * WARPS, each = (n + 31) / 32;
-  double mine = 0.0;
-  for (int i = lane * each; i < min(n, (lane + 1) * each); ++i) mine += s.warp_sums[i];
-  const double upto_lane = warp_scan_d(mine, lane), aim = u * __shfl_sync(0xffffffffu, upto_lane, 31);
-  double before = upto_lane - mine, before_at = 0.0, before_last = 0.0;
-  uint32_t passes = 0xffffffffu, last = 0;
-  for (int i = lane * each; i < min(n, (lane + 1) * each); ++i) {
-    const double v = s.warp_sums[i];
-    if (v > 0.0) {
-      if (passes == 0xffffffffu && before + v > aim) passes = i, before_at = before;
-      last = i, before_last = before;
-    }
-    before += v;
+  // (which of the lanes' numbers in a row passes the aim, what lies before it); the last that holds any where none does
+  const auto passing = [&](double v, double start, double aim, double& before) {
+    const double upto = start + warp_scan_d(v, lane);
+    const uint32_t any = __ballot_sync(0xffffffffu, v > 0.0), past = __ballot_sync(0xffffffffu, v > 0.0 && upto > aim);
+    const int at = past ? __ffs(past) - 1 : 31 - __clz(any | 1u);
+    before = __shfl_sync(0xffffffffu, upto - v, at);
+    return at;
+  };
+  const double cta = lane < C ? s.cta_sums[lane] : 0.0, aim = u * warp_sum_d(cta);
+  double before;
+  if (passing(cta, 0.0, aim, before) != rank) return;
+  const int at_warp = passing(lane < WARPS ? s.warp_sums[lane] : 0.0, before, aim, before);
+  // all warps weigh that warp's logits, each its runs
+  const float* part = s_logits + at_warp * per_warp + lane;
+  const uint32_t part_index = rank * a.slice + at_warp * per_warp + lane;
+  const auto weight_at = [&](int j) {
+    const float v = part[32 * j];
+    const uint32_t key = key_of(v);
+    const double w = weigh(v);
+    return key != 0 && stays(key, part_index + 32 * j, cut) && w >= m ? w : 0.0;
+  };
+  for (int j = warp; j < its; j += WARPS) {
+    const double run = warp_sum_d(weight_at(j));
+    if (lane == 0) s.run_sums[j] = run;
   }
-  const uint32_t first_past = __reduce_min_sync(0xffffffffu, passes), last_any = __reduce_max_sync(0xffffffffu, last);
-  const int at = first_past == 0xffffffffu ? last_any : first_past;
-  before_at = __shfl_sync(0xffffffffu, first_past == 0xffffffffu ? before_last : before_at, at / each);
-  if (at == rank * WARPS + warp) {
-    double upto = before_at;
-    uint32_t chosen = 0;
-    bool found = false;
-    for (int j0 = 0; j0 < its && !found; j0 += 4) {                        // four at a time hide each other's latency
-      double w[4], of[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = j0 + i < its ? weight_of(j0 + i) : 0.0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) of[i] = warp_sum_d(w[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (found || !(of[i] > 0.0)) continue;
-        const double c_i = upto + warp_scan_d(w[i], lane);
-        const uint32_t any = __ballot_sync(0xffffffffu, w[i] > 0.0), past = __ballot_sync(0xffffffffu, w[i] > 0.0 && c_i > aim);
-        chosen = __shfl_sync(0xffffffffu, index_of(j0 + i), past ? __ffs(past) - 1 : 31 - __clz(any));
-        found = past != 0;
-        upto += of[i];
-      }
+  __syncthreads();
+  if (warp != 0) return;
+  int at_run = -1, last_run = 0;
+  double last_before = before;
+  for (int j0 = 0; j0 < its && at_run < 0; j0 += 32) {
+    const double v = j0 + lane < its ? s.run_sums[j0 + lane] : 0.0;
+    const double upto = before + warp_scan_d(v, lane);
+    const uint32_t any = __ballot_sync(0xffffffffu, v > 0.0), past = __ballot_sync(0xffffffffu, v > 0.0 && upto > aim);
+    if (any) {
+      const int at = past ? __ffs(past) - 1 : 31 - __clz(any);
+      last_run = j0 + at;
+      last_before = __shfl_sync(0xffffffffu, upto - v, at);
+      if (past) at_run = last_run;
     }
-    if (lane == 0) a.token[row] = chosen;
+    before = __shfl_sync(0xffffffffu, upto, 31);
   }
+  double unused;
+  const int at = passing(weight_at(last_run), last_before, aim, unused);
+  if (lane == at) a.token[row] = part_index + 32 * last_run;
 }
 
 template <typename T>
