@@ -81,12 +81,16 @@ struct Partial { double above, in, all; uint32_t count, low, high, pad; };
 struct SampleShared {
   uint32_t bins[kSampleBins], total[kSampleBins];
   unsigned long long list[kSampleList];
-  double weight[kSampleList];
+  union {                                                                  // of the list
+    double weight[kSampleList];
+    unsigned long long fixed[kSampleList];
+  };
   double warp_sums[kSampleWarps], cta_sums[kSampleCluster], run_sums[kSampleLargest / kSampleThreads];
   Partial part[2][kSampleCluster], warp_part[kSampleWarps];
   double warp_above[kSampleWarps];                                         // of a warp's logits above the bin of the cut
   float tops[kSampleCluster], warp_top[kSampleWarps];
   unsigned long long own[kSampleList];                                     // of the bin of the cut, this CTA's
+  unsigned long long best, bests[kSampleCluster];
   uint32_t scan[kSampleWarps], listed, collected, counts[kSampleCluster * kSampleWarps];
   double scan_d[kSampleWarps];
   Place cut;
@@ -126,6 +130,19 @@ __device__ __forceinline__ double block_scan_d(double v, double* s, double& tota
     total += s[i];
   }
   return v + before;
+}
+// n different items, largest first: as many threads as there are to an item count those before it.
+__device__ __forceinline__ void block_rank(unsigned long long* v, unsigned long long* to, int n) {
+  const int each = n > 128 ? 2 : n > 64 ? 4 : n > 32 ? 8 : n > 16 ? 16 : 32, i = threadIdx.x / each;
+  __syncthreads();
+  const unsigned long long x = i < n ? v[i] : ~0ull;
+  int before = 0;
+  for (int j = threadIdx.x % each; j < n; j += each) before += v[j] > x;
+  for (int o = 1; o < each; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (i < n && threadIdx.x % each == 0) to[before] = x;
+  __syncthreads();
+  if (threadIdx.x < n) v[threadIdx.x] = to[threadIdx.x];
+  __syncthreads();
 }
 // n items (a power of two, 64 at least), largest first: a bitonic network over two neighbouring items a thread.  Exchanges within a warp's 64 items take no shared
 // memory and no barrier, which leaves one exchange in ten for 64 items more, two for 128 and so on.
@@ -305,10 +322,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     cluster.sync();
     return lead->listed;
   };
-  const auto list_power = [&](int n) {
+  constexpr int kFewItems = 256;                                           // 50 items take 0.3 us so and 2.5 by the network, 514 more than by it
+  const auto sort_list = [&](int n) {
+    if (n <= kFewItems) {
+      block_rank(s.list, s.own, n);
+      return n;
+    }
     int size = 64;
     while (size < n) size <<= 1;
     for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
+    block_sort(s.list, size);
     return size;
   };
 
@@ -331,8 +354,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         // ---- all that can stay lies in CTA 0's list ----------------------------------------------------------------------------
         cluster.sync();                                                    // the others have read its length
         if (rank != 0) return;
-        const int size = list_power(n);
-        block_sort(s.list, size);
+        sort_list(n);
         const int kept = min(static_cast<int>(n), k_row);
         constexpr int PER = kSampleList / kSampleThreads;
         double w[PER], sum = 0.0, total;
@@ -357,20 +379,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int at = tid * PER + i;
-          moved[i] = at < size && s.weight[at] > 0.0 ? s.list[at] << 32 | static_cast<unsigned>(at) : 0ull;
+          moved[i] = at < kept && s.weight[at] > 0.0 ? s.list[at] << 32 | static_cast<unsigned>(at) : 0ull;
         }
+        if (tid == 0) s.listed = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          if (tid * PER + i < size) s.list[tid * PER + i] = moved[i];
+          if (moved[i] != 0) s.list[atomicAdd(&s.listed, 1u)] = moved[i];
         if (tid == 0) s.found = 0x7fffffff, s.flag = 0;
-        block_sort(s.list, size);
+        __syncthreads();
+        const int left = s.listed;
+        sort_list(left);
         double v[PER];
         sum = 0.0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int at = tid * PER + i;
-          v[i] = at < size && s.list[at] != 0 ? s.weight[static_cast<uint32_t>(s.list[at])] : 0.0;
+          v[i] = at < left ? s.weight[static_cast<uint32_t>(s.list[at])] : 0.0;
           sum += v[i];
         }
         double upto = block_scan_d(sum, s.scan_d, total) - sum;
@@ -393,6 +418,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
   }
 
+  const auto fix_of = [&](float largest) {                                 // 2^52 over the power of two above its weight
+    return __hiloint2double((2046 + 52 - (__double2hiint(weigh(largest)) >> 20 & 0x7ff)) << 20, 0);
+  };
+  float cut_high = 0.f;
   // One cut in the order: by the number of what stays (k), or by its weight (below p times the weight of all that the present cut keeps).
   int cut_bin = -1;                                                        // the bin of values in which a cut by weight over all lies
   const auto select = [&](bool mass, uint32_t k) {
@@ -435,19 +464,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         if (mass && first && whole) {
           if (tid == 0) s.collected = 0;
           __syncthreads();
-#pragma unroll 4
-          for (int j = 0; j < its; ++j) {
-            const float v = x[32 * j];
-            const double w = weigh(v);
-            const float far = far_of(v);
-            q.all += w;
-            if (far < b) q.above += w;
-            if (in_bin(v, far, b)) {
-              const uint32_t key = key_of(v);
-              q.in += w;
-              note(key);
-              const uint32_t at = atomicAdd(&s.collected, 1u);
-              if (at < kSampleList) s.own[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j);
+          for (int j0 = 0; j0 < its; j0 += 4) {                            // four weights hide each other's latency
+            float v[4];
+            double w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = j0 + i < its ? x[32 * (j0 + i)] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = weigh(v[i]);
+            bool hit[4], any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float far = far_of(v[i]);
+              q.all += w[i];
+              if (far < b) q.above += w[i];
+              any |= hit[i] = in_bin(v[i], far, b);
+            }
+            if (any) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (!hit[i]) continue;
+                const uint32_t key = key_of(v[i]);
+                q.in += w[i];
+                note(key);
+                const uint32_t at = atomicAdd(&s.collected, 1u);
+                if (at < kSampleList) s.own[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j0 + i);
+              }
             }
           }
         } else {
@@ -552,7 +593,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       low = all.low;
       high = all.high;
       if (low >= high || in_n <= kSampleList) {
-        if (mass && first && whole) cut_bin = bin;
+        if (mass && first && whole && in_n <= kSampleList) cut_bin = bin, cut_high = value_of(high);
         break;
       }
       first = false;
@@ -561,22 +602,42 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     const auto member = [&](uint32_t key, uint32_t index) { return key >= low && key <= high && stays(key, index, cut); };
     if (in_n <= kSampleList) {
-      uint32_t n;
-      if (mass && first && whole) {                                        // collected beside the sums
+      if (mass && first && whole) {
+        // collected beside the sums: every CTA gets all of it and places its own, by the weight of what comes before.  Weights here are whole numbers, of the
+        // largest's 2^-52, so that their sums do not depend on the order in which they were collected.
+        const int own_n = s.part[last_turn][rank].count;
         uint32_t before = 0;
-        n = 0;
-        for (int r = 0; r < C; ++r) {
-          if (r < rank) before += s.part[last_turn][r].count;
-          n += s.part[last_turn][r].count;
-        }
-        SampleShared* lead = cluster.map_shared_rank(&s, 0);
-        for (int i = tid; i < static_cast<int>(s.part[last_turn][rank].count); i += kSampleThreads) lead->list[before + i] = s.own[i];
+        for (int r = 0; r < rank; ++r) before += s.part[last_turn][r].count;
+        for (int i = tid; i < own_n * C; i += kSampleThreads) cluster.map_shared_rank(&s, i / own_n)->list[before + i % own_n] = s.own[i % own_n];
+        if (tid == 0) s.best = ~0ull;
         cluster.sync();
-      } else {
-        n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); }, [](float) { return true; });
+        const double unit = fix_of(value_of(high));
+        for (int i = tid; i < (static_cast<int>(in_n) + 31) / 32 * 32; i += kSampleThreads) {      // whole warps weigh
+          const double w = weigh(value_of(static_cast<uint32_t>(s.list[min(i, static_cast<int>(in_n) - 1)] >> 32)));
+          if (i < static_cast<int>(in_n)) s.fixed[i] = static_cast<unsigned long long>(w * unit);
+        }
+        __syncthreads();
+        const int each = own_n > 256 ? 1 : own_n > 64 ? 2 : own_n > 16 ? 8 : 32;      // threads an item
+        for (int i0 = 0; i0 < own_n; i0 += kSampleThreads / each) {
+          const int i = i0 + tid / each;
+          const unsigned long long item = s.own[min(i, own_n - 1)];
+          unsigned long long ahead = 0;
+          for (int j = tid % each; j < static_cast<int>(in_n); j += each) ahead += s.list[j] > item ? s.fixed[j] : 0ull;
+          for (int o = 1; o < each; o <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+          if (i < own_n && tid % each == 0 && above + static_cast<double>(ahead) / unit < aim) atomicMin(&s.best, item);
+        }
+        __syncthreads();
+        if (tid < C) cluster.map_shared_rank(s.bests, tid)[rank] = s.best;
+        cluster.sync();
+        unsigned long long last = ~0ull;
+        for (int r = 0; r < C; ++r) last = min(last, s.bests[r]);
+        if (last == ~0ull) last = static_cast<unsigned long long>(high) << 32;      // not even the first: by a rounding of the sums alone
+        cut = Place{static_cast<uint32_t>(last >> 32), ~static_cast<uint32_t>(last)};
+        return;
       }
+      const uint32_t n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); }, [](float) { return true; });
       if (rank == 0) {
-        block_sort(s.list, list_power(n));
+        sort_list(n);
         int last;                                                          // the last of the list that stays
         if (!mass) {
           last = static_cast<int>(k - above_n) - 1;
@@ -658,17 +719,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     sum = warp_sum_d(sum);
     if (sum < 1e-200) sum = 0.0;                                           // nothing but what is never chosen
   } else if (cut_bin >= 0 && m <= 0.0) {
-    // what lies above the cut's bin has been summed up
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) {
-      const float v = x[32 * j];
-      const bool in = in_bin(v, far_of(v), cut_bin);
-      if (__any_sync(0xffffffffu, in)) {
-        const double w = weigh(v);
-        if (in && stays(key_of(v), index_of(j), cut)) sum += w;
-      }
+    // what lies above the cut's bin has been summed up, and what lies in it is listed
+    if (tid < WARPS) s.fixed[tid] = 0;
+    __syncthreads();
+    const double unit = fix_of(cut_high);
+    const int own_n = s.collected;
+    for (int i = tid; i < (own_n + 31) / 32 * 32; i += kSampleThreads) {
+      const unsigned long long item = s.own[min(i, own_n - 1)];
+      const uint32_t key = static_cast<uint32_t>(item >> 32), index = ~static_cast<uint32_t>(item);
+      const double w = weigh(value_of(key));
+      if (i < own_n && stays(key, index, cut)) atomicAdd(&s.fixed[(index - rank * a.slice) / per_warp], static_cast<unsigned long long>(w * unit));
     }
-    sum = warp_sum_d(sum) + s.warp_above[warp];
+    __syncthreads();
+    sum = s.warp_above[warp] + static_cast<double>(s.fixed[warp]) / unit;
   } else {
 #pragma unroll 4
     for (int j = 0; j < its; ++j) sum += weight_of(j);
