@@ -70,14 +70,22 @@ def right_pad(rows: List[List[int]], pad: int) -> Tuple[torch.Tensor, List[int]]
     return torch.tensor([r + [pad] * (w - len(r)) for r in rows]), [len(r) for r in rows]
 
 
-def load_text_family(family: str, model_dir: str, device, dtype):
-    """Returns (generate(ids, max_new, strategy, on_step[, lengths]) -> ids, tokenizer, render(prompt) -> str, eos ids, pad id)."""
+CACHES = {"paged": None, "paged8": torch.float8_e4m3fn}       # type of the pages (None: the model's)
+
+
+def load_text_family(family: str, model_dir: str, device, dtype, cache: str = "dense"):
+    """Returns (generate(ids, max_new, strategy, on_step[, lengths]) -> ids, tokenizer, render(prompt) -> str, eos ids, pad id); with a paged ``cache`` generate
+    takes lists of ids of any lengths and returns lists of new ones."""
+    if cache != "dense" and family not in ("qwen3", "qwen25omni"):
+        raise ValueError(f"{family} has no paged cache")
     if family in ("qwen3", "qwen25omni"):
         from ..models import qwen as Q
         lm = Q.load_qwen25_omni_thinker(model_dir, device, dtype) if family == "qwen25omni" else Q.load_from_pretrained(model_dir, device, dtype)
         tok = tok_hf.load_qwen3(model_dir)
         eos = [i for i in (tok.token_id("<|im_end|>"), tok.token_id("<|endoftext|>")) if i is not None]
         gen = lambda ids, n, st, cb: Q.generate(lm, ids, n, st, eos, cb)
+        if cache != "dense":
+            gen = lambda rows, n, st, cb: Q.generate_paged(lm, rows, n, st, eos, cb, cache=CACHES[cache] or dtype)
         return gen, tok, lambda p: tok_hf.chatml_prompt([{"role": "user", "content": p}]), eos, eos[-1] if eos else 0
     if family == "qwen35":
         from ..models import qwen35 as Q5
@@ -114,17 +122,21 @@ def run_text(a, device, dtype, out=print) -> int:
         a.family = registry.detect_dir(model_dir).name
         if a.family not in TEXT_FAMILIES:
             raise ValueError(f"{a.family} has its own command line")
-    gen, tok, render, eos, pad = load_text_family(a.family, model_dir, device, dtype)
-    strategy = SamplingStrategy.greedy() if a.temperature <= 0 else SamplingStrategy.multinomial(a.temperature, a.top_k, a.top_p)
+    gen, tok, render, eos, pad = load_text_family(a.family, model_dir, device, dtype, a.cache)
+    strategy = (SamplingStrategy.greedy() if a.temperature <= 0 else SamplingStrategy.drawn(a.temperature, a.top_k, a.top_p, a.min_p) if a.min_p is not None
+                else SamplingStrategy.multinomial(a.temperature, a.top_k, a.top_p))
     prompts = load_prompts(a.prompt_file, a.prompt)
     for chunk in batches(prompts, a.batch_size):
         rows, extra = [tok.encode(render(p)) for p in chunk], ()
-        if registry.by_name(a.family).ragged:        # prompts padded at the end, their lengths passed on
+        if a.cache != "dense":
+            ids = rows
+        elif registry.by_name(a.family).ragged:        # prompts padded at the end, their lengths passed on
             ids, lengths = right_pad(rows, pad)
             extra = (lengths,)
         else:
             ids = left_pad(rows, pad)
-        ids = ids.to(device)
+        if a.cache == "dense":
+            ids = ids.to(device)
         on_step = None
         if a.stream and len(chunk) == 1:
             on_step = lambda step, t: print(tok.decode([int(t[0])], skip_special=True), end="", flush=True)
@@ -133,15 +145,15 @@ def run_text(a, device, dtype, out=print) -> int:
         if device.type == "cuda":
             torch.cuda.synchronize(device)
         dt = time.perf_counter() - t0
-        new = res[:, ids.shape[1]:]
+        new = res if a.cache != "dense" else res[:, ids.shape[1]:].tolist()
         if on_step is not None:
             print()
         else:
-            for p, row in zip(chunk, new.tolist()):
+            for p, row in zip(chunk, new):
                 cut = next((i for i, t in enumerate(row) if t in eos), len(row))
                 out(f"> {p}\n{tok.decode(row[:cut], skip_special=True)}")
         if a.bench:
-            out(f"BENCH batch={len(chunk)} prompt_tokens={ids.shape[1]} new_tokens={new.shape[1]} seconds={dt:.3f} tok_s={new.numel() / dt:.1f}")
+            out(f"BENCH batch={len(chunk)} prompt_tokens={max(len(r) for r in ids)} new_tokens={max(map(len, new))} seconds={dt:.3f} tok_s={sum(map(len, new)) / dt:.1f}")
     return 0
 
 
@@ -184,6 +196,8 @@ def parse(argv):
     p.add_argument("--temperature", type=float, default=0.0)
     p.add_argument("--top-k", type=int, default=None)
     p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=None, help="draw with min-p as well, all filters in one launch")
+    p.add_argument("--cache", default="dense", choices=("dense", *CACHES), help="paged: prompts of any lengths without padding; paged8: in 8 bits")
     p.add_argument("--stream", action="store_true")
     p.add_argument("--bench", action="store_true")
     p.add_argument("--device", default="auto")

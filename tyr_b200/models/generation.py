@@ -6,14 +6,18 @@ from typing import Callable, Optional, Sequence
 
 import torch
 
+from ..ops.sampling import sample
+
 
 @dataclass(frozen=True)
 class SamplingStrategy:
-    """``greedy`` or ``multinomial(temperature, top_k, top_p)`` (Generation.lean:22-25)."""
+    """``greedy`` or ``multinomial(temperature, top_k, top_p)`` (Generation.lean:22-25), or ``drawn``: the same filters and min-p, decided in 64 bits in one launch
+    from uniform numbers (ops/sampling.py)."""
     kind: str = "greedy"
     temperature: float = 1.0
     top_k: Optional[int] = None
     top_p: float = 1.0
+    min_p: float = 0.0
 
     @staticmethod
     def greedy() -> "SamplingStrategy":
@@ -22,6 +26,10 @@ class SamplingStrategy:
     @staticmethod
     def multinomial(temperature: float = 1.0, top_k: Optional[int] = None, top_p: float = 1.0) -> "SamplingStrategy":
         return SamplingStrategy("multinomial", temperature, top_k, top_p)
+
+    @staticmethod
+    def drawn(temperature: float = 1.0, top_k: Optional[int] = None, top_p: float = 1.0, min_p: float = 0.0) -> "SamplingStrategy":
+        return SamplingStrategy("drawn", temperature, top_k, top_p, min_p)
 
 
 def top_k_filter(logits: torch.Tensor, k: Optional[int]) -> torch.Tensor:
@@ -49,6 +57,9 @@ def sample_from_logits(logits: torch.Tensor, strategy: SamplingStrategy, generat
         raise ValueError("greedy sampling requires a nonempty vocabulary")
     if strategy.kind == "greedy":
         return torch.argmax(logits, dim=-1)
+    if strategy.kind == "drawn":
+        draws = torch.rand(logits.shape[0], device=logits.device, generator=generator)
+        return sample(logits, draws, temperature=strategy.temperature, top_k=strategy.top_k, top_p=strategy.top_p, min_p=strategy.min_p)
     if strategy.temperature <= 0.0:
         raise ValueError(f"multinomial sampling requires temperature > 0, got {strategy.temperature}")
     scaled = logits if strategy.temperature == 1.0 else logits * (1.0 / strategy.temperature)
@@ -87,7 +98,7 @@ def generate_cached(prefill: Callable[[torch.Tensor], torch.Tensor], step: Calla
     ids = input_ids
     eos = list(eos_token_ids)
     for i in range(max_new_tokens):
-        nxt_raw = sample_from_logits(logits.float(), strategy, generator)
+        nxt_raw = sample_from_logits(logits if strategy.kind == "drawn" else logits.float(), strategy, generator)
         if eos:
             nxt = apply_finished_eos(nxt_raw, finished, eos[0])
             finished = finished | token_in_set(nxt_raw, eos)

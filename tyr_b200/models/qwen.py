@@ -16,8 +16,9 @@ import torch.nn.functional as F
 
 from ..io import safetensors as st
 from ..ops.attention import attention
+from ..ops.paged_cache import PagedStore, paged_append, paged_attention
 from .common import KVCache, apply_rotary_partial, cached_attention, cos_sin_tables, head_norm, lin, norm_w, plain_inv_freq, swiglu_mlp
-from .generation import SamplingStrategy, generate_cached
+from .generation import SamplingStrategy, generate_cached, sample_from_logits
 
 
 @dataclass
@@ -302,6 +303,124 @@ class Qwen3Session:
         for c in self.caches:
             c.length += 1
         return out
+
+
+class PagedQwen3Session:
+    """Sequences of any lengths over one paged cache a layer: prompts (or further pieces of them) of ragged length without padding, one token a sequence from then
+    on, and pages that a finished sequence gives back.  ``cache``: type of the pages, e4m3 with a scale for each page and head, or the model's."""
+
+    def __init__(self, lm: Qwen3ForCausalLM, sequences: int, max_len: int, *, page: int = 64, pages: Optional[int] = None, cache: torch.dtype = torch.float8_e4m3fn):
+        cfg = lm.cfg
+        dev = lm.model.embed_tokens.device
+        width = -(-max_len // page)
+        if sequences <= 0 or max_len <= 0:
+            raise ValueError("a paged session needs sequences and room for their tokens")
+        pages = sequences * width if pages is None else pages
+        self.lm, self.page, self.max_len = lm, page, max_len
+        self.rope = RoPECache.init(max_len, cfg.half_head_dim, cfg.rope_theta, dev)
+        self.stores = [PagedStore.allocate(pages, cfg.num_key_value_heads, page, cfg.head_dim, dev, cache) for _ in range(cfg.num_hidden_layers)]
+        self.held = [0] * sequences                        # tokens of each sequence
+        self.owned: List[List[int]] = [[] for _ in range(sequences)]
+        self.free = list(range(pages))[::-1]
+        self._rows = torch.zeros((sequences, width), dtype=torch.int32)
+        self.table, self.lengths = self._rows.to(dev), torch.zeros(sequences, dtype=torch.int32, device=dev)
+        self._graph = None
+
+    def _room(self, new: Sequence[int]) -> None:
+        """Pages for these new tokens of every sequence, or none at all."""
+        want = [-(-(h + n) // self.page) - len(o) if n else 0 for h, n, o in zip(self.held, new, self.owned)]
+        if any(h + n > self.max_len for h, n in zip(self.held, new)) or sum(want) > len(self.free):
+            raise ValueError("paged cache overflow")
+        for b, n in enumerate(want):
+            for _ in range(n):
+                self._rows[b, len(self.owned[b])] = self.free[-1]
+                self.owned[b].append(self.free.pop())
+        if any(want):
+            self.table.copy_(self._rows)
+
+    def _layers(self, x: torch.Tensor, starts: Optional[torch.Tensor]) -> torch.Tensor:
+        """Rows [1, rows, hidden] of new tokens, already counted in ``lengths``, through all layers."""
+        cfg, (_, rows, _) = self.lm.cfg, x.shape
+        H, Hkv, D, eps = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rms_norm_eps
+        for l, store in zip(self.lm.model.layers, self.stores):
+            a = l.self_attn
+            h = norm_w(x, l.input_layernorm, eps)
+            q, k, v = (lin(h, w, b).reshape(rows, n, D) for w, b, n in ((a.q_proj, a.q_bias, H), (a.k_proj, a.k_bias, Hkv), (a.v_proj, a.v_bias, Hkv)))
+            q = paged_append(store, k, v, self.table, self.lengths, starts, q=q, cos=self.rope.cos, sin=self.rope.sin, q_weight=a.q_norm, k_weight=a.k_norm, eps=eps)
+            o = paged_attention(q, store, self.table, self.lengths, starts)
+            x = x + lin(o.reshape(1, rows, H * D), a.o_proj)
+            x = x + swiglu_mlp(norm_w(x, l.post_attention_layernorm, eps), l.mlp.gate_proj, l.mlp.up_proj, l.mlp.down_proj)
+        return norm_w(x, self.lm.model.norm, eps)
+
+    @torch.no_grad()
+    def extend(self, prompts: Sequence[Sequence[int]]) -> torch.Tensor:
+        """Appends these tokens to the sequences (none to some) -> logits [sequences, V] after each one's last; rows without new tokens are zeros."""
+        if len(prompts) != len(self.held) or not any(prompts):
+            raise ValueError(f"a session of {len(self.held)} sequences takes that many prompts, not all of them empty")
+        new = [len(p) for p in prompts]
+        self._room(new)
+        dev = self.table.device
+        self.held = [h + n for h, n in zip(self.held, new)]
+        self.lengths.copy_(torch.tensor(self.held, dtype=torch.int32))
+        starts = torch.tensor([0] + new).cumsum(0)
+        ids = torch.tensor([t for p in prompts for t in p], device=dev)
+        h = self._layers(self.lm.embed_tokens(ids)[None], starts.to(device=dev, dtype=torch.int32))[0]
+        there = torch.tensor([b for b, n in enumerate(new) if n])
+        logits = lin(h[(starts[1:] - 1)[there].to(dev)], self.lm.lm_head)
+        return logits.new_zeros(len(new), logits.shape[1]).index_copy_(0, there.to(dev), logits)
+
+    def _device_step(self, tok: torch.Tensor) -> torch.Tensor:
+        self.lengths += self.lengths > 0
+        return lin(self._layers(self.lm.embed_tokens(tok)[None], None)[0], self.lm.lm_head)
+
+    @torch.no_grad()
+    def step(self, tok: torch.Tensor) -> torch.Tensor:
+        """One token for every sequence that holds any -> logits [sequences, V] (rows of the others mean nothing)."""
+        self._room([int(h > 0) for h in self.held])
+        self.held = [h + (h > 0) for h in self.held]
+        tok = tok.reshape(-1)
+        if not self.table.is_cuda or os.environ.get("TYR_DECODE_GRAPH", "1") == "0":
+            return self._device_step(tok)
+        if self._graph is None:
+            from ..utils.graph import GraphedStep
+            self._graph = GraphedStep(self._device_step, (tok.clone(),), advancing_state=(self.lengths,))
+        return self._graph(tok)
+
+    def release(self, sequence: int) -> None:
+        """The sequence is over: its pages are free, its place takes another one."""
+        self.free += self.owned[sequence]
+        self.owned[sequence], self.held[sequence] = [], 0
+        self.lengths[sequence] = 0
+
+    def nbytes(self) -> int:
+        return sum(s.nbytes() for s in self.stores)
+
+
+@torch.no_grad()
+def generate_paged(lm: Qwen3ForCausalLM, prompts: Sequence[Sequence[int]], max_new_tokens: int = 64, strategy: SamplingStrategy = SamplingStrategy(), eos_token_ids=None,
+                   on_step=None, *, generator: Optional[torch.Generator] = None, **session) -> List[List[int]]:
+    """New tokens of every prompt, up to the first end of text (kept) each; prompts need no padding (options of :class:`PagedQwen3Session`)."""
+    eos = set(lm.cfg.eos_token_ids if eos_token_ids is None else eos_token_ids)
+    if not prompts or not all(prompts):
+        raise ValueError("generate requires non-empty prompt sequence")
+    out: List[List[int]] = [[] for _ in prompts]
+    if max_new_tokens <= 0:
+        return out
+    s = PagedQwen3Session(lm, len(prompts), max(map(len, prompts)) + max_new_tokens, **session)
+    logits = s.extend(prompts)
+    for i in range(max_new_tokens):
+        tok = sample_from_logits(logits if strategy.kind == "drawn" else logits.float(), strategy, generator)
+        for b, t in enumerate(tok.tolist()):
+            if s.held[b]:
+                out[b].append(t)
+                if t in eos:
+                    s.release(b)
+        if on_step is not None:
+            on_step(i, tok)
+        if i + 1 == max_new_tokens or not any(s.held):
+            break
+        logits = s.step(tok)
+    return out
 
 
 def generate(lm: Qwen3ForCausalLM, input_ids, max_new_tokens=64, strategy=SamplingStrategy(), eos_token_ids=None, on_step=None):
