@@ -89,17 +89,18 @@ struct Share {
   long long item_end;
 
   __device__ __forceinline__ Share(const PagedAttnArgs& args, int lane_) : a(args), lane(lane_) {
-    long long sum = 0;
-    for (int i = lane; i < a.B; i += 32) sum += seq_work(a, seq_of<ROWS, KEYS>(a, i));
+    const long long first_work = lane < a.B ? seq_work(a, seq_of<ROWS, KEYS>(a, lane)) : 0;
+    long long sum = first_work;
+    for (int i = lane + 32; i < a.B; i += 32) sum += seq_work(a, seq_of<ROWS, KEYS>(a, i));
     const long long total = warp_sum64(sum);
-    per = (total + gridDim.x - 1) / gridDim.x;
+    per = total >> 31 ? (total + gridDim.x - 1) / gridDim.x : (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x;
     at = min(static_cast<long long>(blockIdx.x) * per, total);
     end = min(at + per, total);
     before = 0;
     b = 0;
     if (at >= end) return;
     for (int base = 0; base < a.B; base += 32) {
-      const long long mine = base + lane < a.B ? seq_work(a, seq_of<ROWS, KEYS>(a, base + lane)) : 0;
+      const long long mine = base == 0 ? first_work : base + lane < a.B ? seq_work(a, seq_of<ROWS, KEYS>(a, base + lane)) : 0;
       long long upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -477,13 +478,15 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       }
       const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
       // ---- scores: keys pi(g) and pi(g) + 8 of every 16, rows 2 t and 2 t + 1 --------------------------------------------------
-      float s[GROUPS][NR][4];
+      // one run of keys and rows: its products in two sums, each half as long a chain
+      constexpr int CHAINS = GROUPS * NR == 1 ? 2 : 1;
+      float s[GROUPS][NR][4], s_odd[CHAINS][4];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][r][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[j][r][e] = s_odd[0][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < TL::kChunks / 4; ++c) {
         constexpr int STEPS = F8 ? 4 : 2;
@@ -518,9 +521,13 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
               x[0] = u[2 * i]; x[1] = v[2 * i]; x[2] = u[2 * i + 1]; x[3] = v[2 * i + 1];
             }
 #pragma unroll
-            for (int r = 0; r < NR; ++r) mma<M>(s[j][r], x[0], x[1], x[2], x[3], qs[i][r], qs[i][NR + r]);
+            for (int r = 0; r < NR; ++r) mma<M>(CHAINS == 2 && i % 2 ? s_odd[0] : s[j][r], x[0], x[1], x[2], x[3], qs[i][r], qs[i][NR + r]);
           }
         }
+      }
+      if constexpr (CHAINS == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][0][e] += s_odd[0][e];
       }
       // ---- running maxima --------------------------------------------------------------------------------------------------
       const int key0 = tile * KEYS;
@@ -676,49 +683,59 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       return make_float4(o[k][r][e] * f, o[k][r][2 + e] * f, o[k + 1][r][e] * f, o[k + 1][r][2 + e] * f);
     };
     if constexpr (ROWS == 16) {
-      // 32 channels at a time: four of each of a box's eight runs
+      // a thread has a row and a run of the box: the warps' factors once, then 32 channels at a time, four of each of a box's eight runs
+      asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");              // the last piece's sums are no longer read
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (g == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + 8 * r + 2 * t + e) * 4) = make_float4(m[r][e], l[r][e], top[r][e], 0.f);
+      const int row_in = tid >> 3;
+      float by_warp[kWarps], mm = -INFINITY, tt = -INFINITY, ll = 0.f, scale_out = kUndo;
+      T* dst = nullptr;
+      float* sums = nullptr;
 #pragma unroll
       for (int part = 0; part < D / 32; ++part) {
         const int c = part / (TL::kRun / 4), q = part % (TL::kRun / 4);
-        asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");                      // the last sums are no longer read
+        if (part > 0) asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");      // the last channels are no longer read
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = 8 * r + 2 * t + e;
-            if (part == 0 && g == 0) *reinterpret_cast<float4*>(s_stats + (warp * 16 + row) * 4) = make_float4(m[r][e], l[r][e], top[r][e], 0.f);
-            *reinterpret_cast<float4*>(s_sum + (warp * 8 * NR + row) * 32 + 4 * g) = four(r, e, c, q, 1.f);
-          }
+          for (int e = 0; e < 2; ++e) *reinterpret_cast<float4*>(s_sum + (warp * 8 * NR + 8 * r + 2 * t + e) * 32 + 4 * g) = four(r, e, c, q, 1.f);
         asm volatile("bar.sync 1, %0;" ::"n"(kSync) : "memory");
-        const int r = tid >> 3;
-        if (r < used) {
-          const int d = (8 * c + (tid & 7)) * TL::kRun + 4 * q;
-          float mm = -INFINITY, tt = -INFINITY;
+        if (row_in >= used) continue;
+        if (part == 0) {
+          float4 st[kWarps];
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
-            mm = fmaxf(mm, st.x);
-            tt = fmaxf(tt, st.z);
+            st[w] = *reinterpret_cast<const float4*>(s_stats + (w * 16 + row_in) * 4);
+            mm = fmaxf(mm, st[w].x);
+            tt = fmaxf(tt, st[w].z);
           }
-          float ll = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float4 st = *reinterpret_cast<const float4*>(s_stats + (w * 16 + r) * 4);
-            if (st.x != -INFINITY || st.y != 0.f) ll += st.y * (st.x == -INFINITY ? 1.f : pt_exp2(st.x - mm));
-            const float f = st.z == -INFINITY ? (st.y != st.y ? 1.f : 0.f) : pt_exp2(st.z - tt);
-            const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + r) * 32 + 4 * (tid & 7));
-            v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+            if (st[w].x != -INFINITY || st[w].y != 0.f) ll += st[w].y * (st[w].x == -INFINITY ? 1.f : pt_exp2(st[w].x - mm));
+            by_warp[w] = st[w].z == -INFINITY ? (st[w].y != st[w].y ? 1.f : 0.f) : pt_exp2(st[w].z - tt);
           }
           if (done) {
-            const int row = sh.row_tile * ROWS + r;
-            const float f = ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(tt - mm) : 1.f) / ll : 0.f;
-            write4(static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+            const int row = sh.row_tile * ROWS + row_in;
+            scale_out = ll > 0.f || ll != ll ? kUndo * (F8 ? pt_exp2(tt - mm) : 1.f) / ll : 0.f;
+            dst = static_cast<T*>(a.out) + ((first_row + row / R) * a.H + sh.head * R + row % R) * D;
           } else {
-            *reinterpret_cast<float4*>(part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(r) * D + d) = make_float4(v.x * kUndo, v.y * kUndo, v.z * kUndo, v.w * kUndo);
-            if (d == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + r * 4) = make_float4(mm, ll, tt, 0.f);
+            sums = part_sums(a, gridDim.x, ROWS, piece) + static_cast<long long>(row_in) * D;
+            if ((tid & 7) == 0) *reinterpret_cast<float4*>(part_stats(a, gridDim.x, ROWS, piece) + row_in * 4) = make_float4(mm, ll, tt, 0.f);
           }
         }
+        const int d = (8 * c + (tid & 7)) * TL::kRun + 4 * q;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(s_sum + (w * 8 * NR + row_in) * 32 + 4 * (tid & 7));
+          v.x += x.x * by_warp[w]; v.y += x.y * by_warp[w]; v.z += x.z * by_warp[w]; v.w += x.w * by_warp[w];
+        }
+        v = make_float4(v.x * scale_out, v.y * scale_out, v.z * scale_out, v.w * scale_out);
+        if (done) write4(dst + d, v);
+        else *reinterpret_cast<float4*>(sums + d) = v;
       }
     } else {
 #pragma unroll
