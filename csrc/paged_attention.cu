@@ -42,7 +42,7 @@ struct PagedAttnArgs {
   float* part;                                 // workspace (see part_stats)
   int* err;
   long long q_row, q_head, table_row;
-  int rows, B, H, G, D, P, pages, width, window, whole;
+  int rows, B, H, G, D, P, pages, width, window, whole;       // P: 16, 32, 64 or 128
   float scale;
   int ctas;                                    // shares of the work that `part` has room for (not read where shares are whole items)
 };
@@ -59,7 +59,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   s.len = a.lengths[b];
   s.row = a.starts ? a.starts[b] : b;
   s.n = a.starts ? a.starts[b + 1] - s.row : (s.len > 0 ? 1 : 0);
-  if (s.n != 0 && (s.n < 0 || s.row < 0 || s.row + s.n > a.rows || s.len < s.n || (s.len - 1) / a.P >= a.width)) {
+  if (s.n != 0 && (s.n < 0 || s.row < 0 || s.row + s.n > a.rows || s.len < s.n || (s.len - 1) >> (31 - __clz(a.P)) >= a.width)) {
     report_error(a.err, ERR_BOUNDS, b);
     s.n = 0;
   }
@@ -300,15 +300,15 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
 
   if (warp == kWarps) {
     // ---- producer ---------------------------------------------------------------------------------------------------
-    const int page_rows = min(a.P, KEYS), per_tile = KEYS / page_rows;
+    const int page_rows = min(a.P, KEYS), page_bits = 31 - __clz(a.P), per_tile = KEYS >> min(page_bits, 31 - __clz(KEYS));
     while (sh.next()) {
-      const int last_page = (sh.s.len - 1) / a.P;
+      const int last_page = (sh.s.len - 1) >> page_bits;
       const int* table = a.table + sh.b * a.table_row;
       int batch = -1, id = 0;                       // pages 32 batch .. of the sequence, one a lane
       float2 scale = make_float2(1.f, 0.f);
       for (int tile = sh.first; tile < sh.last; ++tile, ++turn) {
         const int stage = turn % STAGES, phase = turn / STAGES & 1;
-        const int p0 = tile * KEYS / a.P;
+        const int p0 = tile * KEYS >> page_bits;
         if (p0 >> 5 != batch) {
           batch = p0 >> 5;
           const int p = batch * 32 + lane;
@@ -329,11 +329,16 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         __syncwarp();
         if (lane < n) {
           uint8_t* dst = smem + stage * 2 * TL::kSize + lane * page_rows * TL::kRow;
-          const int row = (tile * KEYS) % a.P, z = page * a.G + sh.head;
+          const int row = (tile * KEYS) & (a.P - 1), z = page * a.G + sh.head;
+          if (TL::kBoxes == 1 || per_tile == 1) {                           // all columns at once: they lie as the tile has them
+            tma_load_4d(dst, &map_k, full + stage, 0, row, 0, z);
+            tma_load_4d(dst + TL::kSize, &map_v, full + stage, 0, row, 0, z);
+          } else {
 #pragma unroll
-          for (int c = 0; c < TL::kBoxes; ++c) {
-            tma_load_3d(dst + c * KEYS * TL::kRow, &map_k, full + stage, c * (TL::kRow / TL::kBytes), row, z);
-            tma_load_3d(dst + TL::kSize + c * KEYS * TL::kRow, &map_v, full + stage, c * (TL::kRow / TL::kBytes), row, z);
+            for (int c = 0; c < TL::kBoxes; ++c) {
+              tma_load_4d(dst + c * KEYS * TL::kRow, &map_k, full + stage, 0, row, c, z);
+              tma_load_4d(dst + TL::kSize + c * KEYS * TL::kRow, &map_v, full + stage, 0, row, c, z);
+            }
           }
         }
       }
@@ -342,6 +347,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   }
 
   // ---- consumers ------------------------------------------------------------------------------------------------------
+  const int page_bits = 31 - __clz(a.P);
   const int g = lane >> 2, t = lane & 3, pi = g & 1 ? g ^ 4 : g;
   const int tid = threadIdx.x;
   // this lane's pieces of a tile: rows 8 apart and boxes lie the same way
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         float ks = 1.f;
         lv[j] = 0.f;
         if constexpr (F8) {
-          const int at = a.P >= KEYS ? 0 : 16 * j / a.P;
+          const int at = a.P >= KEYS ? 0 : 16 * j >> page_bits;
           const float2 sc = s_scale[stage * 4 + at];
           ks = sc.y == sc.y ? sc.x : sc.y;                                   // a page whose values hold no numbers shows at the keys that are seen
           lv[j] = sc.y == sc.y ? sc.y : 0.f;
@@ -817,7 +823,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
 typedef CUresult (*PagedEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Pages as [pages * G, P, D]; boxes of 128 bytes (a whole row where it is shorter) of min(P, KEYS) tokens of one page and head.
+// Pages as the tiles want them: boxes of min(P, KEYS) tokens of one page and head, in columns of 128 bytes (a whole row where it is shorter).
 template <bool F8, int D, int KEYS>
 int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
   static const PagedEncodeFn encode = [] {
@@ -828,10 +834,12 @@ int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
   }();
   if (encode == nullptr) return -20;
   using TL = Tile<F8, D, KEYS>;
-  const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(a.P), static_cast<cuuint64_t>(a.pages) * a.G};
-  const cuuint64_t strides[2] = {D * TL::kBytes, static_cast<cuuint64_t>(a.P) * D * TL::kBytes};
-  const cuuint32_t box[3] = {TL::kRow / TL::kBytes, static_cast<cuuint32_t>(a.P < KEYS ? a.P : KEYS), 1}, step[3] = {1, 1, 1};
-  const CUresult r = encode(map, F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
+  // [row of 128 bytes][token][128-byte column][page and head]; a page that is part of a tile comes column by column
+  const cuuint32_t rows = a.P < KEYS ? a.P : KEYS, columns = a.P < KEYS ? 1 : TL::kBoxes;
+  const cuuint64_t dims[4] = {TL::kRow / TL::kBytes, static_cast<cuuint64_t>(a.P), TL::kBoxes, static_cast<cuuint64_t>(a.pages) * a.G};
+  const cuuint64_t strides[3] = {D * TL::kBytes, TL::kRow, static_cast<cuuint64_t>(a.P) * D * TL::kBytes};
+  const cuuint32_t box[4] = {TL::kRow / TL::kBytes, rows, columns, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, TL::kRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 4000 + static_cast<int>(r);
