@@ -39,6 +39,10 @@
 // first, then the window's), the gate may be one number per head, and the output's channel pairs (m, m + dv / 2) are turned back by
 // the query's angles (values that were rotated by their positions).
 //
+// Ragged sequences (BIAS 5, and 6 in fp16): the queries are rows starts[b] .. starts[b + 1] - 1 of one [rows, Hq, D] tensor, the last of the lengths[b] keys and
+// values that batch entry b holds; both counts are read on the device.  Blocks count pairs of tiles through the sequences: sequence b has those from
+// starts[b] / 256 + b on, at most one of which is not taken.
+//
 // The reference calls at::scaled_dot_product_attention, or a query-chunked masked-math fallback
 // for windows (cc/include/tyr_attention.h:58-130).
 #include "common.cuh"
@@ -75,6 +79,9 @@ struct AttnParams {
   int gate_head;      // the gate is one number per (row, head)
   const float2* back; // [Tq, back_half] (cos, sin) of the query's turns (nullable)
   int back_half;
+  // ragged form only
+  const int *starts, *lengths;   // [B + 1], [B]
+  int rows;           // of the queries
 };
 
 constexpr int ATT_TBL_PAD = 256;       // table entries below distance 0 and past the window that boundary blocks can touch
@@ -118,6 +125,15 @@ __device__ __forceinline__ bool pair_exchange(uint2* mine, const uint2* theirs, 
   }
   other = __uint_as_float(a);
   return true;
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack_16x2(float a, float b) {
+  if constexpr (HALF) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -176,6 +192,7 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
                       const __grid_constant__ CUtensorMap tmV, AttnParams p) {
   constexpr bool kPenalty = BIAS == 1 || BIAS == 2;
   constexpr bool kKept = BIAS == 4, kGated = BIAS == 3 || kKept;
+  constexpr bool kRagged = BIAS == 5 || BIAS == 6, kHalf = BIAS == 6;
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   AttnSmem& s = *reinterpret_cast<AttnSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -184,11 +201,29 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
   const int lane = threadIdx.x & 31;
 
   // heavy (late) query tiles first: causal work grows with the row index
-  int rank, bh;
-  tile_of_block(p.order, blockIdx.x, rank, bh);
-  const int pair = p.order.tiles - 1 - rank;
-  const int head = bh % p.Hq;
-  const int batch = bh / p.Hq;
+  int rank, bh, pair, head, batch, q_row0 = 0, q_batch;
+  if constexpr (kRagged) {
+    pdl_wait();
+    const int unit = blockIdx.x / p.Hq;
+    head = blockIdx.x % p.Hq;
+    batch = -1;
+    for (int i = lane; i - lane < p.B; i += 32) batch += __popc(__ballot_sync(0xffffffffu, i < p.B && p.starts[i] / (2 * ATT_BM) + i <= unit));
+    if (batch < 0) return;
+    q_row0 = p.starts[batch];
+    p.Tq = p.starts[batch + 1] - q_row0;
+    p.Tk = p.lengths[batch];
+    if (p.Tq < 0 || q_row0 < 0 || q_row0 + p.Tq > p.rows || p.Tk < p.Tq || p.Tk > p.keep) return;      // recorded where the keys were brought
+    p.q_offset = p.Tk - p.Tq;
+    pair = unit - (q_row0 / (2 * ATT_BM) + batch);
+    if (pair * 2 * ATT_BM >= p.Tq) return;
+    q_batch = 0;
+  } else {
+    tile_of_block(p.order, blockIdx.x, rank, bh);
+    pair = p.order.tiles - 1 - rank;
+    head = bh % p.Hq;
+    batch = bh / p.Hq;
+    q_batch = batch;
+  }
   const int kv_head = head / (p.Hq / p.Hkv);
   const int row0 = pair * 2 * ATT_BM;
 
@@ -239,7 +274,7 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = s.tmem_base;
-  pdl_wait();                                   // everything above touched no global memory
+  if constexpr (!kRagged) pdl_wait();           // everything above touched no global memory
   constexpr uint32_t kChunk = ATT_BM * 64 * 2;   // one [128 x 64] bf16 swizzled chunk = 16 KB
 
   // Register re-allocation between warpgroups: the four softmax warpgroups keep 64 scores per thread in registers, the
@@ -258,7 +293,7 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
       mbar_expect_tx(&s.q_full, ntile * 2 * kChunk);
       for (int t = 0; t < ntile; ++t)
         for (int c = 0; c < 2; ++c)
-          tma_load_4d(s.q[t] + c * kChunk, &tmQ, &s.q_full, c * 64, head, row0 + t * ATT_BM, batch);
+          tma_load_4d(s.q[t] + c * kChunk, &tmQ, &s.q_full, c * 64, head, q_row0 + row0 + t * ATT_BM, q_batch);
       uint32_t it = 0;
       bool ok = true;
       for (int j = jfirst; j < jhi && ok; j = after(j, jlo), ++it) {
@@ -283,8 +318,8 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
   } else if (warp == 16) {
     // ------------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      constexpr uint32_t idesc_s = make_idesc_f16(1, ATT_BM, ATT_BN, 0, 0);   // Q K^T
-      constexpr uint32_t idesc_o = make_idesc_f16(1, ATT_BM, ATT_D, 0, 1);    // P V (V is MN-major)
+      constexpr uint32_t idesc_s = make_idesc_f16(kHalf ? 0 : 1, ATT_BM, ATT_BN, 0, 0);   // Q K^T
+      constexpr uint32_t idesc_o = make_idesc_f16(kHalf ? 0 : 1, ATT_BM, ATT_D, 0, 1);    // P V (V is MN-major)
       bool ok = mbar_wait(&s.q_full, 0, p.err, 600);
       tc_fence_after();
       auto issue_s = [&](int t, int st) {
@@ -491,7 +526,7 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
             }
             const float p0 = exp2f(e0);
             const float p1 = exp2f(e1);
-            pk[q] = pack_bf16x2(p0, p1);
+            pk[q] = pack_16x2<kHalf>(p0, p1);
             ls4[q & 3] += p0 + p1;
           }
           tmem_st_32x16(p_addr + c * 16, pk);
@@ -525,7 +560,7 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
           if (kKept && p.gate && p.gate_head && row_ok)
             inv = __fdividef(inv, 1.f + __expf(-__bfloat162float(p.gate[batch * p.g_batch_stride + static_cast<long long>(row) * p.g_row_stride + head * p.g_head_stride])));
         }
-        __nv_bfloat16* out = p.O + batch * p.o_batch_stride + static_cast<long long>(row) * p.o_row_stride +
+        __nv_bfloat16* out = p.O + q_batch * p.o_batch_stride + (q_row0 + static_cast<long long>(row)) * p.o_row_stride +
                              head * p.o_head_stride + h * 64;
         if (kKept && p.back != nullptr) {
           // eight channel pairs at a time, the two halves of the row taking turns
@@ -574,10 +609,10 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
                 }
               }
               uint4 u;
-              u.x = pack_bf16x2(__uint_as_float(o[q * 8 + 0]) * inv, __uint_as_float(o[q * 8 + 1]) * inv);
-              u.y = pack_bf16x2(__uint_as_float(o[q * 8 + 2]) * inv, __uint_as_float(o[q * 8 + 3]) * inv);
-              u.z = pack_bf16x2(__uint_as_float(o[q * 8 + 4]) * inv, __uint_as_float(o[q * 8 + 5]) * inv);
-              u.w = pack_bf16x2(__uint_as_float(o[q * 8 + 6]) * inv, __uint_as_float(o[q * 8 + 7]) * inv);
+              u.x = pack_16x2<kHalf>(__uint_as_float(o[q * 8 + 0]) * inv, __uint_as_float(o[q * 8 + 1]) * inv);
+              u.y = pack_16x2<kHalf>(__uint_as_float(o[q * 8 + 2]) * inv, __uint_as_float(o[q * 8 + 3]) * inv);
+              u.z = pack_16x2<kHalf>(__uint_as_float(o[q * 8 + 4]) * inv, __uint_as_float(o[q * 8 + 5]) * inv);
+              u.w = pack_16x2<kHalf>(__uint_as_float(o[q * 8 + 6]) * inv, __uint_as_float(o[q * 8 + 7]) * inv);
               *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = u;
             }
           }
@@ -744,4 +779,36 @@ extern "C" TYR_EXPORT int tyr_flash_fwd_kept(const void* q, const void* k, const
   ex.keep = keep; ex.gate_head = gate_head; ex.back_half = dv / 2;
   ex.back = static_cast<const float2*>(back);
   return flash_fwd_launch(q, k, v, o, nullptr, B, Hq, Hkv, T, T, dk, dv, strides, 1, window, 0, scale, nullptr, nullptr, err, stream, &ex);
+}
+
+// Attention of ragged rows q [rows, Hq, D] (strides of rows and heads) over the keys and values [B, Hkv, capacity, D] of their sequences (see the kernel's head);
+// out [rows, Hq, D].  dtype: 0 = bf16, 1 = fp16.  D: 64 or 128.
+int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
+                         int Hq, int Hkv, int D, long long capacity, int window, float scale, int dtype, int* err, cudaStream_t stream) {
+  const long long st[6] = {0, q_row, q_head, Hkv * capacity * D, D, capacity * D};
+  CUtensorMap tq, tk, tv;
+  int r;
+  if ((r = make_tmap_bthd(&tq, q, 1, rows, Hq, D, st[0], st[1], st[2], ATT_BM))) return 3000 + r;
+  if ((r = make_tmap_bthd(&tk, k, B, static_cast<int>(capacity), Hkv, D, st[3], st[4], st[5], ATT_BN))) return 4000 + r;
+  if ((r = make_tmap_bthd(&tv, v, B, static_cast<int>(capacity), Hkv, D, st[3], st[4], st[5], ATT_BN))) return 5000 + r;
+  auto kernel = dtype == 1 ? flash_fwd_d128_kernel<6> : flash_fwd_d128_kernel<5>;
+  constexpr size_t kSmem = sizeof(AttnSmem) + 1024;
+  static bool configured_dev[64][2] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!configured_dev[dev][dtype]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+    if (e != cudaSuccess) return 1000 + static_cast<int>(e);
+    configured_dev[dev][dtype] = true;
+  }
+  AttnParams p{};
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.causal = 1; p.window = window;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.O = static_cast<__nv_bfloat16*>(out); p.o_row_stride = static_cast<long long>(Hq) * D; p.o_head_stride = D;
+  p.err = err; p.k_steps = D / 16; p.dv = D; p.starts = starts; p.lengths = lengths; p.rows = rows;
+  p.keep = static_cast<int>(capacity);
+  const long long blocks = (static_cast<long long>(rows) / (2 * ATT_BM) + B) * Hq;
+  if (blocks > 0x7fffffff) return -5;
+  const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), dim3(640), kSmem, stream, tq, tk, tv, p);
+  return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }

@@ -820,6 +820,72 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
   }
 }
 
+// The pages of every sequence as the ragged form of the attention kernel on tcgen05 (csrc/attention_fwd.cu) takes them: keys and values [B, G, capacity, D] in the
+// queries' type, zeros behind the end up to a multiple of 128.  A (sequence, head) is one blockIdx.(z, y).  The codes of a page whose
+// scales are no numbers give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence are zeroed on the way.
+template <typename T, bool F8>
+__global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedAttnArgs a, void* k_out, void* v_out, long long capacity) {
+  pdl_entry();
+  const int b = blockIdx.z, head = blockIdx.y, lanes = a.D / 8, lane = threadIdx.x % lanes, per = 256 / lanes;
+  if (b == 0 && head == 0)
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x)
+      if (row < a.starts[0] || row >= a.starts[a.B])
+        for (int i = threadIdx.x * 8; i < a.H * a.D; i += 2048) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * a.D + i) = make_uint4(0u, 0u, 0u, 0u);
+  const Seq s = seq_of<16, 128>(a, b);
+  if (s.n == 0) return;
+  const int end = min(static_cast<long long>((s.len + 127) / 128 * 128), capacity), page_bits = 31 - __clz(a.P);
+  // four tokens a thread, their pages and then their rows in flight together
+  for (int token0 = s.tile0 * 128 + blockIdx.x * 4 * per; token0 < end; token0 += gridDim.x * 4 * per) {
+    long long from[4];
+    float ks[4], vs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int token = token0 + i * per + threadIdx.x / lanes;
+      from[i] = -1;
+      if (token >= s.len) continue;
+      int page = a.table[b * a.table_row + (token >> page_bits)];
+      if (page < 0 || page >= a.pages) {
+        report_error(a.err, ERR_BOUNDS, page);
+        page = 0;
+      }
+      const long long at = static_cast<long long>(page) * a.G + head;
+      from[i] = (at * a.P + (token & (a.P - 1))) * a.D + lane * 8;
+      if (F8) ks[i] = a.k_scale[at], vs[i] = a.v_scale[at];
+    }
+    typedef typename std::conditional<F8, uint2, uint4>::type Raw;          // eight channels
+    Raw k[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k[i] = v[i] = Raw{};
+      if (from[i] < 0) continue;
+      k[i] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(a.k_pages) + from[i] * (F8 ? 1 : 2));
+      v[i] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(a.v_pages) + from[i] * (F8 ? 1 : 2));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int token = token0 + i * per + threadIdx.x / lanes;
+      if (token >= end) continue;
+      const long long to = ((static_cast<long long>(b) * a.G + head) * capacity + token) * a.D + lane * 8;
+      uint4 x, y;
+      if constexpr (F8) {
+        const bool none = from[i] < 0, lost = !none && vs[i] != vs[i];
+        const float kf = none ? 0.f : lost ? vs[i] : ks[i], vf = none || lost ? 0.f : vs[i];
+        const auto two = [](uint32_t codes, float scale) {
+          const float2 f = Num<__half>::two(halves_of_codes(codes));
+          return Num<T>::pack(f.x * scale, f.y * scale);
+        };
+        x = make_uint4(two(k[i].x, kf), two(k[i].x >> 16, kf), two(k[i].y, kf), two(k[i].y >> 16, kf));
+        y = make_uint4(two(v[i].x, vf), two(v[i].x >> 16, vf), two(v[i].y, vf), two(v[i].y >> 16, vf));
+      } else {
+        x = k[i];
+        y = v[i];
+      }
+      *reinterpret_cast<uint4*>(static_cast<T*>(k_out) + to) = x;
+      *reinterpret_cast<uint4*>(static_cast<T*>(v_out) + to) = y;
+    }
+  }
+}
+
 typedef CUresult (*PagedEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
@@ -901,7 +967,29 @@ int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool 
 
 }  // namespace tyr
 
+int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
+                         int Hq, int Hkv, int D, long long capacity, int window, float scale, int dtype, int* err, cudaStream_t stream);
+
 using namespace tyr;
+
+// The same result for many new tokens a sequence: the pages laid out in `part` (2 * B * G * capacity * D numbers of the queries' type, capacity a multiple of 128 that
+// holds the table's tokens), then the kernel on tcgen05.
+extern "C" TYR_EXPORT int tyr_paged_attention_gathered(const void* packed, int dtype, long long capacity, void* stream) {
+  const PagedAttnArgs& a = *static_cast<const PagedAttnArgs*>(packed);
+  if (a.rows <= 0 || a.B <= 0 || a.B > 65535 || a.H <= 0 || a.G <= 0 || a.G > 65535 || a.H % a.G != 0 || a.pages <= 0 || a.width <= 0 || a.window < 0) return -1;
+  if ((a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) || (a.D != 64 && a.D != 128) || a.starts == nullptr || a.part == nullptr) return -2;
+  if (capacity % 128 != 0 || capacity < static_cast<long long>(a.width) * a.P || capacity > 0x7fffffffLL || (a.k_scale != nullptr) != (a.v_scale != nullptr)) return -3;
+  void *k = a.part, *v = reinterpret_cast<uint8_t*>(a.part) + 2LL * a.B * a.G * capacity * a.D;
+  // some eight rounds of blocks over the SMs' places, or as many as the longest sequence may fill
+  const long long chunks = capacity * a.D / 8192, most = 9472 / (static_cast<long long>(a.G) * a.B) + 1;
+  const dim3 grid(static_cast<unsigned>(chunks < most ? chunks : most), a.G, a.B);
+  const bool f8 = a.k_scale != nullptr;
+  const auto gather = dtype == 0 ? (f8 ? paged_gather_kernel<__nv_bfloat16, true> : paged_gather_kernel<__nv_bfloat16, false>)
+                                 : (f8 ? paged_gather_kernel<__half, true> : paged_gather_kernel<__half, false>);
+  const cudaError_t e = launch_dependent(gather, grid, dim3(256), 0, (cudaStream_t)stream, a, k, v, capacity);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return tyr_flash_fwd_ragged(a.q, a.q_row, a.q_head, k, v, a.out, a.starts, a.lengths, a.rows, a.B, a.H, a.G, a.D, capacity, a.window, a.scale, dtype, a.err, (cudaStream_t)stream);
+}
 
 // dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows of a tile: 16, or 128 (64 of heads of 256).
 extern "C" TYR_EXPORT int tyr_paged_attention(const void* packed, int dtype, int rows, void* stream) {

@@ -107,6 +107,8 @@ def check_attention(batch, got, window=None, scale=None, dtype=None):
     # (D + 3) roundings of the sum of magnitudes, and a probability's relative error is the scores' difference from the maximum's, twice that; exp2 and the sums
     # over the keys add some 2^-20
     p = HALF_STEP[torch.bfloat16 if batch.store.k.dtype == torch.bfloat16 else torch.float16]
+    if got.is_cuda and gathered(batch):
+        p = HALF_STEP[got.dtype]                       # the kernel on tcgen05 rounds them to the queries' type
     tol = HALF_STEP[dtype] * want.abs() + size * (1.01 * p + 2.0 ** -20 + 2 * 1.45 * (batch.D + 3) * 2.0 ** -24 * reach) + 1e-7
     err = (got.to(F64) - want).abs()
     assert torch.isfinite(got).all()
@@ -312,8 +314,19 @@ ATTENDS = [
     (dict(held=[1500, 0], new=[200, 333]), False, 2, 5, 16, 128, torch.bfloat16, torch.bfloat16, None),
     (dict(held=[1500, 0], new=[200, 333]), False, 1, 6, 64, 256, torch.bfloat16, pc.E4M3, 500),
     (dict(held=[7] * 150, new=[n % 3 for n in range(150)]), False, 1, 2, 16, 64, torch.float16, pc.E4M3, None),
+    (dict(held=[0, 1000, 130, 7, 0, 300], new=[257, 1, 256, 0, 511, 129]), False, 2, 3, 16, 128, torch.bfloat16, pc.E4M3, None),
+    (dict(held=[0, 1000, 130, 7, 0, 300], new=[257, 1, 256, 0, 511, 129]), False, 4, 4, 32, 64, torch.bfloat16, pc.E4M3, 100),
+    (dict(held=[0, 1000, 130, 7, 0, 300], new=[257, 1, 256, 0, 511, 129]), False, 1, 5, 128, 128, torch.float16, torch.float16, 333),
+    (dict(held=[0, 1000, 130, 7, 0, 300], new=[257, 1, 256, 0, 511, 129]), False, 2, 1, 64, 64, torch.bfloat16, torch.bfloat16, None),
+    (dict(held=[0, 1000, 130, 7, 0, 300], new=[257, 1, 256, 0, 511, 129]), False, 1, 2, 64, 128, torch.float16, pc.E4M3, None),
+    (dict(held=[5000], new=[1000]), False, 2, 4, 64, 128, torch.bfloat16, pc.E4M3, None),
     (dict(held=[40 * n for n in range(90)], new=[1] * 90), True, 2, 4, 64, 128, torch.bfloat16, pc.E4M3, None),
 ]
+
+
+def gathered(batch):
+    return batch.args[2] is not None and pc.gathers(batch.q.dtype, batch.store.k_scale is not None, batch.rows, len(batch.lens), batch.H, batch.G, batch.D,
+                                                    batch.table.shape[1] * batch.P, 1.0)
 
 
 def run_attention(dev, seqs, decode, G, R, P, D, dtype, cache, window, rows_behind=0):
@@ -334,6 +347,26 @@ def test_attention_cpu(case):
 def test_attention_gpu(case):
     run_attention("cuda", *ATTENDS[case], rows_behind=0 if ATTENDS[case][1] else 3)
     _common.raise_on_device_error()
+
+
+RAGGED_CASES = [i for i, c in enumerate(ATTENDS) if not c[1] and c[5] <= 128 and not (c[6] == torch.float16 and c[7] == pc.E4M3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", RAGGED_CASES)
+@pytest.mark.parametrize("way", (True, False))
+def test_both_ways_over_ragged_rows(monkeypatch, case, way):
+    monkeypatch.setattr(pc, "gathers", lambda *a: way)
+    run_attention("cuda", *ATTENDS[case], rows_behind=3)
+    _common.raise_on_device_error()
+
+
+def test_way_by_rows_heads_and_types():
+    bf, half = torch.bfloat16, torch.float16
+    way = lambda rows, B=6, H=20, G=4, D=128, dtype=bf, f8=True, cap=3000, scale=0.1: pc.gathers(dtype, f8, rows, B, H, G, D, cap, scale)
+    assert way(6 * 256) and way(6 * 100) and not way(6 * 8) and not way(6)
+    assert not way(6 * 256, D=256) and not way(6 * 256, dtype=half) and way(6 * 256, dtype=half, f8=False) and not way(6 * 256, scale=-1.0)
+    assert not way(6 * 256, cap=10 ** 6) and not way(2 * 64, B=2, H=10, G=10)
 
 
 @pytest.mark.gpu
@@ -375,6 +408,18 @@ def test_queries_of_any_size():
         batch.q = (batch.q * size).contiguous()
         scale = 0.1 / size
         check_attention(batch, paged_attention(batch.q, batch.store, *batch.args, scale=scale), scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", (True, False))
+def test_poisoned_pages_over_ragged_rows(monkeypatch, way):
+    """Rows before a token that is no number do not show it, though they share its tile of keys."""
+    monkeypatch.setattr(pc, "gathers", lambda *a: way)
+    for name in ("k_scale", "v_scale"):
+        batch = Batch(held=[100], new=[60], G=2, R=2, P=16, D=64, dtype=torch.bfloat16, cache=pc.E4M3, dev="cuda", strided=False)
+        getattr(batch.store, name)[int(batch.table[0, 8]), 1] = math.nan            # positions 128 to 143
+        out = paged_attention(batch.q, batch.store, *batch.args)
+        assert torch.isfinite(out[:, :2]).all() and torch.isfinite(out[:28]).all() and torch.isnan(out[28:, 2:]).all()
 
 
 def poisoned(dev):

@@ -40,6 +40,7 @@ def _sigs(lib_):
         lib_.tyr_paged_append.argtypes, lib_.tyr_paged_append.restype = [P, I, P], I
     if hasattr(lib_, "tyr_paged_attention"):
         lib_.tyr_paged_attention.argtypes, lib_.tyr_paged_attention.restype = [P, I, I, P], I
+        lib_.tyr_paged_attention_gathered.argtypes, lib_.tyr_paged_attention_gathered.restype = [P, I, ctypes.c_longlong, P], I
         lib_.tyr_paged_attention_resident.argtypes, lib_.tyr_paged_attention_resident.restype = [I] * 5, I
 
 
@@ -274,6 +275,21 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     return out
 
 
+# the most that pages laid out for the kernel on tcgen05 may take
+GATHER_MAX_BYTES = 2 ** 30
+
+
+def gathers(dtype: torch.dtype, f8: bool, rows: int, sequences: int, heads: int, kv_heads: int, D: int, capacity: int, scale: float) -> bool:
+    """Whether the pages are laid out for the tensor core's kernel first.  It serves heads of 64 and 128 and numbers of the queries' type (a code times its page's scale
+    may leave fp16's range), and takes 128 or 256 rows of one head against 128 keys in 2.5 us an SM, however few rows there are; the other kernel multiplies at 140
+    TFLOP/s.  In us a key of context, with the pages' way at 5 TB/s; measured, other / this, 3000 tokens of context: 6 sequences, 20 heads of 128, 32 / 64 / 256
+    new tokens each 72 / 64, 98 / 65, 273 / 77; 16, 48 heads 264 / 357, 418 / 364, 1476 / 428; 2, 10 heads 38 / 59, 40 / 60, 67 / 68."""
+    if D > 128 or not scale > 0 or (f8 and dtype == torch.float16) or sequences > 65535 or 4 * sequences * kv_heads * (capacity + 127) * D > GATHER_MAX_BYTES:
+        return False
+    blocks = sequences * -(-rows // (256 * sequences)) * heads
+    return max(1.0, blocks / 148) * 2.5 / 128 + sequences * kv_heads * D * (6 if f8 else 8) / 5e6 < rows * heads * D * 4 / 1.4e8
+
+
 @functools.lru_cache(maxsize=256)
 def _resident(index: int, number: int, f8: bool, D: int, tile: int, few: bool) -> int:
     """CTAs of a form of the kernel that device ``index`` holds at once: the shares that a call's work is cut into."""
@@ -321,6 +337,14 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     q, f8 = _rows_of(q), store.k_scale is not None
     stride, R = q.stride(), H // G
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if starts is not None and gathers(dtype, f8, rows, B, H, G, D, width * P, scale):
+        capacity = -(-width * P // 128) * 128
+        work = torch.empty(2 * B * G * capacity * D, dtype=dtype, device=device)
+        packed = _ATTEND.pack(q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), store.k_scale.data_ptr() if f8 else 0, store.v_scale.data_ptr() if f8 else 0,
+                              table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), work.data_ptr(), err_word(device).data_ptr(), stride[0], stride[1], table_row, rows, B, H, G,
+                              D, P, pages, width, min(window or 0, 2 ** 30), 0, scale, 0)
+        check(lib().tyr_paged_attention_gathered(packed, number, capacity, cur_stream(device)), "paged_attention")
+        return out
     tile = (64 if D == 256 else 128) if starts is not None and rows * R > 16 * B else 16
     whole = width * P <= WHOLE_MAX_KEYS
     work = None
