@@ -8,8 +8,8 @@
 //
 // A cluster of CTAs holds a row in shared memory: it is read once.  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
 // decide, by exact sums above, in and below the bin that the counts suggest.  What is left of a bin goes into a list that one CTA sorts; equal logits beyond the list
-// are cut by their indices alone.  top-k up to the list's size needs no counts over all: the k-th largest of the threads' maxima bounds the k-th logit from below, and
-// the few logits above it are listed.  Compiled without fast math.
+// are cut by their indices alone.  What top-k leaves of up to 1024 is listed whole, and one CTA cuts and draws among it, by bins of whole-number weights; for small k
+// the k-th largest of the threads' maxima, which bounds the k-th logit from below, saves the counts over all.  Compiled without fast math.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -19,6 +19,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048, kSampleList = 1024, kSampleCluster = 16;
+constexpr int kSampleMost = 2048;                                          // of a list that holds all that top-k leaves
+constexpr int kSampleScratch = 3 * kSampleMost * 8;                        // bytes that CTA 0 needs beside it, where its logits were
 constexpr int kSampleSlice = 16384, kSampleLargest = 40960;                // logits of a CTA: with two of them on an SM, and at most
 
 struct SampleArgs {
@@ -79,12 +81,11 @@ struct Weights {                         // 2^((x - top) c), all lanes of a warp
 struct Partial { double above, in, all; uint32_t count, low, high, pad; };
 
 struct SampleShared {
-  uint32_t bins[kSampleBins], total[kSampleBins];
-  unsigned long long list[kSampleList];
-  union {                                                                  // of the list
-    double weight[kSampleList];
-    unsigned long long fixed[kSampleList];
+  union {
+    struct { uint32_t bins[kSampleBins], total[kSampleBins]; };
+    unsigned long long mass[kSampleBins];
   };
+  unsigned long long list[kSampleList], fixed[kSampleList];                // items and their weights
   double warp_sums[kSampleWarps], cta_sums[kSampleCluster], run_sums[kSampleLargest / kSampleThreads];
   Partial part[2][kSampleCluster], warp_part[kSampleWarps];
   double warp_above[kSampleWarps];                                         // of a warp's logits above the bin of the cut
@@ -94,6 +95,7 @@ struct SampleShared {
   uint32_t scan[kSampleWarps], listed, collected, counts[kSampleCluster * kSampleWarps];
   double scan_d[kSampleWarps];
   Place cut;
+  unsigned long long scan_u[kSampleWarps], base;
   int found, flag;
 };
 
@@ -124,6 +126,25 @@ __device__ __forceinline__ double block_scan_d(double v, double* s, double& tota
   __syncthreads();
   double before = 0.0;
   total = 0.0;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) {
+    if (i < warp) before += s[i];
+    total += s[i];
+  }
+  return v + before;
+}
+__device__ __forceinline__ unsigned long long block_scan_u(unsigned long long v, unsigned long long* s, unsigned long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = v;
+  __syncthreads();
+  unsigned long long before = 0;
+  total = 0;
 #pragma unroll
   for (int i = 0; i < kSampleWarps; ++i) {
     if (i < warp) before += s[i];
@@ -322,6 +343,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     cluster.sync();
     return lead->listed;
   };
+  constexpr int kMaximaK = 128;                                            // with more, too many threads hold several of the k
   constexpr int kFewItems = 256;                                           // 50 items take 0.3 us so and 2.5 by the network, 514 more than by it
   const auto sort_list = [&](int n) {
     if (n <= kFewItems) {
@@ -341,81 +363,205 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   Place cut{1u, 0xffffffffu};                                              // keeps all
 
   // ---- top-k -------------------------------------------------------------------------------------------------------------
-  if (k_row > 0 && k_row < a.V) {
-    bool listed = false;
-    if (k_row <= kSampleList) {
+  if (k_row > 0 && k_row < a.V && k_row <= kSampleList) {
+    // the bin with the k-th logit, or with the k-th of the threads' maxima, which lies no higher
+    if (k_row <= kMaximaK && a.V >= 64 * k_row) {
       const int own = bin_of(own_top);
       if (own < kSampleBins) atomicAdd(&s.bins[own], 1u);
-      merge_bins();
-      const int bin = bin_reaching(k_row);                                 // none: fewer maxima than k
-      const uint32_t n = gather([&](float, uint32_t, uint32_t) { return true; }, [&](float v) { return bin < kSampleBins && bin_of(v) <= bin; });
-      listed = bin < kSampleBins && n <= kSampleList;
-      if (listed) {
-        // ---- all that can stay lies in CTA 0's list ----------------------------------------------------------------------------
-        cluster.sync();                                                    // the others have read its length
-        if (rank != 0) return;
-        sort_list(n);
-        const int kept = min(static_cast<int>(n), k_row);
-        constexpr int PER = kSampleList / kSampleThreads;
-        double w[PER], sum = 0.0, total;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int at = tid * PER + i;
-          const double v = weigh(at < kept ? value_of(static_cast<uint32_t>(s.list[at] >> 32)) : 0.f);
-          w[i] = at < kept ? v : 0.0;
-          sum += w[i];
+    } else {
+#pragma unroll 8
+      for (int j = 0; j < its; ++j) {
+        const int b = bin_of(x[32 * j]);
+        if (b < kSampleBins) atomicAdd(&s.bins[b], 1u);
+      }
+    }
+    merge_bins();
+    const int last = bin_reaching(k_row);                                  // none: not that many
+    if (tid == 0) s.collected = 0;
+    __syncthreads();
+    if (last < kSampleBins - 1) {
+#pragma unroll 4
+      for (int j = 0; j < its; ++j) {
+        const float v = x[32 * j];
+        if (far_of(v) < last + 1) {
+          const uint32_t at = atomicAdd(&s.collected, 1u);
+          if (at < kSampleList) s.own[at] = static_cast<unsigned long long>(key_of(v)) << 32 | ~index_of(j);
         }
-        double before = block_scan_d(sum, s.scan_d, total) - sum;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int at = tid * PER + i;
-          const bool in = at < kept && (at == 0 || (w[i] >= m && (!by_mass || before < p * total)));
-          before += w[i];
-          s.weight[at] = in ? w[i] : 0.0;
-        }
+      }
+    }
+    __syncthreads();
+    const uint32_t own_n = s.collected;
+    if (tid < C) cluster.map_shared_rank(s.counts, tid)[rank] = own_n;
+    cluster.sync();                                                        // from here on nobody looks at logits, if all fits
+    uint32_t before = 0, n = 0;
+    bool fits = last < kSampleBins - 1;
+    for (int r = 0; r < C; ++r) {
+      fits &= s.counts[r] <= kSampleList;
+      if (r < rank) before += s.counts[r];
+      n += s.counts[r];
+    }
+    fits &= n <= kSampleMost;
+    if (fits) {
+      unsigned long long* list = reinterpret_cast<unsigned long long*>(s_logits);
+      unsigned long long* to = cluster.map_shared_rank(list, 0) + before;
+      for (int i = tid; i < static_cast<int>(own_n); i += kSampleThreads) to[i] = s.own[i];
+      cluster.sync();
+      if (rank != 0) return;
+      // ---- all that can stay lies in CTA 0's list: weights as whole numbers of 2^-52, whose sums do not depend on their order -----------
+      unsigned long long *some = list + kSampleMost, *some_w = some + kSampleMost;
+      constexpr int PER = kSampleMost / kSampleThreads, BINS = kSampleBins / kSampleThreads;
+      constexpr double kUnit = 4503599627370496.0;
+      // the first index whose running weight passes the aim, else the last: from the items (~index in their lower halves), their weights and what lies before them
+      const auto draw_from = [&](unsigned long long item, unsigned long long w, unsigned long long base, const unsigned long long* items, const unsigned long long* weights, int n,
+                                 double aim) {
+        if (w == 0) return;
+        const uint32_t mine = static_cast<uint32_t>(item);
+        unsigned long long upto = base;
+        for (int j = 0; j < n; ++j) upto += static_cast<uint32_t>(items[j]) >= mine ? weights[j] : 0ull;
+        if (static_cast<double>(upto) > aim) atomicMax(&s.best, static_cast<unsigned long long>(mine) + 1);
+        atomicMax(&s.bests[0], static_cast<unsigned long long>(~mine) + 1);
+      };
+      const auto write_token = [&]() {
         __syncthreads();
-        // into vocabulary order: ~index in the upper half sorts the lowest first
-        unsigned long long moved[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int at = tid * PER + i;
-          moved[i] = at < kept && s.weight[at] > 0.0 ? s.list[at] << 32 | static_cast<unsigned>(at) : 0ull;
-        }
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (moved[i] != 0) s.list[atomicAdd(&s.listed, 1u)] = moved[i];
-        if (tid == 0) s.found = 0x7fffffff, s.flag = 0;
-        __syncthreads();
-        const int left = s.listed;
-        sort_list(left);
-        double v[PER];
-        sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int at = tid * PER + i;
-          v[i] = at < left ? s.weight[static_cast<uint32_t>(s.list[at])] : 0.0;
-          sum += v[i];
-        }
-        double upto = block_scan_d(sum, s.scan_d, total) - sum;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          upto += v[i];
-          if (v[i] > 0.0) {
-            atomicMax(&s.flag, tid * PER + i);
-            if (upto > u * total) atomicMin(&s.found, tid * PER + i);
-          }
-        }
-        __syncthreads();
-        if (tid == 0) a.token[row] = ~static_cast<uint32_t>(s.list[min(s.found, s.flag)] >> 32);
+        if (tid == 0) a.token[row] = s.best != 0 ? ~static_cast<uint32_t>(s.best - 1) : static_cast<uint32_t>(s.bests[0] - 1);
+      };
+      if (n <= kFewItems) {                                                // one a thread, in order: 50 items take 9 us less so than by bins
+        block_rank(list, some, n);
+        const unsigned long long mine = tid < static_cast<int>(n) ? list[tid] : 0;
+        bool stay = tid < min(static_cast<int>(n), k_row);
+        const double exact = weigh(stay ? value_of(static_cast<uint32_t>(mine >> 32)) : top);
+        unsigned long long w = stay ? static_cast<unsigned long long>(exact * kUnit) : 0, total;
+        const unsigned long long ahead = block_scan_u(w, s.scan_u, total) - w;
+        stay &= exact >= m && (!by_mass || tid == 0 || static_cast<double>(ahead) < p * static_cast<double>(total));
+        if (!stay) w = 0;
+        if (tid < static_cast<int>(n)) some_w[tid] = w;
+        if (tid == 0) s.best = 0, s.bests[0] = 0;
+        block_scan_u(w, s.scan_u, total);
+        draw_from(mine, w, 0, list, some_w, n, u * static_cast<double>(total));
+        write_token();
         return;
       }
-      cluster.sync();
-      if (tid == 0) s.listed = 0;
-      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
-      cluster.sync();
+      unsigned long long item[PER], w[PER];
+      int bin[PER];
+      bool in[PER];
+      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.total[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < PER; ++r) {
+        const int i = tid + r * kSampleThreads;
+        in[r] = i < static_cast<int>(n);
+        item[r] = in[r] ? list[i] : 0;
+        const float v = in[r] ? value_of(static_cast<uint32_t>(item[r] >> 32)) : top;
+        w[r] = static_cast<unsigned long long>(weigh(v) * kUnit);
+        bin[r] = bin_of(v);
+        if (in[r]) atomicAdd(&s.total[bin[r]], 1u);
+      }
+      __syncthreads();
+      // items of one bin, listed in any order: their number, after a barrier
+      const auto bring = [&](int b, const int (&of)[PER]) {
+        __syncthreads();
+        if (tid == 0) s.collected = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+          if (in[r] && of[r] == b) {
+            const uint32_t at = atomicAdd(&s.collected, 1u);
+            some[at] = item[r];
+            some_w[at] = w[r];
+          }
+        __syncthreads();
+        return static_cast<int>(s.collected);
+      };
+      const int cut_k = bin_reaching(min(static_cast<uint32_t>(k_row), n));
+      uint32_t above = 0, all;
+      for (int i = tid; i < cut_k; i += kSampleThreads) above += s.total[i];
+      block_scan(above, s.scan, all);
+      const int some_n = bring(cut_k, bin);
+#pragma unroll
+      for (int r = 0; r < PER; ++r) {
+        if (in[r] && bin[r] == cut_k) {
+          int rank_in = 0;
+          for (int j = 0; j < some_n; ++j) rank_in += some[j] > item[r];
+          in[r] = rank_in < k_row - static_cast<int>(all);
+        } else {
+          in[r] &= bin[r] < cut_k;
+        }
+      }
+      // weights by bins (any numbering of 2048), and the bin in which their running sum passes `aim`, with what lies before it; the last that holds any, else
+      const auto passing_bin = [&](const int (&of)[PER], auto passes) {
+        __syncthreads();
+        for (int i = tid; i < kSampleBins; i += kSampleThreads) s.mass[i] = 0;
+        if (tid == 0) s.found = kSampleBins, s.flag = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+          if (in[r] && w[r] != 0) atomicAdd(&s.mass[of[r]], w[r]);
+        __syncthreads();
+        unsigned long long sum = 0, total, v[BINS];
+#pragma unroll
+        for (int i = 0; i < BINS; ++i) sum += v[i] = s.mass[tid * BINS + i];
+        unsigned long long upto = block_scan_u(sum, s.scan_u, total) - sum, start[BINS];
+        passes(0ull, total);                                               // every thread learns the whole
+#pragma unroll
+        for (int i = 0; i < BINS; ++i) {
+          start[i] = upto;
+          upto += v[i];
+          if (v[i] == 0) continue;
+          atomicMax(&s.flag, tid * BINS + i);
+          if (passes(upto, total)) atomicMin(&s.found, tid * BINS + i);
+        }
+        __syncthreads();
+        const int at = s.found < kSampleBins ? s.found : s.flag;
+#pragma unroll
+        for (int i = 0; i < BINS; ++i)
+          if (tid * BINS + i == at) s.base = start[i];
+        __syncthreads();
+        return at;
+      };
+      if (by_mass) {
+        unsigned long long whole = 0, total;
+#pragma unroll
+        for (int r = 0; r < PER; ++r) whole += in[r] ? w[r] : 0;
+        block_scan_u(whole, s.scan_u, total);
+        const double aim = fmax(p * static_cast<double>(total), 0.5);       // nothing lies before the first
+        const int at = passing_bin(bin, [&](unsigned long long upto, unsigned long long) { return static_cast<double>(upto) >= aim; });
+        const unsigned long long base = s.base;
+        const int m_n = bring(at, bin);
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+          if (in[r] && bin[r] == at) {
+            unsigned long long ahead = base;
+            for (int j = 0; j < m_n; ++j) ahead += some[j] > item[r] ? some_w[j] : 0ull;
+            in[r] = static_cast<double>(ahead) < aim;
+          } else {
+            in[r] &= bin[r] < at;
+          }
+        }
+      }
+      // the draw, in vocabulary order
+#pragma unroll
+      for (int r = 0; r < PER; ++r) {
+        const double exact = weigh(in[r] ? value_of(static_cast<uint32_t>(item[r] >> 32)) : top);
+        in[r] = in[r] && exact >= m;
+        bin[r] = static_cast<int>(static_cast<unsigned long long>(~static_cast<uint32_t>(item[r])) * kSampleBins / static_cast<unsigned>(a.V));
+      }
+      double draw_aim = 0.0;
+      const int at = passing_bin(bin, [&](unsigned long long upto, unsigned long long total) {
+        draw_aim = u * static_cast<double>(total);
+        return static_cast<double>(upto) > draw_aim;
+      });
+      const unsigned long long base = s.base;
+      if (tid == 0) s.best = 0, s.bests[0] = 0;
+      const int d_n = bring(at, bin);
+#pragma unroll
+      for (int r = 0; r < PER; ++r)
+        if (in[r] && bin[r] == at) draw_from(item[r], w[r], base, some, some_w, d_n, draw_aim);
+      write_token();
+      return;
     }
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
+    if (tid == 0) s.listed = 0;
+    cluster.sync();
   }
 
   const auto fix_of = [&](float largest) {                                 // 2^52 over the power of two above its weight
@@ -808,7 +954,7 @@ int sample_form(SampleArgs a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = a.slice * 4;
+  cfg.dynamicSmemBytes = a.slice * 4 > kSampleScratch ? a.slice * 4 : kSampleScratch;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

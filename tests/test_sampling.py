@@ -69,6 +69,9 @@ CASES = [
     (8, 33333, torch.float32, 2.0, dict(top_k=5000, top_p=0.9)), (8, 33333, torch.float16, 2.0, dict(top_k=5000)), (8, 33333, torch.float32, 2.0, dict(top_k=1024, min_p=0.01)),
     (8, 33333, torch.float32, 2.0, dict(temperature=1e-3, top_p=0.9)), (8, 33333, torch.float32, 2.0, dict(temperature=50.0, top_p=0.7, top_k=20000)),
     (8, 33333, torch.float32, 2.0, dict(min_p=0.1)), (8, 33333, torch.float32, 2.0, dict(top_k=1)),
+    (8, 33333, torch.bfloat16, 2.0, dict(top_k=1000, top_p=0.9)), (8, 33333, torch.bfloat16, 0.1, dict(top_k=300, top_p=0.5, min_p=0.9)), (8, 3001, torch.float16, 0.0, dict(top_k=1024, top_p=0.7)),
+    (8, 1500, torch.float32, 0.0, dict(top_k=1024)), (8, 140, torch.float32, 2.0, dict(top_k=128, top_p=0.9)), (8, 33333, torch.float32, 60.0, dict(top_k=700, temperature=0.5)),
+    (8, 33333, torch.float32, 1e-3, dict(top_k=1024, top_p=0.99, min_p=0.999)),
 ]
 LARGE = [(3, 151936, torch.float32, 2.0, dict(temperature=0.7, top_k=50, top_p=0.9)), (150, 65536, torch.float32, 2.0, dict(top_p=0.95)), (20, 262144, torch.float32, 2.0, dict(top_p=0.95)),
          (5, 248320, torch.bfloat16, 2.0, "mixed"), (2, 300001, torch.float16, 3.0, dict(top_p=0.9)), (2, MAX_VOCAB, torch.float32, 2.0, dict(top_p=0.9, top_k=100000))]
