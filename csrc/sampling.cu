@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     own_top = own_top == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
   }
-  const double c = fmax(1.4426950408889634 / T_row, 1e-300);
+  const double c = fmin(fmax(1.4426950408889634 / T_row, 1e-300), 1e300);      // finite: no distance of 0 becomes NaN
   const Weights weigh{exp2(lane / 32.0), static_cast<double>(top), c};
   const double u = a.draws64 ? static_cast<const double*>(a.draws)[row] : static_cast<double>(static_cast<const float*>(a.draws)[row]);
   const bool by_mass = p < 1.0;

@@ -621,3 +621,84 @@ def test_prompt_pieces_and_steps_together(cache):
         if step:
             assert all(bool((out[b] == 0).all()) for b in range(3) if not new[b])
     _common.raise_on_device_error()
+
+
+SHIFTED = [(STEPS, True, 4, 5, 16, 128, torch.bfloat16, pc.E4M3, 64, True), (RAGGED, False, 2, 3, 32, 64, torch.float16, torch.float16, 16, True)]
+
+
+@pytest.mark.parametrize("case", range(len(SHIFTED)))
+def test_norm_of_one_plus_weight_cpu(case):
+    run_append("cpu", *SHIFTED[case], one_plus_w=True, eps=0.03)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(SHIFTED)))
+def test_norm_of_one_plus_weight_gpu(case):
+    run_append("cuda", *SHIFTED[case], one_plus_w=True, eps=0.03)
+    _common.raise_on_device_error()
+
+
+def test_weights_of_another_type_and_gradients_are_refused():
+    b = small()
+    table, lens, _ = b.args
+    weight = torch.ones(64)
+    need = lambda t: t.clone().requires_grad_(True)
+    for call in (lambda: paged_append(b.store, b.k, b.v, table, lens, k_weight=weight), lambda: paged_append(b.store, b.k, b.v, table, lens, q=b.q, q_weight=weight),
+                 lambda: paged_append(b.store, need(b.k), b.v, table, lens), lambda: paged_append(b.store, b.k, need(b.v), table, lens),
+                 lambda: paged_append(b.store, b.k, b.v, table, lens, q=need(b.q)), lambda: paged_attention(need(b.q), b.store, table, lens)):
+        with pytest.raises(ValueError):
+            call()
+    with torch.no_grad():
+        paged_append(b.store, need(b.k), b.v, table, lens)
+        paged_attention(need(b.q), b.store, table, lens)
+    assert not b.store.k.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", (pc.E4M3, torch.bfloat16))
+def test_pages_behind_32_bits(monkeypatch, cache):
+    """The same pages at the start of a small store and behind 2^32 elements of a large one: equal results."""
+    G, P, D, far = 8, 128, 128, 32768                       # far * G * P * D = 2^32
+    seqs = dict(held=[300, 0, 128, 1000], new=[1, 1, 1, 1])
+    for decode, more in ((True, {}), (False, dict(held=[300, 0, 127, 1000], new=[70, 5, 1, 129]))):
+        b = Batch(**(more or seqs), G=G, R=2, P=P, D=D, dtype=torch.bfloat16, cache=cache, dev="cuda", decode=decode)
+        n, kw = b.store.k.shape[0], turns(1200, 64, "cuda")
+        large = PagedStore.allocate(far + n, G, P, D, "cuda", cache)
+        for name in FIELDS:
+            if getattr(large, name) is not None:
+                getattr(large, name)[far:] = getattr(b.store, name)
+        table = torch.where(b.table < n, b.table + far, b.table)
+        q = paged_append(b.store, b.k, b.v, *b.args, q=b.q, **kw)
+        assert torch.equal(paged_append(large, b.k, b.v, table, *b.args[1:], q=b.q, **kw), q)
+        for name in FIELDS:
+            if getattr(large, name) is not None:
+                raw = lambda t: t.view(torch.uint8)
+                assert torch.equal(raw(getattr(large, name)[far:].contiguous()), raw(getattr(b.store, name)))
+        for way in (False,) if decode else (False, True):
+            monkeypatch.setattr(pc, "gathers", lambda *a: way)
+            assert torch.equal(paged_attention(q, large, table, *b.args[1:]), paged_attention(q, b.store, *b.args))
+        assert not large.k[:far].view(torch.uint8).any() and not large.v[:far].view(torch.uint8).any()
+        del large
+    _common.raise_on_device_error()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(monkeypatch):
+    """Different batches on two streams, both kernels of both ways in flight together: as one after the other."""
+    batches = [Batch(held=[900, 40, 2000], new=[70, 33, 129], G=4, R=3, P=16, D=128, dtype=torch.bfloat16, cache=pc.E4M3, dev="cuda", seed=s) for s in (1, 2)]
+    steps = [Batch(held=[900, 40, 2000, 7], new=[1, 1, 1, 1], G=4, R=3, P=16, D=128, dtype=torch.bfloat16, cache=pc.E4M3, dev="cuda", seed=s, decode=True) for s in (3, 4)]
+    for way in (True, False):
+        monkeypatch.setattr(pc, "gathers", lambda *a: way)
+        want = [[paged_attention(b.q, b.store, *b.args) for b in pair] for pair in (batches, steps)]
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+        for _ in range(5):
+            for pair in (batches, steps):
+                for s, b, g in zip(streams, pair, got):
+                    with torch.cuda.stream(s):
+                        g.append(paged_attention(b.q, b.store, *b.args))
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for j, out in enumerate(got[i]):
+                assert torch.equal(out, want[j % 2][i])
+    _common.raise_on_device_error()

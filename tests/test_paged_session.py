@@ -131,3 +131,11 @@ def test_gpu_generation_in_8_bits_with_drawn_tokens():
     draw = lambda: Q.generate_paged(lm, prompts, 30, SamplingStrategy.drawn(0.8, 50, 0.95), generator=torch.Generator("cuda").manual_seed(5))
     a, b = draw(), draw()
     assert a == b and all(len(r) == 30 for r in a)
+
+
+def test_drawn_rows_with_nothing_to_choose_from():
+    """Such a row's token goes into an embedding all the same: it is an index, the one that the greedy choice gives."""
+    logits = torch.full((3, 40), -float("inf"))
+    logits[1] = float("nan")
+    logits[2, 7] = 0.0
+    assert sample_from_logits(logits, SamplingStrategy.drawn(0.8, 20, 0.9)).tolist() == [0, 0, 7]

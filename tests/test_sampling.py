@@ -181,3 +181,46 @@ def test_refusals_gpu():
     for call in (lambda: sample(x, u.cpu()), lambda: sample(x.double(), u), lambda: sample(x, u, top_p=torch.ones(2)), lambda: sample(torch.zeros(1, MAX_VOCAB + 1, device="cuda"), u[:1])):
         with pytest.raises(ValueError):
             call()
+
+
+def least_temperatures(dev):
+    """Temperatures down to the least number that is none: the largest logits share the draw."""
+    x = torch.tensor([[1.0, 3.0, 3.0, -2.0, math.nextafter(3.0, 0.0)], [0.0, 1e-45, 0.0, -1.0, 1e-45]])
+    for t in (5e-324, 1e-310, 1e-300, 1e-60, torch.tensor([1e-45, 1e-45])):
+        t = t.to(dev) if isinstance(t, torch.Tensor) else t
+        for kw in (dict(), dict(top_k=4), dict(top_p=0.7), dict(min_p=0.5)):
+            # 3.0 stands three times in fp32: thirds; 1e-45 twice, and at its own temperature zeros weigh 1 / e beside it: 0.37, 1.37, 1.74, 2.74
+            for u, want in ((0.2, [1, 1]), (0.7, [4, 4])):
+                assert sample(x.to(dev), torch.tensor([u, u], device=dev), temperature=t, **kw).tolist() == want
+
+
+def test_least_temperatures_cpu():
+    least_temperatures("cpu")
+
+
+@pytest.mark.gpu
+def test_least_temperatures_gpu():
+    least_temperatures("cuda")
+
+
+def test_top_k_is_a_whole_number():
+    for k in (2.0, 2.5, "2"):
+        with pytest.raises(ValueError):
+            sample(torch.zeros(2, 8), torch.zeros(2), top_k=k)
+    assert sample(torch.zeros(2, 8), torch.full((2,), 0.9), top_k=10 ** 12).tolist() == [7, 7]
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    rows = [3 * torch.randn(40, 50304, device="cuda", generator=torch.Generator(device="cuda").manual_seed(s)) for s in (1, 2)]
+    draws = torch.rand(40, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    settings = (dict(top_p=0.9), dict(top_k=50, top_p=0.9), dict(), dict(top_k=2000))
+    want = [[sample(x, draws, **kw) for kw in settings] for x in rows]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for kw in settings:
+        for s, x, g in zip(streams, rows, got):
+            with torch.cuda.stream(s):
+                g.append(sample(x, draws, **kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))

@@ -59,7 +59,8 @@ def sample_from_logits(logits: torch.Tensor, strategy: SamplingStrategy, generat
         return torch.argmax(logits, dim=-1)
     if strategy.kind == "drawn":
         draws = torch.rand(logits.shape[0], device=logits.device, generator=generator)
-        return sample(logits, draws, temperature=strategy.temperature, top_k=strategy.top_k, top_p=strategy.top_p, min_p=strategy.min_p)
+        token = sample(logits, draws, temperature=strategy.temperature, top_k=strategy.top_k, top_p=strategy.top_p, min_p=strategy.min_p)
+        return token.clamp_(min=0)              # a row with nothing to choose from: what the greedy choice gives, and an index that an embedding can take
     if strategy.temperature <= 0.0:
         raise ValueError(f"multinomial sampling requires temperature > 0, got {strategy.temperature}")
     scaled = logits if strategy.temperature == 1.0 else logits * (1.0 / strategy.temperature)

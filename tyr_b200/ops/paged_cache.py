@@ -211,7 +211,7 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     """Writes the new tokens' keys and values ``[rows, kv heads, D]`` into their pages and returns the queries ``[rows, heads, D]`` (when given) as attention takes
     them; rows of no sequence come back as zeros.
 
-    Keys and queries get their RMS norm over the head (with ``k_weight`` / ``q_weight`` [D], ``1 + weight`` with ``one_plus_w``), then channels ``i`` and ``i + half``
+    Keys and queries get their RMS norm over the head (with ``k_weight`` / ``q_weight`` [D] of their type, ``1 + weight`` with ``one_plus_w``), then channels ``i`` and ``i + half``
     are turned by the row's position (``cos``, ``sin`` fp32 [positions, half]), in 32 bits with one rounding at the end.  Operands may be strided views.
 
     e4m3 pages: the scale of a (page, head) is the smallest power of two, 2^-100 at least, that keeps its largest magnitude within 448.  It grows with later tokens of
@@ -240,8 +240,10 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
             raise ValueError(f"paged_append: cos {tuple(size)} and sin {tuple(sin.shape)} do not fit heads of {D}")
         positions, half = size
     for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (D,) or w.get_device() != dev):
-            raise ValueError(f"paged_append: norm weights are [{D}] beside the pages")
+        if w is not None and (w.shape != (D,) or w.dtype != dtype or w.get_device() != dev):
+            raise ValueError(f"paged_append: norm weights are {dtype} [{D}] beside the pages")
+    if (k.requires_grad or v.requires_grad or q is not None and q.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("paged_append: serves inference and has no gradient")
     if dev < 0:
         return _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w)
     number = _on_gpu("paged_append", store, dtype)
@@ -326,6 +328,8 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     if len(shape) != 3 or shape[0] == 0 or shape[2] != D or shape[1] == 0 or shape[1] % G or q.get_device() != store.index:
         raise ValueError(f"paged_attention: queries {tuple(shape)} on {q.device} do not fit pages {store.shape} on {store.k.device}")
     rows, H, _ = shape
+    if q.requires_grad and torch.is_grad_enabled():
+        raise ValueError("paged_attention: serves inference and has no gradient")
     if window is not None and window <= 0:
         raise ValueError(f"paged_attention: the window must be positive, got {window}")
     B, width, table_row = _together("paged_attention", store, rows, table, lengths, starts)

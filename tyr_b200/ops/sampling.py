@@ -80,6 +80,8 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
     if draws.shape != (B,) or draws.dtype not in (torch.float32, torch.float64) or draws.get_device() != dev:
         raise ValueError(f"sample: draws are fp32 or fp64 [{B}] beside the logits")
     top_k = 0 if top_k is None else top_k
+    if not isinstance(top_k, (int, torch.Tensor)):
+        raise ValueError(f"sample: top_k is a whole number, got {top_k}")
     t_at, t = _setting("temperature", temperature, B, dev, torch.float32, 0.0)
     k_at, k = _setting("top_k", top_k, B, dev, torch.int32, 0)
     p_at, p = _setting("top_p", top_p, B, dev, torch.float32, 0.0)
@@ -97,6 +99,6 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
     draws, device = draws.contiguous(), logits.device
     token = torch.empty(B, dtype=torch.int64, device=device)
     packed = _ARGS.pack(logits.data_ptr(), draws.data_ptr(), t_at, p_at, m_at, k_at, token.data_ptr(), row, t, p, m, B, V, 0, draws.dtype == torch.float64,
-                        min(int(k), V), 0)
+                        min(k, V), 0)
     check(lib().tyr_sample(packed, number, cur_stream(device)), "sample")
     return token
