@@ -6,11 +6,13 @@
 // A token is a whole number: what decides it is computed in 64 bits (a relative error of 1e-7 in the sums would move one draw in some thousand over a flat
 // vocabulary).  2^t is the table method of P. T. P. Tang (1989): 2^(k/32) from a table that lies across a warp's lanes, times a polynomial of degree 5 in the rest.
 //
-// A cluster of CTAs holds a row in shared memory: it is read once.  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
+// A cluster of CTAs holds a row in shared memory: it is read once (with many long rows fewer CTAs read it again, from L2).  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
 // decide, by exact sums above, in and below the bin that the counts suggest.  What is left of a bin goes into a list that one CTA sorts; equal logits beyond the list
 // are cut by their indices alone.  What top-k leaves of up to 1024 is listed whole, and one CTA cuts and draws among it, by bins of whole-number weights; for small k
 // the k-th largest of the threads' maxima, which bounds the k-th logit from below, saves the counts over all.  Compiled without fast math.
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -21,7 +23,8 @@ constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048, kSampleList = 1024, kSampleCluster = 16;
 constexpr int kSampleMost = 2048;                                          // of a list that holds all that top-k leaves
 constexpr int kSampleScratch = 3 * kSampleMost * 8;                        // bytes that CTA 0 needs beside it, where its logits were
-constexpr int kSampleSlice = 16384, kSampleLargest = 40960;                // logits of a CTA: with two of them on an SM, and at most
+constexpr int kSampleSlice = 16384, kSampleLargest = 40960;                // logits that a CTA holds: with two of them on an SM, and at most
+constexpr int kSampleRead = 65536;                                         // logits of a CTA that reads them anew for every pass
 
 struct SampleArgs {
   const void* logits;                    // [rows, V], row stride below
@@ -45,9 +48,12 @@ __device__ __forceinline__ uint32_t key_of(float x) {                      // 0:
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ bool stays(uint32_t key, uint32_t index, Place c) { return key > c.key || (key == c.key && index <= c.index); }
 
-__device__ __forceinline__ float load_logit(const float* p) { return *p; }
-__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(__ldg(p)); }
+__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(__ldg(p)); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
@@ -86,7 +92,7 @@ struct SampleShared {
     unsigned long long mass[kSampleBins];
   };
   unsigned long long list[kSampleList], fixed[kSampleList];                // items and their weights
-  double warp_sums[kSampleWarps], cta_sums[kSampleCluster], run_sums[kSampleLargest / kSampleThreads];
+  double warp_sums[kSampleWarps], cta_sums[kSampleCluster], run_sums[kSampleRead / kSampleThreads];
   Partial part[2][kSampleCluster], warp_part[kSampleWarps];
   double warp_above[kSampleWarps];                                         // of a warp's logits above the bin of the cut
   float tops[kSampleCluster], warp_top[kSampleWarps];
@@ -204,7 +210,7 @@ __device__ __forceinline__ void block_sort(unsigned long long* v, int n) {
   __syncthreads();
 }
 
-template <typename T>
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   constexpr int WARPS = kSampleWarps;
   pdl_trigger();
@@ -218,13 +224,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const T* logits = static_cast<const T*>(a.logits) + row * a.row;
   // a CTA's slice and a warp's part of it are consecutive; a lane looks at every 32nd
   const int per_warp = a.slice / WARPS, its = per_warp / 32, base = rank * a.slice + warp * per_warp + lane;
-  float* x = s_logits + warp * per_warp + lane;
   const auto clean = [](float v) { return v == 0.f ? 0.f : (v != v ? -INFINITY : v); };        // -0 is 0, NaN is never chosen
   float top = -INFINITY;
   {
     constexpr int VEC = 16 / sizeof(T);
     const int first = base - lane, here = max(0, min(per_warp, a.V - first));
-    float* part = x - lane;
+    float* part = s_logits + warp * per_warp;
     int done = 0;
     if ((reinterpret_cast<uintptr_t>(logits + first) & 15) == 0) {
       done = here / VEC * VEC;
@@ -235,15 +240,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         *reinterpret_cast<uint4*>(v) = u;
         float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e] = clean(load_logit(v + e)));
+        for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e] = clean(to_float(v[e])));
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(part + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        for (int e = 0; HELD && e < VEC; e += 4) *reinterpret_cast<float4*>(part + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
       }
     }
 #pragma unroll 16
     for (int i = done + lane; i < per_warp; i += 32) {
       const float v = i < here ? clean(load_logit(logits + first + i)) : -INFINITY;
-      part[i] = v;
+      if constexpr (HELD) part[i] = v;
       top = fmaxf(top, v);
     }
     __syncwarp();
@@ -263,11 +268,49 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   cluster.sync();
   for (int i = 0; i < C; ++i) top = fmaxf(top, s.tops[i]);
   const auto index_of = [&](int j) { return static_cast<uint32_t>(base + 32 * j); };
+  const bool infinite = top == INFINITY;                                   // infinite logits share the draw
+  if constexpr (HELD) {
+    if (infinite) {
+#pragma unroll 4
+      for (int j = 0; j < its; ++j) {
+        float& v = s_logits[warp * per_warp + lane + 32 * j];
+        v = v == INFINITY ? 0.f : -INFINITY;
+      }
+    }
+  }
+  // this lane's j-th of a warp's logits; -inf behind them
+  const auto logit_of = [&](int w, int j) {
+    if constexpr (HELD) return j < its ? s_logits[w * per_warp + lane + 32 * j] : -INFINITY;
+    const int i = rank * a.slice + w * per_warp + lane + 32 * j;
+    const float v = j < its && i < a.V ? clean(load_logit(logits + i)) : -INFINITY;
+    return !infinite ? v : v == INFINITY ? 0.f : -INFINITY;
+  };
+  // f(j, logit) for all of them, N loads on their way at a time
+  const auto for_all = [&](auto n, auto f) {
+    constexpr int N = decltype(n)::value;
+    if constexpr (HELD) {
+#pragma unroll N
+      for (int j = 0; j < its; ++j) f(j, s_logits[warp * per_warp + lane + 32 * j]);
+      return;
+    }
+    for (int j0 = 0; j0 < its; j0 += N) {
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = logit_of(warp, j0 + i);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f(j0 + i, v[i]);
+    }
+  };
+  using Four = std::integral_constant<int, 4>;
+  using Eight = std::integral_constant<int, 8>;
 
   if (top == -INFINITY || !(T_row > 0.0)) {                                // nothing to choose from, or the largest: the lowest index that holds it
     uint32_t first = 0xffffffffu;
-    for (int j = its - 1; j >= 0; --j)
-      if (x[32 * j] == top && top > -INFINITY) first = index_of(j);
+    const bool any = top > -INFINITY;
+    if (infinite) top = 0.f;                                               // as for_all gives it
+    for_all(Eight{}, [&](int j, float v) {
+      if (any && v == top) first = min(first, index_of(j));
+    });
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) s.scan[warp] = first;
     __syncthreads();
@@ -282,9 +325,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     return;
   }
-  if (top == INFINITY) {                                                   // infinite logits share the draw
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) x[32 * j] = x[32 * j] == INFINITY ? 0.f : -INFINITY;
+  if (infinite) {
     own_top = own_top == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
   }
@@ -330,16 +371,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   // puts what `take` names into CTA 0's list; its length (beyond the list's end: too many), in every CTA after a cluster.sync()
   const auto gather = [&](auto take, auto near) {                         // `near`: a cheap test that none fails
     SampleShared* lead = cluster.map_shared_rank(&s, 0);
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) {
-      const float v = x[32 * j];
-      if (!near(v)) continue;
+    for_all(Four{}, [&](int j, float v) {
+      if (!near(v)) return;
       const uint32_t key = key_of(v);
       if (key != 0 && take(v, key, index_of(j))) {
         const uint32_t at = atomicAdd(&lead->listed, 1u);
         if (at < kSampleList) lead->list[at] = static_cast<unsigned long long>(key) << 32 | ~index_of(j);
       }
-    }
+    });
     cluster.sync();
     return lead->listed;
   };
@@ -369,25 +408,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       const int own = bin_of(own_top);
       if (own < kSampleBins) atomicAdd(&s.bins[own], 1u);
     } else {
-#pragma unroll 8
-      for (int j = 0; j < its; ++j) {
-        const int b = bin_of(x[32 * j]);
+      for_all(Eight{}, [&](int, float v) {
+        const int b = bin_of(v);
         if (b < kSampleBins) atomicAdd(&s.bins[b], 1u);
-      }
+      });
     }
     merge_bins();
     const int last = bin_reaching(k_row);                                  // none: not that many
     if (tid == 0) s.collected = 0;
     __syncthreads();
     if (last < kSampleBins - 1) {
-#pragma unroll 4
-      for (int j = 0; j < its; ++j) {
-        const float v = x[32 * j];
+      for_all(Eight{}, [&](int j, float v) {
         if (far_of(v) < last + 1) {
           const uint32_t at = atomicAdd(&s.collected, 1u);
           if (at < kSampleList) s.own[at] = static_cast<unsigned long long>(key_of(v)) << 32 | ~index_of(j);
         }
-      }
+      });
     }
     __syncthreads();
     const uint32_t own_n = s.collected;
@@ -570,7 +606,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   float cut_high = 0.f;
   // One cut in the order: by the number of what stays (k), or by its weight (below p times the weight of all that the present cut keeps).
   int cut_bin = -1;                                                        // the bin of values in which a cut by weight over all lies
-  const auto select = [&](bool mass, uint32_t k) {
+  const auto select = [&](bool mass, uint32_t k) __attribute__((always_inline)) {
     const bool whole = cut.key == 1u;                                      // nothing is cut yet
     uint32_t low = 0, high = 0xffffffffu, above_n = 0;
     double above = 0.0, aim = 0.0;
@@ -583,17 +619,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const auto inside = [&](uint32_t key, uint32_t index) { return key != 0 && key >= low && key <= high && stays(key, index, cut); };
     while (true) {
       if (first && whole) {
-#pragma unroll 8
-        for (int j = 0; j < its; ++j) {
-          const int b = bin_of(x[32 * j]);
+        for_all(Eight{}, [&](int, float v) {
+          const int b = bin_of(v);
           if (b < kSampleBins) atomicAdd(&s.bins[b], 1u);
-        }
+        });
       } else {
-#pragma unroll 4
-        for (int j = 0; j < its; ++j) {
-          const uint32_t key = key_of(x[32 * j]);
-          if (inside(key, index_of(j))) atomicAdd(&s.bins[place(x[32 * j], key)], 1u);
-        }
+        for_all(Four{}, [&](int j, float v) {
+          const uint32_t key = key_of(v);
+          if (inside(key, index_of(j))) atomicAdd(&s.bins[place(v, key)], 1u);
+        });
       }
       merge_bins();
       for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
@@ -610,11 +644,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         if (mass && first && whole) {
           if (tid == 0) s.collected = 0;
           __syncthreads();
+          float ahead[4];
+          if constexpr (!HELD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ahead[i] = logit_of(warp, i);
+          }
           for (int j0 = 0; j0 < its; j0 += 4) {                            // four weights hide each other's latency
             float v[4];
             double w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = j0 + i < its ? x[32 * (j0 + i)] : -INFINITY;
+            for (int i = 0; i < 4; ++i) {
+              v[i] = HELD ? logit_of(warp, j0 + i) : ahead[i];
+              if constexpr (!HELD) ahead[i] = logit_of(warp, j0 + 4 + i);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = weigh(v[i]);
             bool hit[4], any = false;
@@ -638,9 +680,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             }
           }
         } else {
-#pragma unroll 4
-          for (int j = 0; j < its; ++j) {
-            const float v = x[32 * j];
+          for_all(Four{}, [&](int j, float v) {
             const uint32_t key = key_of(v);
             const bool is_in = inside(key, index_of(j));
             const int at = is_in ? place(v, key) : 0;
@@ -652,7 +692,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
               }
             }
             if (is_in && at == b) note(key);
-          }
+          });
         }
         q.above = warp_sum_d(q.above), q.in = warp_sum_d(q.in), q.all = warp_sum_d(q.all);
         if (lane == 0) s.warp_above[warp] = q.above;
@@ -819,8 +859,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       const double take = mass ? ceil((aim - above) / w) : static_cast<double>(k - above_n);
       const uint32_t want = take >= in_n ? in_n : take < 1.0 ? 1u : static_cast<uint32_t>(take);
       uint32_t n = 0;
-#pragma unroll 4
-      for (int j = 0; j < its; ++j) n += member(key_of(x[32 * j]), index_of(j)) ? 1u : 0u;
+      for_all(Four{}, [&](int j, float v) { n += member(key_of(v), index_of(j)) ? 1u : 0u; });
       n = __reduce_add_sync(0xffffffffu, n);
       if (lane < C) cluster.map_shared_rank(s.counts, lane)[rank * WARPS + warp] = n;
       cluster.sync();
@@ -828,14 +867,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       for (int i = lane; i < rank * WARPS + warp; i += 32) before += s.counts[i];
       before = __reduce_add_sync(0xffffffffu, before);
       if (before < want && before + n >= want) {
-#pragma unroll 4
-        for (int j = 0; j < its; ++j) {
-          const uint32_t in = __ballot_sync(0xffffffffu, member(key_of(x[32 * j]), index_of(j)));
+        for_all(Four{}, [&](int j, float v) {
+          const uint32_t in = __ballot_sync(0xffffffffu, member(key_of(v), index_of(j)));
           const uint32_t mine = before + __popc(in & ((2u << lane) - 1u));
           if (before < want && before + __popc(in) >= want && (in >> lane & 1) && mine == want)
             for (int r = 0; r < C; ++r) cluster.map_shared_rank(&s, r)->cut = Place{high, index_of(j)};
           before += __popc(in);
-        }
+        });
       }
     }
     cluster.sync();
@@ -850,8 +888,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 
   // ---- the draw ------------------------------------------------------------------------------------------------------------
   const float low_m = m > 0.0 ? static_cast<float>(top + log2(m) / c - 1e-6 * (fabs(top) + fabs(log2(m) / c))) : -INFINITY;      // no weight below it reaches min_p
-  const auto weight_of = [&](int j) {
-    const float v = x[32 * j];
+  const auto weight_of = [&](int j, float v) {
     const uint32_t key = key_of(v);
     const bool in = key != 0 && v >= low_m && stays(key, index_of(j), cut);
     if (!__any_sync(0xffffffffu, in)) return 0.0;
@@ -860,8 +897,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   };
   double sum = 0.0;
   if (cut.key == 1u && m <= 0.0) {
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) sum += weigh(x[32 * j]);
+    for_all(std::integral_constant<int, HELD ? 4 : 8>{}, [&](int, float v) { sum += weigh(v); });
     sum = warp_sum_d(sum);
     if (sum < 1e-200) sum = 0.0;                                           // nothing but what is never chosen
   } else if (cut_bin >= 0 && m <= 0.0) {
@@ -879,8 +915,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     __syncthreads();
     sum = s.warp_above[warp] + static_cast<double>(s.fixed[warp]) / unit;
   } else {
-#pragma unroll 4
-    for (int j = 0; j < its; ++j) sum += weight_of(j);
+    for_all(Four{}, [&](int j, float v) { sum += weight_of(j, v); });
     sum = warp_sum_d(sum);
   }
   // the CTA in which the cumulative weight passes the aim, else the last that holds any; then the warp in it, then the run of 32
@@ -906,10 +941,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (passing(cta, 0.0, aim, before) != rank) return;
   const int at_warp = passing(lane < WARPS ? s.warp_sums[lane] : 0.0, before, aim, before);
   // all warps weigh that warp's logits, each its runs
-  const float* part = s_logits + at_warp * per_warp + lane;
   const uint32_t part_index = rank * a.slice + at_warp * per_warp + lane;
   const auto weight_at = [&](int j) {
-    const float v = part[32 * j];
+    const float v = logit_of(at_warp, j);
     const uint32_t key = key_of(v);
     const double w = weigh(v);
     return key != 0 && stays(key, part_index + 32 * j, cut) && w >= m ? w : 0.0;
@@ -939,22 +973,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (lane == at) a.token[row] = part_index + 32 * last_run;
 }
 
-template <typename T>
-int sample_form(SampleArgs a, cudaStream_t stream) {
+template <typename T, bool HELD>
+int sample_form(const SampleArgs& a, int ctas, cudaStream_t stream) {
   static const cudaError_t ready = [] {
-    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleLargest * 4);
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleLargest * 4);
   }();
   if (ready != cudaSuccess) return static_cast<int>(ready);
-  // the fewest CTAs a row that leave room for two on an SM; more while there are few rows
-  int ctas = 1;
-  while (ctas < kSampleCluster && (static_cast<long long>(ctas) * kSampleSlice < a.V || (a.rows * ctas * 2 <= 148 && ctas * kSampleThreads * 4 < a.V))) ctas *= 2;
-  if (static_cast<long long>(ctas) * kSampleLargest < a.V) return -2;
-  a.slice = (a.V + ctas * kSampleThreads - 1) / (ctas * kSampleThreads) * kSampleThreads;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = a.slice * 4 > kSampleScratch ? a.slice * 4 : kSampleScratch;
+  cfg.dynamicSmemBytes = HELD && a.slice * 4 > kSampleScratch ? a.slice * 4 : kSampleScratch;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -964,7 +993,23 @@ int sample_form(SampleArgs a, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, sample_kernel<T, HELD>, a));
+}
+
+template <typename T>
+int sample_any(SampleArgs a, cudaStream_t stream) {
+  // the fewest CTAs a row that leave room for two on an SM; more while there are few rows
+  int ctas = 1;
+  while (ctas < kSampleCluster && (static_cast<long long>(ctas) * kSampleSlice < a.V || (a.rows * ctas * 2 <= 148 && ctas * kSampleThreads * 4 < a.V))) ctas *= 2;
+  if (static_cast<long long>(ctas) * kSampleLargest < a.V) return -2;
+  const int held = ctas;
+  // Where that would take three rounds and more, fewer CTAs a row that read it anew for every pass: fewer steps in which they wait for one another.  In us, held /
+  // read, fp32: 128 x 262144 by top-p 401 / 324, by top-k 133 / 93, no filter 120 / 109; 256 x 50304 157 / 142, 70 / 43, 50 / 43.  At two rounds it takes longer:
+  // 33 x 248320 in bf16, no filter 33 / 36, settings of all kinds 65 / 81.
+  if (static_cast<long long>(a.rows) * ctas > 3 * 296)
+    while (ctas > 1 && static_cast<long long>(a.rows) * ctas > 296 && static_cast<long long>(ctas / 2) * kSampleRead >= a.V) ctas /= 2;
+  a.slice = (a.V + ctas * kSampleThreads - 1) / (ctas * kSampleThreads) * kSampleThreads;
+  return ctas == held ? sample_form<T, true>(a, ctas, stream) : sample_form<T, false>(a, ctas, stream);
 }
 
 }  // namespace tyr
@@ -976,9 +1021,9 @@ extern "C" TYR_EXPORT int tyr_sample(const void* packed, int dtype, void* stream
   const SampleArgs& a = *static_cast<const SampleArgs*>(packed);
   if (a.rows <= 0 || a.V <= 0 || a.rows > (1 << 26)) return -1;
   switch (dtype) {
-    case 0: return sample_form<__nv_bfloat16>(a, (cudaStream_t)stream);
-    case 1: return sample_form<__half>(a, (cudaStream_t)stream);
-    case 2: return sample_form<float>(a, (cudaStream_t)stream);
+    case 0: return sample_any<__nv_bfloat16>(a, (cudaStream_t)stream);
+    case 1: return sample_any<__half>(a, (cudaStream_t)stream);
+    case 2: return sample_any<float>(a, (cudaStream_t)stream);
   }
   return -3;
 }

@@ -224,3 +224,19 @@ def test_two_streams_at_once():
                 g.append(sample(x, draws, **kw))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, V, dtype", ((300, 20011, torch.float32), (230, 50304, torch.bfloat16), (70, 262144, torch.float16)))
+def test_many_long_rows(B, V, dtype):
+    """Rows that are read anew for every pass, against few at a time, which are held: the same tokens, odd rows among them."""
+    gen = torch.Generator().manual_seed(V)
+    x = (2 * torch.randn(B, V + 1, generator=gen)).to(dtype)[:, 1:]
+    x[0], x[1, 5:], x[2, ::2], x[3, 7], x[4, V - 1] = -math.inf, -math.inf, math.nan, math.inf, math.inf
+    x[4, 3], x[5], x[6, :V // 2] = math.inf, 0.25, -math.inf
+    x, draws = x.cuda(), torch.rand(B, generator=gen).cuda()
+    for kw in (dict(), dict(temperature=0.0), dict(top_p=0.9), dict(top_k=40, top_p=0.9), dict(top_k=1500), dict(top_k=3001, top_p=0.8), dict(min_p=0.02), dict(temperature=0.01, top_p=0.5)):
+        got = sample(x, draws, **kw)
+        held = torch.cat([sample(x[i:i + 10], draws[i:i + 10], **kw) for i in range(0, B, 10)])
+        # cuts and draws within a rounding of the sums may fall otherwise: a part in 10^12 of the draws
+        assert torch.equal(got, held)
