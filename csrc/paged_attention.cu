@@ -22,6 +22,11 @@
 //
 // Work is cut into equal shares of tiles, one for each resident CTA, whatever the lengths: a share may begin and end inside a (sequence, head).  Such pieces go to
 // a workspace of the call, and a second launch joins them in the order of the keys.
+//
+// Measured, e4m3: 32 sequences of some 16 000 tokens, 48 query heads over 8 of 128: 137 us and 7 for the join, 5.7 TB/s, while it streams 93 % of what a copy moves.
+// 32 of some 2000, 24 heads over 4 of 256: 31.6 us, of which 4 pass before the first keys arrive (the shares are found from the lengths) and 5 in the join; two CTAs
+// of five warps are what 168 registers leave room for.  One of 500: 8.6 us and 4.6.  The join is a launch of its own: the last CTA to
+// end would need a counter that each call clears, and two replayed graphs would share it.
 #include <type_traits>
 
 #include "common.cuh"

@@ -7,7 +7,7 @@ executables: Qwen3, Qwen2.5-Omni thinker, Qwen3.5 / 3.6, Gemma 4, Zatorax, Kinet
     python -m tyr_b200.cli.model_runner --family whisper --source openai/whisper-small --audio speech.wav
 
 Common flags: ``--family`` (default ``auto``: by config.json, ``models/registry.py``), ``--source`` (directory or hub repo id), ``--prompt`` / ``--prompt-file``, ``--batch-size``, ``--max-new-tokens``,
-``--stream``, ``--device`` (auto | cpu | cuda | cuda:N, falling back to CPU with a warning), ``--bench``.
+``--cache`` (Qwen3 and the Qwen2.5-Omni thinker: ``dense``; ``paged`` or, in 8 bits, ``paged8``: prompts of any lengths without padding), ``--min-p``, ``--stream``, ``--device`` (auto | cpu | cuda | cuda:N, falling back to CPU with a warning), ``--bench``.
 """
 from __future__ import annotations
 
