@@ -6,14 +6,14 @@
 // A token is a whole number: what decides it is computed in 64 bits (a relative error of 1e-7 in the sums would move one draw in some thousand over a flat
 // vocabulary).  2^t is the table method of P. T. P. Tang (1989): 2^(k/32) from a table that lies across a warp's lanes, times a polynomial of degree 5 in the rest.
 //
-// A cluster of CTAs holds a row in shared memory: it is read once (with many long rows fewer CTAs read it again, from L2).  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
+// A cluster of CTAs holds a row in shared memory: it is read once (with many long rows fewer CTAs read it again, from L2, four logits a lane: one a lane took 363 us for 280).  Every cut is a place in the one order (key, index), found by counts over 2048 bins and, where weights
 // decide, by exact sums above, in and below the bin that the counts suggest.  What is left of a bin goes into a list that one CTA sorts; equal logits beyond the list
 // are cut by their indices alone.  What top-k leaves of up to 1024 is listed whole, and one CTA cuts and draws among it, by bins of whole-number weights; for small k
 // the k-th largest of the threads' maxima, which bounds the k-th logit from below, saves the counts over all.  Compiled without fast math.
 //
 // Bound: neither memory nor arithmetic but the chain of some ten steps in which a row's CTAs wait for one another, and by mass the counts (atomics in shared memory,
 // 5 us for 16384 logits) and the weights in 64 bits (8 to 11 us; the units for 64 bits are half busy).  1 row of 151936, top-k 50 and top-p: 12 us, 9 of
-// them the host's; 33 rows of 248320 in bf16, settings of all kinds: 55; 256 of 50304 in fp32, no filter: 47; 128 of 262144 by mass: 360.
+// them the host's; 33 rows of 248320 in bf16, settings of all kinds: 55; 256 of 50304 in fp32, no filter: 39; 128 of 262144 by mass: 280.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -271,7 +271,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   for (int i = tid; i < kSampleBins; i += kSampleThreads) s.bins[i] = 0;
   cluster.sync();
   for (int i = 0; i < C; ++i) top = fmaxf(top, s.tops[i]);
-  const auto index_of = [&](int j) { return static_cast<uint32_t>(base + 32 * j); };
+  // rows that are read again are, where they are aligned, read by runs of four a lane
+  const bool runs = !HELD && (reinterpret_cast<uintptr_t>(logits) & (4 * sizeof(T) - 1)) == 0;
+  const auto index_of = [&](int j) { return static_cast<uint32_t>(runs ? base + 3 * lane + (j >> 2) * 128 + (j & 3) : base + 32 * j); };
   const bool infinite = top == INFINITY;                                   // infinite logits share the draw
   if constexpr (HELD) {
     if (infinite) {
@@ -289,7 +291,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const float v = j < its && i < a.V ? clean(load_logit(logits + i)) : -INFINITY;
     return !infinite ? v : v == INFINITY ? 0.f : -INFINITY;
   };
-  // f(j, logit) for all of them, N loads on their way at a time
+  // this lane's logits j0 .. j0 + 3 of its warp's, j0 a multiple of four, as index_of counts them
+  const auto fetch = [&](int j0, float (&v)[4]) {
+    const int at = static_cast<int>(index_of(j0));
+    if (runs && j0 < its && at + 4 <= a.V) {
+      T four[4];
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(four) = __ldg(reinterpret_cast<const uint4*>(logits + at));
+      else *reinterpret_cast<uint2*>(four) = __ldg(reinterpret_cast<const uint2*>(logits + at));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_float(four[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = j0 < its && static_cast<int>(index_of(j0 + i)) < a.V ? load_logit(logits + index_of(j0 + i)) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = clean(v[i]);
+      if (infinite) v[i] = v[i] == INFINITY ? 0.f : -INFINITY;
+    }
+  };
+  // f(j, logit) for all of them, N on their way at a time
   const auto for_all = [&](auto n, auto f) {
     constexpr int N = decltype(n)::value;
     if constexpr (HELD) {
@@ -297,11 +318,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       for (int j = 0; j < its; ++j) f(j, s_logits[warp * per_warp + lane + 32 * j]);
     } else {
       for (int j0 = 0; j0 < its; j0 += N) {
-        float v[N];
+        float v[N / 4][4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = logit_of(warp, j0 + i);
+        for (int i = 0; i < N / 4; ++i) fetch(j0 + 4 * i, v[i]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f(j0 + i, v[i]);
+        for (int i = 0; i < N; ++i) f(j0 + i, v[i >> 2][i & 3]);
       }
     }
   };
@@ -649,18 +670,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
           if (tid == 0) s.collected = 0;
           __syncthreads();
           float ahead[4];
-          if constexpr (!HELD) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ahead[i] = logit_of(warp, i);
-          }
+          if constexpr (!HELD) fetch(0, ahead);
           for (int j0 = 0; j0 < its; j0 += 4) {                            // four weights hide each other's latency
             float v[4];
             double w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[i] = HELD ? logit_of(warp, j0 + i) : ahead[i];
-              if constexpr (!HELD) ahead[i] = logit_of(warp, j0 + 4 + i);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = HELD ? logit_of(warp, j0 + i) : ahead[i];
+            if constexpr (!HELD) fetch(j0 + 4, ahead);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = weigh(v[i]);
             bool hit[4], any = false;
@@ -873,13 +889,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       for (int i = lane; i < rank * WARPS + warp; i += 32) before += s.counts[i];
       before = __reduce_add_sync(0xffffffffu, before);
       if (before < want && before + n >= want) {
-        for_all(Four{}, [&](int j, float v) {
-          const uint32_t in = __ballot_sync(0xffffffffu, member(key_of(v), index_of(j)));
+#pragma unroll 4
+        for (int j = 0; j < its; ++j) {                                    // in vocabulary order
+          const uint32_t index = base + 32 * j, in = __ballot_sync(0xffffffffu, member(key_of(logit_of(warp, j)), index));
           const uint32_t mine = before + __popc(in & ((2u << lane) - 1u));
           if (before < want && before + __popc(in) >= want && (in >> lane & 1) && mine == want)
-            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&s, r)->cut = Place{high, index_of(j)};
+            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&s, r)->cut = Place{high, index};
           before += __popc(in);
-        });
+        }
       }
     }
     cluster.sync();
@@ -1010,11 +1027,12 @@ int sample_any(SampleArgs a, cudaStream_t stream) {
   if (static_cast<long long>(ctas) * kSampleLargest < a.V) return -2;
   const int held = ctas;
   // Where that would take three rounds and more, fewer CTAs a row that read it anew for every pass: fewer steps in which they wait for one another.  In us, held /
-  // read, fp32: 128 x 262144 by top-p 401 / 324, by top-k 133 / 93, no filter 120 / 109; 256 x 50304 157 / 142, 70 / 43, 50 / 43.  At two rounds it takes longer:
-  // 33 x 248320 in bf16, no filter 33 / 36, settings of all kinds 65 / 81.
+  // read, fp32: 128 x 262144 by top-p 401 / 262, by top-k 133 / 74, no filter 120 / 91; 256 x 50304 157 / 93, 70 / 33, 50 / 37.  With less it depends: 48 x 248320 in
+  // bf16, 2.6 rounds, by top-p 152 / 125, no filter 42 / 50, settings of all kinds 88 / 116, since a row that is cut by mass holds up all.
   if (static_cast<long long>(a.rows) * ctas > 3 * 296)
     while (ctas > 1 && static_cast<long long>(a.rows) * ctas > 296 && static_cast<long long>(ctas / 2) * kSampleRead >= a.V) ctas /= 2;
-  a.slice = (a.V + ctas * kSampleThreads - 1) / (ctas * kSampleThreads) * kSampleThreads;
+  const int step = ctas * kSampleThreads * (ctas == held ? 1 : 4);          // whole runs of four where rows are read again
+  a.slice = (a.V + step - 1) / step * step / ctas;
   return ctas == held ? sample_form<T, true>(a, ctas, stream) : sample_form<T, false>(a, ctas, stream);
 }
 
