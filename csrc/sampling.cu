@@ -394,10 +394,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return s.found;
   };
   // puts what `take` names into CTA 0's list; its length (beyond the list's end: too many), in every CTA after a cluster.sync()
-  const auto gather = [&](auto take, auto near) {                         // `near`: a cheap test that none fails
+  const auto gather = [&](auto take) {
     SampleShared* lead = cluster.map_shared_rank(&s, 0);
     for_all(Four{}, [&](int j, float v) {
-      if (!near(v)) return;
       const uint32_t key = key_of(v);
       if (key != 0 && take(v, key, index_of(j))) {
         const uint32_t at = atomicAdd(&lead->listed, 1u);
@@ -843,7 +842,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         cut = Place{static_cast<uint32_t>(last >> 32), ~static_cast<uint32_t>(last)};
         return;
       }
-      const uint32_t n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); }, [](float) { return true; });
+      const uint32_t n = gather([&](float, uint32_t key, uint32_t index) { return member(key, index); });
       if (rank == 0) {
         sort_list(n);
         int last;                                                          // the last of the list that stays
