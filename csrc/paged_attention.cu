@@ -57,17 +57,25 @@ struct PartHead { int row, heads, used, last, slot, pad[3]; };      // a (sequen
 
 struct Seq { int row, n, len, tile0, tiles, row_tiles; };
 
+// Rows row .. end - 1 that sequence b brings, and whether they go together with its length, the table and the call.
+struct Rows { int row, end, len; bool fits; };
+__device__ __forceinline__ Rows rows_of(const PagedAttnArgs& a, int b) {
+  Rows r;
+  r.len = a.lengths[b];
+  r.row = a.starts ? a.starts[b] : b;
+  r.end = a.starts ? a.starts[b + 1] : b + (r.len > 0 ? 1 : 0);
+  r.fits = r.row == r.end || (r.row >= 0 && r.row < r.end && r.end <= a.rows && r.len >= r.end - r.row && (r.len - 1) >> (31 - __clz(a.P)) < a.width);
+  return r;
+}
 // Rows, keys and tiles of sequence b; none where the operands do not go together (recorded).
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   Seq s;
-  s.len = a.lengths[b];
-  s.row = a.starts ? a.starts[b] : b;
-  s.n = a.starts ? a.starts[b + 1] - s.row : (s.len > 0 ? 1 : 0);
-  if (s.n != 0 && (s.n < 0 || s.row < 0 || s.row + s.n > a.rows || s.len < s.n || (s.len - 1) >> (31 - __clz(a.P)) >= a.width)) {
-    report_error(a.err, ERR_BOUNDS, b);
-    s.n = 0;
-  }
+  const Rows r = rows_of(a, b);
+  s.len = r.len;
+  s.row = r.row;
+  s.n = r.fits ? r.end - r.row : 0;
+  if (!r.fits) report_error(a.err, ERR_BOUNDS, b);
   const int first = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
   s.tile0 = first / KEYS;
   s.tiles = s.n == 0 ? 0 : (s.len + KEYS - 1) / KEYS - s.tile0;
@@ -362,12 +370,18 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   for (int c = 0; c < PIECES_BOX; ++c) k_at[c] = TL::at(0, pi, t + 4 * c);
 #pragma unroll
   for (int i = 0; i < 2; ++i) v_at[i] = F8 && D == 64 ? TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g >> 1) + (g & 1) * 8 : TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g);
-  // rows of no sequence
-  for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps) {
-    const bool none = a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0;
-    if (none)
-      for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * D + i) = make_uint4(0u, 0u, 0u, 0u);
-  }
+  // rows of no sequence, and of those whose operands do not go together
+  const auto clear = [&](int row) {
+    for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * D + i) = make_uint4(0u, 0u, 0u, 0u);
+  };
+  for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps)
+    if (a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0 || !rows_of(a, row).fits) clear(row);
+  if (a.starts)
+    for (int b = blockIdx.x * kWarps + warp; b < a.B; b += gridDim.x * kWarps) {
+      const Rows r = rows_of(a, b);
+      if (!r.fits)
+        for (int row = max(r.row, 0); row < min(r.end, a.rows); ++row) clear(row);
+    }
   PartHead head{0, 0, 0, -1, 0, {0, 0, 0}};
   if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
   bool first_piece = true, lost = false;
@@ -827,15 +841,22 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
 
 // The pages of every sequence as the ragged form of the attention kernel on tcgen05 (csrc/attention_fwd.cu) takes them: keys and values [B, G, capacity, D] in the
 // queries' type, zeros behind the end up to a multiple of 128.  A (sequence, head) is one blockIdx.(z, y).  The codes of a page whose
-// scales are no numbers give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence are zeroed on the way.
+// scales are no numbers give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence, or of one whose operands do not go together, are zeroed on the way.
 template <typename T, bool F8>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedAttnArgs a, void* k_out, void* v_out, long long capacity) {
   pdl_entry();
   const int b = blockIdx.z, head = blockIdx.y, lanes = a.D / 8, lane = threadIdx.x % lanes, per = 256 / lanes;
-  if (b == 0 && head == 0)
-    for (int row = blockIdx.x; row < a.rows; row += gridDim.x)
-      if (row < a.starts[0] || row >= a.starts[a.B])
-        for (int i = threadIdx.x * 8; i < a.H * a.D; i += 2048) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * a.D + i) = make_uint4(0u, 0u, 0u, 0u);
+  if (head == 0) {
+    const auto clear = [&](int row) {
+      for (int i = threadIdx.x * 8; i < a.H * a.D; i += 2048) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * a.D + i) = make_uint4(0u, 0u, 0u, 0u);
+    };
+    if (b == 0)
+      for (int row = blockIdx.x; row < a.rows; row += gridDim.x)
+        if (row < a.starts[0] || row >= a.starts[a.B]) clear(row);
+    const Rows r = rows_of(a, b);
+    if (!r.fits)
+      for (int row = max(r.row, 0) + blockIdx.x; row < min(r.end, a.rows); row += gridDim.x) clear(row);
+  }
   const Seq s = seq_of<16, 128>(a, b);
   if (s.n == 0) return;
   const int end = min(static_cast<long long>((s.len + 127) / 128 * 128), capacity), page_bits = 31 - __clz(a.P);

@@ -702,3 +702,32 @@ def test_two_streams_at_once(monkeypatch):
             for j, out in enumerate(got[i]):
                 assert torch.equal(out, want[j % 2][i])
     _common.raise_on_device_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ("step", False, True))
+def test_rows_of_refused_sequences_are_zeros(monkeypatch, way):
+    """A length beyond the table, more rows than tokens, rows outside the call's: recorded, zeros in the result, and the other sequences as without them."""
+    monkeypatch.setattr(pc, "gathers", lambda *a: way is True)
+    step = way == "step"
+    b = Batch(held=[70, 300, 20], new=[1, 1, 1] if step else [40, 3, 60], G=2, R=2, P=16, D=64, dtype=torch.bfloat16, cache=torch.bfloat16, dev="cuda", decode=step, strided=False)
+    table, lens, starts = b.args
+    want = paged_attention(b.q, b.store, *b.args)
+    long, few, first, last = lens.clone(), lens.clone(), None, None
+    long[1] = 10 ** 6
+    few[1] = 2
+    cases = [(long, starts, 1)]
+    if not step:
+        first, last = starts.clone(), starts.clone()
+        first[0], last[-1] = -1, 1000
+        cases += [(few, starts, 1), (lens, first, 0), (lens, last, 2)]
+    for n, s, bad in cases:
+        for _ in range(3):
+            torch.full_like(want, math.nan)                    # what the allocator hands out next
+        out = paged_attention(b.q, b.store, table, n, s)
+        rows = slice(bad, bad + 1) if step else slice(b.starts[bad], b.starts[bad + 1])
+        with pytest.raises(RuntimeError):
+            _common.raise_on_device_error()
+        assert not out[rows].any()
+        out[rows] = want[rows]
+        assert torch.equal(out, want)

@@ -322,7 +322,7 @@ def _attend_ref(q, store, table, lengths, starts, window, scale):
 def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
                     window: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
     """Attention of the new tokens' queries ``[rows, heads, D]`` over their sequences' pages, which hold the new tokens already -> ``[rows, heads, D]``; rows of no
-    sequence come back as zeros.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
+    sequence, and of one that is left out, come back as zeros.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
     pages, G, P, D = store.shape
     shape = q.shape
     if len(shape) != 3 or shape[0] == 0 or shape[2] != D or shape[1] == 0 or shape[1] % G or q.get_device() != store.index:
