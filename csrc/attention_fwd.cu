@@ -82,7 +82,7 @@ struct AttnParams {
   int back_half;
   // ragged form only
   const int *starts, *lengths;   // [B + 1], [B]
-  int rows;           // of the queries
+  int rows;           // of the queries; `keep`: the most tokens that a sequence may have
 };
 
 constexpr int ATT_TBL_PAD = 256;       // table entries below distance 0 and past the window that boundary blocks can touch
@@ -782,10 +782,10 @@ extern "C" TYR_EXPORT int tyr_flash_fwd_kept(const void* q, const void* k, const
   return flash_fwd_launch(q, k, v, o, nullptr, B, Hq, Hkv, T, T, dk, dv, strides, 1, window, 0, scale, nullptr, nullptr, err, stream, &ex);
 }
 
-// Attention of ragged rows q [rows, Hq, D] (strides of rows and heads) over the keys and values [B, Hkv, capacity, D] of their sequences (see the kernel's head);
-// out [rows, Hq, D].  dtype: 0 = bf16, 1 = fp16.  D: 64 or 128.
+// Attention of ragged rows q [rows, Hq, D] (strides of rows and heads) over the keys and values [B, Hkv, capacity, D] of their sequences (see the kernel's head), of
+// which `longest` tokens may be there: a sequence of more has none that were brought; out [rows, Hq, D].  dtype: 0 = bf16, 1 = fp16.  D: 64 or 128.
 int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
-                         int Hq, int Hkv, int D, long long capacity, int window, float scale, int dtype, int* err, cudaStream_t stream) {
+                         int Hq, int Hkv, int D, long long capacity, int longest, int window, float scale, int dtype, int* err, cudaStream_t stream) {
   const long long st[6] = {0, q_row, q_head, Hkv * capacity * D, D, capacity * D};
   CUtensorMap tq, tk, tv;
   int r;
@@ -807,7 +807,7 @@ int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const
   p.scale_log2 = scale * 1.4426950408889634f;
   p.O = static_cast<__nv_bfloat16*>(out); p.o_row_stride = static_cast<long long>(Hq) * D; p.o_head_stride = D;
   p.err = err; p.k_steps = D / 16; p.dv = D; p.starts = starts; p.lengths = lengths; p.rows = rows;
-  p.keep = static_cast<int>(capacity);
+  p.keep = longest;
   const long long blocks = (static_cast<long long>(rows) / (2 * ATT_BM) + B) * Hq;
   if (blocks > 0x7fffffff) return -5;
   const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), dim3(640), kSmem, stream, tq, tk, tv, p);

@@ -994,7 +994,7 @@ int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool 
 }  // namespace tyr
 
 int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
-                         int Hq, int Hkv, int D, long long capacity, int window, float scale, int dtype, int* err, cudaStream_t stream);
+                         int Hq, int Hkv, int D, long long capacity, int longest, int window, float scale, int dtype, int* err, cudaStream_t stream);
 
 using namespace tyr;
 
@@ -1014,7 +1014,7 @@ extern "C" TYR_EXPORT int tyr_paged_attention_gathered(const void* packed, int d
                                  : (f8 ? paged_gather_kernel<__half, true> : paged_gather_kernel<__half, false>);
   const cudaError_t e = launch_dependent(gather, grid, dim3(256), 0, (cudaStream_t)stream, a, k, v, capacity);
   if (e != cudaSuccess) return static_cast<int>(e);
-  return tyr_flash_fwd_ragged(a.q, a.q_row, a.q_head, k, v, a.out, a.starts, a.lengths, a.rows, a.B, a.H, a.G, a.D, capacity, a.window, a.scale, dtype, a.err, (cudaStream_t)stream);
+  return tyr_flash_fwd_ragged(a.q, a.q_row, a.q_head, k, v, a.out, a.starts, a.lengths, a.rows, a.B, a.H, a.G, a.D, capacity, a.width * a.P, a.window, a.scale, dtype, a.err, (cudaStream_t)stream);
 }
 
 // dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows of a tile: 16, or 128 (64 of heads of 256).

@@ -731,3 +731,22 @@ def test_rows_of_refused_sequences_are_zeros(monkeypatch, way):
         assert not out[rows].any()
         out[rows] = want[rows]
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", (False, True))
+def test_a_length_just_beyond_the_table(monkeypatch, way):
+    """Three pages of 16 hold 48 tokens, the laid out tile of keys 128: a length between them is refused like any other."""
+    monkeypatch.setattr(pc, "gathers", lambda *a: way)
+    b = Batch(held=[20, 8, 30], new=[10, 20, 1], G=2, R=2, P=16, D=64, dtype=torch.bfloat16, cache=torch.bfloat16, dev="cuda", strided=False)
+    assert b.table.shape[1] == 3
+    want = paged_attention(b.q, b.store, *b.args)
+    for n in (49, 100, 128):
+        lens = b.args[1].clone()
+        lens[1] = n
+        out = paged_attention(b.q, b.store, b.table, lens, b.args[2])
+        with pytest.raises(RuntimeError):
+            _common.raise_on_device_error()
+        assert not out[10:30].any()
+        out[10:30] = want[10:30]
+        assert torch.equal(out, want)
