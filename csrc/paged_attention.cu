@@ -326,11 +326,14 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
           batch = p0 >> 5;
           const int p = batch * 32 + lane;
           id = p <= last_page ? table[p] : 0;
-          if (id < 0 || id >= a.pages) {
+          scale = make_float2(1.f, 0.f);
+          if (id < 0 || id >= a.pages) {                                    // outside the cache: nothing is read, and the keys are no numbers
             report_error(a.err, ERR_BOUNDS, id);
-            id = 0;
+            id = -1;
+            scale.x = __uint_as_float(0x7fffffffu);
+          } else if (F8) {
+            scale = make_float2(a.k_scale[static_cast<long long>(id) * a.G + sh.head], log2f(a.v_scale[static_cast<long long>(id) * a.G + sh.head]));
           }
-          if (F8) scale = make_float2(a.k_scale[static_cast<long long>(id) * a.G + sh.head], log2f(a.v_scale[static_cast<long long>(id) * a.G + sh.head]));
         }
         const int n = min(per_tile, last_page - p0 + 1), from = (p0 & 31) + lane;
         const int page = __shfl_sync(0xffffffffu, id, from & 31);
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         __syncwarp();
         if (lane < n) {
           uint8_t* dst = smem + stage * 2 * TL::kSize + lane * page_rows * TL::kRow;
-          const int row = (tile * KEYS) & (a.P - 1), z = page * a.G + sh.head;
+          const int row = (tile * KEYS) & (a.P - 1), z = page < 0 ? -1 : page * a.G + sh.head;      // -1: what the map fills in
           if (TL::kBoxes == 1 || per_tile == 1) {                           // all columns at once: they lie as the tile has them
             tma_load_4d(dst, &map_k, full + stage, 0, row, 0, z);
             tma_load_4d(dst + TL::kSize, &map_v, full + stage, 0, row, 0, z);
@@ -840,8 +843,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
 }
 
 // The pages of every sequence as the ragged form of the attention kernel on tcgen05 (csrc/attention_fwd.cu) takes them: keys and values [B, G, capacity, D] in the
-// queries' type, zeros behind the end up to a multiple of 128.  A (sequence, head) is one blockIdx.(z, y).  The codes of a page whose
-// scales are no numbers give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence, or of one whose operands do not go together, are zeroed on the way.
+// queries' type, zeros behind the end up to a multiple of 128.  A (sequence, head) is one blockIdx.(z, y).  A page outside the cache,
+// and the codes of one whose scales are no numbers, give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence, or of one whose operands do not go together, are zeroed on the way.
 template <typename T, bool F8>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedAttnArgs a, void* k_out, void* v_out, long long capacity) {
   pdl_entry();
@@ -869,10 +872,11 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
       const int token = token0 + i * per + threadIdx.x / lanes;
       from[i] = -1;
       if (token >= s.len) continue;
-      int page = a.table[b * a.table_row + (token >> page_bits)];
-      if (page < 0 || page >= a.pages) {
+      const int page = a.table[b * a.table_row + (token >> page_bits)];
+      if (page < 0 || page >= a.pages) {                                    // outside the cache: nothing is read
         report_error(a.err, ERR_BOUNDS, page);
-        page = 0;
+        from[i] = -2;
+        continue;
       }
       const long long at = static_cast<long long>(page) * a.G + head;
       from[i] = (at * a.P + (token & (a.P - 1))) * a.D + lane * 8;
@@ -894,8 +898,8 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
       const long long to = ((static_cast<long long>(b) * a.G + head) * capacity + token) * a.D + lane * 8;
       uint4 x, y;
       if constexpr (F8) {
-        const bool none = from[i] < 0, lost = !none && vs[i] != vs[i];
-        const float kf = none ? 0.f : lost ? vs[i] : ks[i], vf = none || lost ? 0.f : vs[i];
+        const bool none = from[i] < 0, lost = from[i] == -2 || (!none && vs[i] != vs[i]);
+        const float kf = lost ? __uint_as_float(0x7fffffffu) : none ? 0.f : ks[i], vf = none || lost ? 0.f : vs[i];
         const auto two = [](uint32_t codes, float scale) {
           const float2 f = Num<__half>::two(halves_of_codes(codes));
           return Num<T>::pack(f.x * scale, f.y * scale);
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
         x = make_uint4(two(k[i].x, kf), two(k[i].x >> 16, kf), two(k[i].y, kf), two(k[i].y >> 16, kf));
         y = make_uint4(two(v[i].x, vf), two(v[i].x >> 16, vf), two(v[i].y, vf), two(v[i].y >> 16, vf));
       } else {
-        x = k[i];
+        x = from[i] == -2 ? make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu) : k[i];
         y = v[i];
       }
       *reinterpret_cast<uint4*>(static_cast<T*>(k_out) + to) = x;
@@ -915,9 +919,10 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
 typedef CUresult (*PagedEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Pages as the tiles want them: boxes of min(P, KEYS) tokens of one page and head, in columns of 128 bytes (a whole row where it is shorter).
-template <bool F8, int D, int KEYS>
-int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
+// Pages as the tiles want them: boxes of min(P, KEYS) tokens of one page and head, in columns of 128 bytes (a whole row where it is shorter).  A page outside the cache
+// comes as zeros; keys in 16 bits as NaN (those in 8 have a scale for that).
+template <typename T, bool F8, int D, int KEYS>
+int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a, bool keys) {
   static const PagedEncodeFn encode = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -931,9 +936,10 @@ int page_map(CUtensorMap* map, const void* base, const PagedAttnArgs& a) {
   const cuuint64_t dims[4] = {TL::kRow / TL::kBytes, static_cast<cuuint64_t>(a.P), TL::kBoxes, static_cast<cuuint64_t>(a.pages) * a.G};
   const cuuint64_t strides[3] = {D * TL::kBytes, TL::kRow, static_cast<cuuint64_t>(a.P) * D * TL::kBytes};
   const cuuint32_t box[4] = {TL::kRow / TL::kBytes, rows, columns, 1}, step[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step,
+  const CUtensorMapDataType type = F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : __is_same(T, __half) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = encode(map, type, 4, const_cast<void*>(base), dims, strides, box, step,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, TL::kRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            keys && !F8 ? CU_TENSOR_MAP_FLOAT_OOB_FILL_NAN_REQUEST_ZERO_FMA : CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 4000 + static_cast<int>(r);
 }
 
@@ -957,8 +963,8 @@ int paged_form(const PagedCall& call) {
   }
   const PagedAttnArgs& a = *call.a;
   CUtensorMap mk, mv;
-  int r = page_map<F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mk, a.k_pages, a);
-  if (r == 0) r = page_map<F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mv, a.v_pages, a);
+  int r = page_map<T, F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mk, a.k_pages, a, true);
+  if (r == 0) r = page_map<T, F8, D, Form<F8, D, ROWS, NR>::kKeys>(&mv, a.v_pages, a, false);
   if (r != 0) return r;
   const int R = a.H / a.G;
   const long long items = (a.starts ? static_cast<long long>(a.rows) * R / ROWS + a.B : static_cast<long long>(a.B) * ((R + ROWS - 1) / ROWS)) * a.G;

@@ -750,3 +750,27 @@ def test_a_length_just_beyond_the_table(monkeypatch, way):
         assert not out[10:30].any()
         out[10:30] = want[10:30]
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ("step", False, True))
+@pytest.mark.parametrize("P, D, dtype, cache", ((16, 64, torch.bfloat16, pc.E4M3), (64, 128, torch.bfloat16, torch.bfloat16), (16, 128, torch.float16, torch.float16), (128, 64, torch.bfloat16, torch.bfloat16),
+                                                (32, 256, torch.bfloat16, pc.E4M3), (32, 256, torch.float16, torch.float16), (128, 128, torch.bfloat16, pc.E4M3)))
+def test_pages_outside_the_cache_show_and_are_not_read(monkeypatch, way, P, D, dtype, cache):
+    """The rows that see such a page are NaN, whatever the cache's first page holds; those before it, and other sequences, are as without it."""
+    if way is True and D > 128:
+        pytest.skip("heads of 256 have one way")
+    monkeypatch.setattr(pc, "gathers", lambda *a: way is True)
+    step = way == "step"
+    b = Batch(held=[200, 600], new=[1, 1] if step else [500, 30], G=2, R=2, P=P, D=D, dtype=dtype, cache=cache, dev="cuda", decode=step, strided=False)
+    want = paged_attention(b.q, b.store, *b.args)
+    for at, page in ((1, 2 ** 31 - 1), (0, -1), (260 // P, -5), (260 // P, b.store.k.shape[0])):
+        if step and at * P > 200:
+            continue
+        table = b.table.clone()
+        table[0, at] = page
+        out = paged_attention(b.q, b.store, table, *b.args[1:])
+        with pytest.raises(RuntimeError):
+            _common.raise_on_device_error()
+        first, rows = max(0, at * P - 200), 1 if step else 500
+        assert torch.isnan(out[first:rows]).all() and torch.equal(out[:first], want[:first]) and torch.equal(out[rows:], want[rows:])

@@ -7,7 +7,8 @@ last positions.  Without ``starts`` every sequence has one row, and none where i
 that depend on them and can be replayed from a CUDA graph.  A page that is written belongs to one sequence; full pages may be shared.
 
 On the GPU, operands that do not go together (a page outside the cache, a length beyond the table or the rotation) are left out and recorded
-(:func:`tyr_b200.ops._common.raise_on_device_error`).  The CPU path states the same contract in plain PyTorch, refuses them, and is the oracle of the numerics tests."""
+(:func:`tyr_b200.ops._common.raise_on_device_error`): nothing is written, the rows of a sequence that is left out are zeros, and those that would see a page outside the
+cache are NaN.  The CPU path states the same contract in plain PyTorch, refuses them, and is the oracle of the numerics tests."""
 from __future__ import annotations
 
 import ctypes
