@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.h"
 
 namespace tyr {
 
@@ -953,12 +954,14 @@ template <typename T, bool F8, int D, int ROWS, int NR>
 int paged_form(const PagedCall& call) {
   constexpr int kSmem = Form<F8, D, ROWS, NR>::kSmem;
   const auto kernel = paged_attention_kernel<T, F8, D, ROWS, NR>;
-  static const cudaError_t ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (ready != cudaSuccess) return -30;
+  static OncePerDevice ready;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -32;
+  if (ready(dev, [&] { return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); }) != 0) return -30;
   if (call.a == nullptr) {
-    int per = 0, dev = 0, sms = 0;
+    int per = 0, sms = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, Form<F8, D, ROWS, NR>::kThreads, kSmem) != cudaSuccess) return -31;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -32;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -32;
     return per * sms;
   }
   const PagedAttnArgs& a = *call.a;

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.h"
 
 namespace tyr {
 namespace cg = cooperative_groups;
@@ -997,11 +998,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 
 template <typename T, bool HELD>
 int sample_form(const SampleArgs& a, int ctas, cudaStream_t stream) {
-  static const cudaError_t ready = [] {
+  static OncePerDevice ready;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -4;
+  const int failed = ready(dev, [] {
     const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleLargest * 4);
-  }();
-  if (ready != cudaSuccess) return static_cast<int>(ready);
+    return static_cast<int>(e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleLargest * 4));
+  });
+  if (failed != 0) return failed;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
   cfg.blockDim = dim3(kSampleThreads);
