@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   pdl_trigger();
   cluster_arrive();                                                        // no CTA writes into another's shared memory before that one runs
   pdl_wait();
-  extern __shared__ float s_logits[];
+  extern __shared__ __align__(16) float s_logits[];                        // 16-byte stores and lists of 64-bit items
   __shared__ SampleShared s;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / C;

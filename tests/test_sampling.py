@@ -240,3 +240,13 @@ def test_many_long_rows(B, V, dtype):
         held = torch.cat([sample(x[i:i + 10], draws[i:i + 10], **kw) for i in range(0, B, 10)])
         # cuts and draws within a rounding of the sums may fall otherwise: a part in 10^12 of the draws
         assert torch.equal(got, held)
+
+
+def test_shared_memory_is_declared_as_it_is_accessed():
+    """Dynamic shared memory follows a kernel's static part: without an alignment of its own, or a base that is rounded up, it starts where that ends."""
+    import pathlib
+    import re
+    for unit in sorted((pathlib.Path(__file__).resolve().parents[1] / "csrc").glob("*.cu")):
+        text = unit.read_text()
+        for decl in re.findall(r"extern __shared__ [^;]*;", text):
+            assert "__align__" in decl or " int " in decl or re.search(r"\+ 1023\)\s*&", text), (unit.name, decl)
