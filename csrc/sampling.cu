@@ -330,14 +330,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   using Four = std::integral_constant<int, 4>;
   using Eight = std::integral_constant<int, 8>;
 
-  if (top == -INFINITY || !(T_row > 0.0)) {                                // nothing to choose from, or the largest: the lowest index that holds it
-    uint32_t first = 0xffffffffu;
-    const bool any = top > -INFINITY;
-    if (infinite) top = 0.f;                                               // as for_all gives it
-    for_all(Eight{}, [&](int j, float v) {
-      if (any && v == top) first = min(first, index_of(j));
-    });
+  // the lowest index of all threads' is the token; none: -1
+  const auto write_lowest = [&](uint32_t first) {
     first = __reduce_min_sync(0xffffffffu, first);
+    __syncthreads();
     if (lane == 0) s.scan[warp] = first;
     __syncthreads();
     if (tid == 0) {
@@ -349,6 +345,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       for (int i = 0; i < C; ++i) first = min(first, s.counts[i]);
       a.token[row] = first == 0xffffffffu ? -1 : static_cast<long long>(first);
     }
+  };
+  if (top == -INFINITY || !(T_row > 0.0)) {                                // nothing to choose from, or the largest: the lowest index that holds it
+    uint32_t first = 0xffffffffu;
+    const bool any = top > -INFINITY;
+    if (infinite) top = 0.f;                                               // as for_all gives it
+    for_all(Eight{}, [&](int j, float v) {
+      if (any && v == top) first = min(first, index_of(j));
+    });
+    write_lowest(first);
     return;
   }
   if (infinite) {
@@ -358,6 +363,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const double c = fmin(fmax(1.4426950408889634 / T_row, 1e-300), 1e300);      // finite: no distance of 0 becomes NaN
   const Weights weigh{exp2(lane / 32.0), static_cast<double>(top), c};
   const double u = a.draws64 ? static_cast<const double*>(a.draws)[row] : static_cast<double>(static_cast<const float*>(a.draws)[row]);
+  // A draw of 0 takes the first index that stays and has a weight in 64 bits (2^-1075 and below rounds to none): sums, in which small weights are lost, do not tell it.
+  const bool at_start = u <= 0.0;
+  const auto weighs = [&](float v) { return (static_cast<double>(v) - weigh.top) * c > -1075.0; };
   const bool by_mass = p < 1.0;
   const float per_bin = fminf(static_cast<float>(c * 64.0), 1e30f);        // bins of 1/64 of a factor of two
   const auto far_of = [&](float v) { return (top - v) * per_bin; };         // in bins; -inf is beyond them all
@@ -498,7 +506,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         if (tid < static_cast<int>(n)) some_w[tid] = w;
         if (tid == 0) s.best = 0, s.bests[0] = 0;
         block_scan_u(w, s.scan_u, total);
-        draw_from(mine, w, 0, list, some_w, n, u * static_cast<double>(total));
+        if (!at_start) draw_from(mine, w, 0, list, some_w, n, u * static_cast<double>(total));
+        else if (stay && weighs(value_of(static_cast<uint32_t>(mine >> 32)))) atomicMax(&s.best, static_cast<unsigned long long>(static_cast<uint32_t>(mine)) + 1);
         write_token();
         return;
       }
@@ -605,6 +614,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         const double exact = weigh(in[r] ? value_of(static_cast<uint32_t>(item[r] >> 32)) : top);
         in[r] = in[r] && exact >= m;
         bin[r] = static_cast<int>(static_cast<unsigned long long>(~static_cast<uint32_t>(item[r])) * kSampleBins / static_cast<unsigned>(a.V));
+      }
+      if (at_start) {
+        if (tid == 0) s.best = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+          if (in[r] && weighs(value_of(static_cast<uint32_t>(item[r] >> 32)))) atomicMax(&s.best, static_cast<unsigned long long>(static_cast<uint32_t>(item[r])) + 1);
+        write_token();
+        return;
       }
       double draw_aim = 0.0;
       const int at = passing_bin(bin, [&](unsigned long long upto, unsigned long long total) {
@@ -910,6 +928,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (by_mass) select(true, 0);
 
   // ---- the draw ------------------------------------------------------------------------------------------------------------
+  if (at_start) {
+    uint32_t first = 0xffffffffu;
+    for_all(Four{}, [&](int j, float v) {
+      const uint32_t key = key_of(v);
+      const bool heavy = m <= 0.0 || weigh(v) >= m;
+      if (key != 0 && heavy && weighs(v) && stays(key, index_of(j), cut)) first = min(first, index_of(j));
+    });
+    write_lowest(first);
+    return;
+  }
   const float low_m = m > 0.0 ? static_cast<float>(top + log2(m) / c - 1e-6 * (fabs(top) + fabs(log2(m) / c))) : -INFINITY;      // no weight below it reaches min_p
   const auto weight_of = [&](int j, float v) {
     const uint32_t key = key_of(v);

@@ -250,3 +250,36 @@ def test_shared_memory_is_declared_as_it_is_accessed():
         text = unit.read_text()
         for decl in re.findall(r"extern __shared__ [^;]*;", text):
             assert "__align__" in decl or " int " in decl or re.search(r"\+ 1023\)\s*&", text), (unit.name, decl)
+
+
+def draws_of_zero(dev, B, V, dtype=torch.float32):
+    """The first index that stays and weighs anything in 64 bits, however far below the largest: by its rank and weight, without sums."""
+    gen = torch.Generator().manual_seed(V)
+    x = 2 * torch.randn(B, V, generator=gen)
+    x[:, :V // 8] -= 20.0                                   # unlikely ones come first
+    x[::3, 3] = -200.0
+    x[1::3, 0] = -math.inf
+    x = x.to(dtype)
+    zeros = torch.zeros(B)
+    rows = x.double()
+    order = torch.sort(rows, dim=1, descending=True, stable=True)[1]
+    rank = torch.empty_like(order).scatter_(1, order, torch.arange(V).expand(B, -1))
+    for kw in (dict(), dict(temperature=0.1), dict(temperature=0.02), dict(top_k=100, temperature=0.1), dict(top_k=1000, temperature=0.1), dict(top_k=V - 1, temperature=0.1),
+               dict(top_p=0.9), dict(min_p=1e-30, temperature=0.2), dict(top_k=V - 2, top_p=0.99, min_p=1e-9, temperature=0.7), dict(top_k=900, min_p=1e-20, temperature=0.1)):
+        w = torch.exp((rows - rows.amax(1, keepdim=True)) / kw.get("temperature", 1.0))
+        first = torch.where(rank < kw.get("top_k", V), w, 0.0)
+        by_rank = first.gather(1, order)
+        before = torch.zeros_like(w).scatter_(1, order, by_rank.cumsum(1) - by_rank)
+        stays = (first > 0) & (w >= kw.get("min_p", 0.0)) & ((before < kw.get("top_p", 2.0) * first.sum(1, keepdim=True)) | (rank == 0))
+        want = stays.int().argmax(1)
+        assert sample(x.to(dev), zeros.to(dev), **kw).tolist() == want.tolist(), kw
+
+
+def test_draws_of_zero_cpu():
+    draws_of_zero("cpu", 9, 5003)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, V, dtype", ((9, 5003, torch.float32), (4, 1500, torch.float16), (6, 151936, torch.bfloat16), (230, 50304, torch.float32)))
+def test_draws_of_zero_gpu(B, V, dtype):
+    draws_of_zero("cuda", B, V, dtype)

@@ -69,7 +69,7 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
     With w = exp((logit - the row's largest) / ``temperature``) and the tokens in the order of their logits, equal ones by index: the first ``top_k`` stay (0 or None:
     all), of these those whose predecessors hold less than ``top_p`` of their weight (1: all; the first always stays), of these those with w >= ``min_p``.  The token is
     the first one, by index, at which the weight of what stays exceeds the row's draw times the whole.  All of it is decided in 64 bits, and a
-    setting given as a number counts as such.
+    setting given as a number counts as such; a draw of 0 takes the first index that stays, however little it weighs, unless that rounds to nothing.
 
     A temperature of 0 takes the largest logit, the lowest index among equals.  -inf and NaN are never chosen, infinite logits share the draw; a row with nothing to
     choose from gives -1.  Every setting is a number or holds one for each row (fp32; ``top_k`` int32), on the logits' device."""
