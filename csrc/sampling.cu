@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const bool at_start = u <= 0.0;
   const auto weighs = [&](float v) { return (static_cast<double>(v) - weigh.top) * c > -1075.0; };
   const bool by_mass = p < 1.0;
-  const float per_bin = fminf(static_cast<float>(c * 64.0), 1e30f);        // bins of 1/64 of a factor of two
+  const float per_bin = fmaxf(fminf(static_cast<float>(c * 64.0), 1e30f), 1e-30f);      // bins of 1/64 of a factor of two; never 0, which no infinite distance takes
   const auto far_of = [&](float v) { return (top - v) * per_bin; };         // in bins; -inf is beyond them all
   const auto bin_of = [&](float v) { return v > -INFINITY ? static_cast<int>(fminf(far_of(v), static_cast<float>(kSampleBins - 1))) : kSampleBins; };
 

@@ -283,3 +283,31 @@ def test_draws_of_zero_cpu():
 @pytest.mark.parametrize("B, V, dtype", ((9, 5003, torch.float32), (4, 1500, torch.float16), (6, 151936, torch.bfloat16), (230, 50304, torch.float32)))
 def test_draws_of_zero_gpu(B, V, dtype):
     draws_of_zero("cuda", B, V, dtype)
+
+
+def greatest_temperatures(dev):
+    """All finite logits weigh the same in the limit, though their distance is beyond 32 bits; -inf stays out."""
+    V = 3000
+    x = torch.where(torch.arange(V) % 2 == 0, 3.3e38, -3.3e38).repeat(3, 1)
+    x[2, 1] = -math.inf
+    order = torch.cat([torch.arange(0, V, 2), torch.arange(1, V, 2)])         # the larger ones first, then the others
+    for t in (math.inf, 1e300, torch.full((3,), math.inf)):
+        for kw in (dict(), dict(top_p=0.75), dict(top_k=2000), dict(top_k=800, top_p=0.5), dict(min_p=0.999)):
+            stays = []
+            for b in range(3):
+                ids = order[~torch.isin(order, torch.tensor([1]))] if b == 2 else order
+                ids = ids[:kw.get("top_k", V)]
+                stays.append(sorted(ids[:math.ceil(kw.get("top_p", 1.0) * len(ids))].tolist()))
+            u = torch.tensor([0.2505, 0.7505, 0.9005])
+            want = [ids[math.floor(len(ids) * float(f))] for ids, f in zip(stays, u)]
+            got = sample(x.to(dev), u.to(dev), temperature=t.to(dev) if torch.is_tensor(t) else t, **kw)
+            assert got.tolist() == want, (t, kw)
+
+
+def test_greatest_temperatures_cpu():
+    greatest_temperatures("cpu")
+
+
+@pytest.mark.gpu
+def test_greatest_temperatures_gpu():
+    greatest_temperatures("cuda")
