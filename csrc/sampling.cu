@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     __syncwarp();
   }
-  const double T_row = a.temperature ? a.temperature[row] : a.t, p = a.top_p ? a.top_p[row] : a.p, m = fmin(a.min_p ? a.min_p[row] : a.m, 1.0);
+  const double T_row = a.temperature ? a.temperature[row] : a.t, p = a.top_p ? a.top_p[row] : a.p, m_row = a.min_p ? a.min_p[row] : a.m;
+  const double m = m_row > 0.0 ? fmin(m_row, 1.0) : 0.0;                   // no number: no filter, as p
   const int k_row = a.top_k ? a.top_k[row] : a.k;
   float own_top = top;
   top = warp_max(top);

@@ -311,3 +311,22 @@ def test_greatest_temperatures_cpu():
 @pytest.mark.gpu
 def test_greatest_temperatures_gpu():
     greatest_temperatures("cuda")
+
+
+def settings_of_no_number(dev):
+    gen = torch.Generator().manual_seed(6)
+    x, u = (2 * torch.randn(6, 4000, generator=gen)).to(dev), torch.rand(6, generator=gen).to(dev)
+    nan, ones = torch.full((6,), math.nan, device=dev), torch.ones(6, device=dev)
+    for kw in (dict(), dict(top_k=50), dict(top_k=2500), dict(temperature=0.5)):
+        plain = sample(x, u, **kw)
+        assert torch.equal(sample(x, u, min_p=nan, **kw), plain) and torch.equal(sample(x, u, top_p=nan, **kw), plain) and torch.equal(sample(x, u, min_p=-ones, **kw), plain)
+    assert torch.equal(sample(x, u, temperature=nan), x.argmax(1)) and torch.equal(sample(x, u, min_p=3 * ones), x.argmax(1))
+
+
+def test_settings_of_no_number_cpu():
+    settings_of_no_number("cpu")
+
+
+@pytest.mark.gpu
+def test_settings_of_no_number_gpu():
+    settings_of_no_number("cuda")

@@ -41,7 +41,7 @@ def _setting(name: str, v, rows: int, dev: int, dtype: torch.dtype, least: float
 
 def _sample_ref(logits, draws, temperature, top_k, top_p, min_p):
     column = lambda v: (v.double() if isinstance(v, torch.Tensor) else torch.full((logits.shape[0],), float(v), dtype=torch.float64, device=logits.device))[:, None]
-    t, k, p, m = column(temperature), column(top_k), column(top_p), column(min_p).clamp(max=1.0)
+    t, k, p, m = column(temperature), column(top_k), column(top_p), column(min_p).nan_to_num(nan=0.0).clamp(max=1.0)
     x = logits.double() + 0.0                                       # -0 is 0
     x = torch.where(torch.isnan(x), -math.inf, x)
     infinite = (x == math.inf).any(-1, keepdim=True)
@@ -72,7 +72,8 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Setting = 
     setting given as a number counts as such; a draw of 0 takes the first index that stays, however little it weighs, unless that rounds to nothing.
 
     A temperature of 0 takes the largest logit, the lowest index among equals.  -inf and NaN are never chosen, infinite logits share the draw; a row with nothing to
-    choose from gives -1.  Every setting is a number or holds one for each row (fp32; ``top_k`` int32), on the logits' device."""
+    choose from gives -1.  Every setting is a number or holds one for each row (fp32; ``top_k`` int32), on the logits' device; NaN for a row filters nothing there, and as its temperature
+    takes the largest logit."""
     shape, dev = logits.shape, logits.get_device()
     if len(shape) != 2 or shape[0] == 0 or shape[1] == 0:
         raise ValueError(f"sample: logits are [rows, vocabulary], got {tuple(shape)}")
