@@ -227,16 +227,36 @@ __device__ __forceinline__ uint32_t halves_of_codes(uint32_t w) {
 
 template <typename T> struct Num;
 template <> struct Num<__nv_bfloat16> {
+  static constexpr uint32_t kExponent = 0x7f80u;
   static __device__ __forceinline__ float2 two(uint32_t u) { return unpack_bf16x2(u); }
   static __device__ __forceinline__ uint32_t pack(float x, float y) { return pack_bf16x2(x, y); }
 };
 template <> struct Num<__half> {
+  static constexpr uint32_t kExponent = 0x7c00u;
   static __device__ __forceinline__ float2 two(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
+// Infinities and NaN among a word's two numbers of type T.
+template <typename T> __device__ __forceinline__ bool low_odd(uint32_t w) { return (w & Num<T>::kExponent) == Num<T>::kExponent; }
+template <typename T> __device__ __forceinline__ bool high_odd(uint32_t w) { return low_odd<T>(w >> 16); }
+// Zeros in their place; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool without_odd(uint4& u) {
+  bool any = false;
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool low = low_odd<T>(w[i]), high = high_odd<T>(w[i]);
+    if (low) w[i] &= 0xffff0000u;
+    if (high) w[i] &= 0xffffu;
+    any |= low || high;
+  }
+  u = make_uint4(w[0], w[1], w[2], w[3]);
+  return any;
+}
 // c [16, 8] += a [16, 16] b [16, 8]; M is the operands' type.
 template <typename M>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -622,6 +642,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             }
           }
       }
+      bool odd = false;                                                     // values that are not finite in a tile that not all rows see
       // ---- probabilities, turned so that a lane holds row g's keys 2 t and 2 t + 1, and their product with the values ----------------
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
@@ -676,6 +697,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
               if (2 * t + 8 >= left) zs = make_uint4(0u, 0u, 0u, 0u);
               if (((2 * t + 1) ^ 4) + 8 >= left) us = make_uint4(0u, 0u, 0u, 0u);
             }
+            if constexpr (!F8) {
+              // ... and no more may a value behind a row's own position, or before its window
+              if (masked) odd |= without_odd<T>(xs) | without_odd<T>(ys) | without_odd<T>(zs) | without_odd<T>(us);
+            }
             const uint32_t x[4] = {xs.x, xs.y, xs.z, xs.w}, y[4] = {ys.x, ys.y, ys.z, ys.w}, z[4] = {zs.x, zs.y, zs.z, zs.w}, u[4] = {us.x, us.y, us.z, us.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -687,6 +712,30 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
               }
             }
           }
+        }
+      }
+      if constexpr (!F8) {
+        // values that are not finite, to the rows that see them: a lane has eight channels of a box
+        if (__any_sync(0xffffffffu, odd)) {
+          for (int key = 0; key < min(KEYS, sh.s.len - key0); ++key)
+#pragma unroll
+            for (int c = 0; c < TL::kBoxes; ++c) {
+              const uint4 u = lds128(TL::at(vb, key, 8 * c + g));
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = Num<T>::two(w[i]);
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int p = pos[r][e];
+                    if (key0 + key > p || (a.window > 0 && key0 + key <= p - a.window)) continue;
+                    if (low_odd<T>(w[i])) o[4 * c + i][r][e] += f.x;
+                    if (high_odd<T>(w[i])) o[4 * c + i][r][2 + e] += f.y;
+                  }
+              }
+            }
         }
       }
       __syncwarp();

@@ -774,3 +774,41 @@ def test_pages_outside_the_cache_show_and_are_not_read(monkeypatch, way, P, D, d
             _common.raise_on_device_error()
         first, rows = max(0, at * P - 200), 1 if step else 500
         assert torch.isnan(out[first:rows]).all() and torch.equal(out[:first], want[:first]) and torch.equal(out[rows:], want[rows:])
+
+
+def odd_values(dev, step, D, dtype, P=16, R=2):
+    """Infinities and NaN among the values in 16 bits: in their channel, at the rows that see them, and nowhere else (a row before its neighbour's token, a window past it)."""
+    b = Batch(held=[150, 70], new=[1, 1] if step else [300, 20], G=2, R=R, P=P, D=D, dtype=dtype, cache=dtype, dev=dev, decode=step, strided=False)
+    b.q = (0.3 * b.q).contiguous()                         # no probability rounds to nothing
+    clean = b.copy()
+    places = ((0, 20, 0, 3, math.inf), (0, 90, 0, 11, math.nan), (0, 100, 1, D - 1, math.nan), (0, 145, 0, 9, -math.inf), (1, 66, 1, 17, math.inf)) if step else (
+        (0, 20, 0, 3, math.inf), (0, 160, 0, 3, -math.inf), (0, 161, 1, D - 1, math.nan), (0, 299, 0, 40, math.inf), (0, 449, 0, 41, -math.inf), (1, 75, 1, 17, math.inf), (1, 89, 0, 0, math.nan))
+    for s, key, g, d, value in places:
+        page = int(b.table[s, key // P])
+        clean.v[page, g, key % P, d], b.store.v[page, g, key % P, d] = 0.0, value
+    for window in (None, 7, 60):
+        want = paged_attention(b.q, clean, *b.args, window=window)
+        assert torch.isfinite(want).all()
+        for s, key, g, d, value in places:
+            new, row0 = b.new[s], b.row_of[s]
+            pos = torch.arange(b.lens[s] - new, b.lens[s])
+            rows = row0 + torch.nonzero((pos >= key) & (pos < key + (window or 10 ** 6)))[:, 0]
+            want[rows.to(dev), g * R:(g + 1) * R, d] += value
+        out = paged_attention(b.q, b.store, *b.args, window=window)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(0.0, 1e4, -1e4), want.nan_to_num(0.0, 1e4, -1e4))
+
+
+@pytest.mark.parametrize("step", (True, False))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_odd_values_show_where_they_are_seen_cpu(step, dtype):
+    odd_values("cpu", step, 64, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step, R", ((True, 2), (True, 12), (False, 2), (False, 5)))
+@pytest.mark.parametrize("D, P", ((64, 16), (128, 64), (256, 16), (128, 128)))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_odd_values_show_where_they_are_seen_gpu(monkeypatch, step, R, D, P, dtype):
+    monkeypatch.setattr(pc, "gathers", lambda *a: False)
+    odd_values("cuda", step, D, dtype, P, R)
+    _common.raise_on_device_error()

@@ -315,8 +315,13 @@ def _attend_ref(q, store, table, lengths, starts, window, scale):
         if store.v_scale is not None:                    # a page whose values hold no numbers shows at the keys that are seen, as in the kernel
             s, v = s.masked_fill(torch.isnan(v[..., 0])[:, None, None], math.nan), torch.nan_to_num(v, nan=0.0)
         ago = torch.arange(n - new, n)[:, None] - torch.arange(n)
-        s = s.masked_fill((ago < 0) | (ago >= (window or n)), -math.inf)
-        out[row:row + new] = torch.einsum("grnl,gld->ngrd", s.softmax(-1), v).reshape(new, H, D).to(q.dtype)
+        unseen = (ago < 0) | (ago >= (window or n))
+        s = s.masked_fill(unseen, -math.inf)
+        odd = ~torch.isfinite(v)
+        o = torch.einsum("grnl,gld->ngrd", s.softmax(-1), v.masked_fill(odd, 0.0))
+        for g, key in odd.any(-1).nonzero().tolist():      # values that are not finite show at the rows that see them, and at no others
+            o[~unseen[:, key], g] += torch.where(odd[g, key], v[g, key], 0.0)
+        out[row:row + new] = o.reshape(new, H, D).to(q.dtype)
     return out
 
 
