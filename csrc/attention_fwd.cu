@@ -83,6 +83,10 @@ struct AttnParams {
   // ragged form only
   const int *starts, *lengths;   // [B + 1], [B]
   int rows;           // of the queries; `keep`: the most tokens that a sequence may have
+  // values that are not finite, which lie in V as zeros: [B, Hkv, capacity, dv], where a flag says so, one for every 256 / dv tokens
+  const void* odd;
+  const uint8_t* odd_flags;
+  long long capacity;
 };
 
 constexpr int ATT_TBL_PAD = 256;       // table entries below distance 0 and past the window that boundary blocks can touch
@@ -135,6 +139,11 @@ __device__ __forceinline__ uint32_t pack_16x2(float a, float b) {
   } else {
     return pack_bf16x2(a, b);
   }
+}
+template <bool HALF>
+__device__ __forceinline__ float2 unpack_16x2(uint32_t u) {
+  if constexpr (HALF) return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  else return unpack_bf16x2(u);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -408,8 +417,17 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
     const bool exact_max = kPenalty && fabsf(penalty(ATT_BN - 1)) > 48.f;
     float m_used = -INFINITY;   // running maximum the exponentials are taken against
     float l_sum = 0.f;          // this half's part of the row sum
-    bool ok = true;
+    bool ok = true, odd = false;                // odd: this tile's keys have values that are not finite
     uint32_t cnt = 0;
+    if constexpr (kRagged) {
+      const int per = ATT_BN * p.dv / 256;      // flags of a key block
+      const uint8_t* flags = p.odd_flags + (static_cast<long long>(batch) * p.Hkv + kv_head) * p.capacity * p.dv / 256;
+      for (int i = lo[t] * per + lane * 16; i < hi[t] * per; i += 512) {
+        const uint4 u = *reinterpret_cast<const uint4*>(flags + i);
+        odd |= (u.x | u.y | u.z | u.w) != 0u;
+      }
+      odd = __any_sync(0xffffffffu, odd);
+    }
     if (tile_live) {
       const int j0 = kept > 0 ? 0 : lo[t];
       for (int j = j0; j < hi[t] && ok; j = after(j, lo[t]), ++cnt) {
@@ -595,6 +613,28 @@ flash_fwd_d128_kernel(const __grid_constant__ CUtensorMap tmQ,
           uint32_t o[32];
           tmem_ld_32x32_nowait(o_addr + c * 32, o);   // warp-collective: every lane takes part
           tmem_wait_ld();
+          if constexpr (kRagged) {
+            if (odd && row_ok && h * 64 + c * 32 < p.dv) {      // added to the rows that see them: a product with a probability of 0 would be NaN
+              const long long first = (static_cast<long long>(batch) * p.Hkv + kv_head) * p.capacity;
+              const int last = min(p.Tk - 1, row + p.q_offset), from = p.window > 0 ? max(0, row + p.q_offset - p.window + 1) : 0;
+#pragma unroll 1
+              for (int key = from; key <= last; ++key) {
+                if (p.odd_flags[(first + key) * p.dv / 256] == 0) continue;
+                const uint4* at = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.odd) + (first + key) * p.dv + h * 64 + c * 32);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const uint4 u = at[q];
+                  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float2 f = unpack_16x2<kHalf>(w[e]);
+                    o[q * 8 + 2 * e] = __float_as_uint(__uint_as_float(o[q * 8 + 2 * e]) + f.x);
+                    o[q * 8 + 2 * e + 1] = __float_as_uint(__uint_as_float(o[q * 8 + 2 * e + 1]) + f.y);
+                  }
+                }
+              }
+            }
+          }
           if (row_ok) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -783,8 +823,8 @@ extern "C" TYR_EXPORT int tyr_flash_fwd_kept(const void* q, const void* k, const
 }
 
 // Attention of ragged rows q [rows, Hq, D] (strides of rows and heads) over the keys and values [B, Hkv, capacity, D] of their sequences (see the kernel's head), of
-// which `longest` tokens may be there: a sequence of more has none that were brought; out [rows, Hq, D].  dtype: 0 = bf16, 1 = fp16.  D: 64 or 128.
-int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
+// which `longest` tokens may be there: a sequence of more has none that were brought; odd, odd_flags: as AttnParams has them; out [rows, Hq, D].  dtype: 0 = bf16, 1 = fp16.  D: 64 or 128.
+int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, const void* odd, const uint8_t* odd_flags, void* out, const int* starts, const int* lengths, int rows, int B,
                          int Hq, int Hkv, int D, long long capacity, int longest, int window, float scale, int dtype, int* err, cudaStream_t stream) {
   const long long st[6] = {0, q_row, q_head, Hkv * capacity * D, D, capacity * D};
   CUtensorMap tq, tk, tv;
@@ -807,7 +847,7 @@ int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const
   p.scale_log2 = scale * 1.4426950408889634f;
   p.O = static_cast<__nv_bfloat16*>(out); p.o_row_stride = static_cast<long long>(Hq) * D; p.o_head_stride = D;
   p.err = err; p.k_steps = D / 16; p.dv = D; p.starts = starts; p.lengths = lengths; p.rows = rows;
-  p.keep = longest;
+  p.keep = longest; p.odd = odd; p.odd_flags = odd_flags; p.capacity = capacity;
   const long long blocks = (static_cast<long long>(rows) / (2 * ATT_BM) + B) * Hq;
   if (blocks > 0x7fffffff) return -5;
   const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), dim3(640), kSmem, stream, tq, tk, tv, p);

@@ -895,8 +895,9 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
 // The pages of every sequence as the ragged form of the attention kernel on tcgen05 (csrc/attention_fwd.cu) takes them: keys and values [B, G, capacity, D] in the
 // queries' type, zeros behind the end up to a multiple of 128.  A (sequence, head) is one blockIdx.(z, y).  A page outside the cache,
 // and the codes of one whose scales are no numbers, give keys that are none and values of zero, so that it shows at the rows that see it.  Rows of no sequence, or of one whose operands do not go together, are zeroed on the way.
+// Values that are not finite go to a place of their own, with a flag for each warp's tokens, and are zeros among the values.
 template <typename T, bool F8>
-__global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedAttnArgs a, void* k_out, void* v_out, long long capacity) {
+__global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedAttnArgs a, void* k_out, void* v_out, void* odd_out, uint8_t* odd_flags, long long capacity) {
   pdl_entry();
   const int b = blockIdx.z, head = blockIdx.y, lanes = a.D / 8, lane = threadIdx.x % lanes, per = 256 / lanes;
   if (head == 0) {
@@ -960,6 +961,10 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
         x = from[i] == -2 ? make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu) : k[i];
         y = v[i];
       }
+      const uint4 all = y;
+      const bool odd = __any_sync(0xffffffffu, without_odd<T>(y));          // a warp has whole tokens, all before `end`
+      if (threadIdx.x % 32 == 0) odd_flags[to >> 8] = odd;
+      if (odd) *reinterpret_cast<uint4*>(static_cast<T*>(odd_out) + to) = make_uint4(all.x ^ y.x, all.y ^ y.y, all.z ^ y.z, all.w ^ y.w);
       *reinterpret_cast<uint4*>(static_cast<T*>(k_out) + to) = x;
       *reinterpret_cast<uint4*>(static_cast<T*>(v_out) + to) = y;
     }
@@ -1051,28 +1056,31 @@ int paged_type(const PagedCall& call, int dtype, bool f8, int D, int rows, bool 
 
 }  // namespace tyr
 
-int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, void* out, const int* starts, const int* lengths, int rows, int B,
+int tyr_flash_fwd_ragged(const void* q, long long q_row, long long q_head, const void* k, const void* v, const void* odd, const uint8_t* odd_flags, void* out, const int* starts, const int* lengths, int rows, int B,
                          int Hq, int Hkv, int D, long long capacity, int longest, int window, float scale, int dtype, int* err, cudaStream_t stream);
 
 using namespace tyr;
 
-// The same result for many new tokens a sequence: the pages laid out in `part` (2 * B * G * capacity * D numbers of the queries' type, capacity a multiple of 128 that
-// holds the table's tokens), then the kernel on tcgen05.
+// The same result for many new tokens a sequence: the pages laid out in `part` (with n = B * G * capacity * D: n keys, n values and room for n values that are not
+// finite, in the queries' type, and n / 256 bytes of flags; capacity a multiple of 128 that holds the table's tokens), then the kernel on tcgen05.
 extern "C" TYR_EXPORT int tyr_paged_attention_gathered(const void* packed, int dtype, long long capacity, void* stream) {
   const PagedAttnArgs& a = *static_cast<const PagedAttnArgs*>(packed);
   if (a.rows <= 0 || a.B <= 0 || a.B > 65535 || a.H <= 0 || a.G <= 0 || a.G > 65535 || a.H % a.G != 0 || a.pages <= 0 || a.width <= 0 || a.window < 0) return -1;
   if ((a.P != 16 && a.P != 32 && a.P != 64 && a.P != 128) || (a.D != 64 && a.D != 128) || a.starts == nullptr || a.part == nullptr) return -2;
   if (capacity % 128 != 0 || capacity < static_cast<long long>(a.width) * a.P || capacity > 0x7fffffffLL || (a.k_scale != nullptr) != (a.v_scale != nullptr)) return -3;
-  void *k = a.part, *v = reinterpret_cast<uint8_t*>(a.part) + 2LL * a.B * a.G * capacity * a.D;
+  const long long numbers = static_cast<long long>(a.B) * a.G * capacity * a.D;
+  uint8_t* work = reinterpret_cast<uint8_t*>(a.part);
+  void *k = work, *v = work + 2 * numbers, *odd = work + 4 * numbers;
+  uint8_t* flags = work + 6 * numbers;
   // some eight rounds of blocks over the SMs' places, or as many as the longest sequence may fill
   const long long chunks = capacity * a.D / 8192, most = 9472 / (static_cast<long long>(a.G) * a.B) + 1;
   const dim3 grid(static_cast<unsigned>(chunks < most ? chunks : most), a.G, a.B);
   const bool f8 = a.k_scale != nullptr;
   const auto gather = dtype == 0 ? (f8 ? paged_gather_kernel<__nv_bfloat16, true> : paged_gather_kernel<__nv_bfloat16, false>)
                                  : (f8 ? paged_gather_kernel<__half, true> : paged_gather_kernel<__half, false>);
-  const cudaError_t e = launch_dependent(gather, grid, dim3(256), 0, (cudaStream_t)stream, a, k, v, capacity);
+  const cudaError_t e = launch_dependent(gather, grid, dim3(256), 0, (cudaStream_t)stream, a, k, v, odd, flags, capacity);
   if (e != cudaSuccess) return static_cast<int>(e);
-  return tyr_flash_fwd_ragged(a.q, a.q_row, a.q_head, k, v, a.out, a.starts, a.lengths, a.rows, a.B, a.H, a.G, a.D, capacity, a.width * a.P, a.window, a.scale, dtype, a.err, (cudaStream_t)stream);
+  return tyr_flash_fwd_ragged(a.q, a.q_row, a.q_head, k, v, odd, flags, a.out, a.starts, a.lengths, a.rows, a.B, a.H, a.G, a.D, capacity, a.width * a.P, a.window, a.scale, dtype, a.err, (cudaStream_t)stream);
 }
 
 // dtype: 0 = bf16, 1 = fp16 (queries, results, and pages without scales); rows of a tile: 16, or 128 (64 of heads of 256).

@@ -812,3 +812,28 @@ def test_odd_values_show_where_they_are_seen_gpu(monkeypatch, step, R, D, P, dty
     monkeypatch.setattr(pc, "gathers", lambda *a: False)
     odd_values("cuda", step, D, dtype, P, R)
     _common.raise_on_device_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", (2, 5))
+@pytest.mark.parametrize("D, P", ((64, 16), (128, 64), (64, 128), (128, 16)))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_odd_values_show_where_they_are_seen_laid_out(monkeypatch, R, D, P, dtype):
+    monkeypatch.setattr(pc, "gathers", lambda *a: True)
+    odd_values("cuda", False, D, dtype, P, R)
+    _common.raise_on_device_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", (True, False))
+def test_values_in_8_bits_beyond_the_types_end(monkeypatch, way):
+    """256 in units of 2^120 is infinite in 32 bits: rows that do not see it are as without it."""
+    monkeypatch.setattr(pc, "gathers", lambda *a: way)
+    b = Batch(held=[100], new=[300], G=2, R=2, P=16, D=64, dtype=torch.bfloat16, cache=pc.E4M3, dev="cuda", strided=False)
+    b.store.v[int(b.table[0, 18]), 1] = 0.0                # positions 288 to 303
+    want = paged_attention(b.q, b.store, *b.args)
+    page = int(b.table[0, 18])
+    b.store.v[page, 1, 5, 7] = 256.0
+    b.store.v_scale[page, 1] = 2.0 ** 120
+    out = paged_attention(b.q, b.store, *b.args)
+    assert torch.equal(out[:188], want[:188]) and torch.equal(out[:, :2], want[:, :2]) and bool((out[193:, 2:, 7] > 1e30).all())

@@ -278,7 +278,7 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     return out
 
 
-# the most that pages laid out for the kernel on tcgen05 may take
+# the most that keys and values laid out for the kernel on tcgen05 may take
 GATHER_MAX_BYTES = 2 ** 30
 
 
@@ -349,7 +349,8 @@ def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, len
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if starts is not None and gathers(dtype, f8, rows, B, H, G, D, width * P, scale):
         capacity = -(-width * P // 128) * 128
-        work = torch.empty(2 * B * G * capacity * D, dtype=dtype, device=device)
+        numbers = B * G * capacity * D                # keys, values, room for values that are not finite, and a byte for 256 of them
+        work = torch.empty(3 * numbers + numbers // 512, dtype=dtype, device=device)
         packed = _ATTEND.pack(q.data_ptr(), out.data_ptr(), store.k.data_ptr(), store.v.data_ptr(), store.k_scale.data_ptr() if f8 else 0, store.v_scale.data_ptr() if f8 else 0,
                               table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), work.data_ptr(), err_word(device).data_ptr(), stride[0], stride[1], table_row, rows, B, H, G,
                               D, P, pages, width, min(window or 0, 2 ** 30), 0, scale, 0)
