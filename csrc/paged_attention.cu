@@ -380,6 +380,18 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         }
       }
     }
+    // rows of no sequence, and of those whose operands do not go together
+    const auto clear = [&](int row) {
+      for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * D + i) = make_uint4(0u, 0u, 0u, 0u);
+    };
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x)
+      if (a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0 || !rows_of(a, row).fits) clear(row);
+    if (a.starts)
+      for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+        const Rows r = rows_of(a, b);
+        if (!r.fits)
+          for (int row = max(r.row, 0); row < min(r.end, a.rows); ++row) clear(row);
+      }
     return;
   }
 
@@ -394,18 +406,6 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   for (int c = 0; c < PIECES_BOX; ++c) k_at[c] = TL::at(0, pi, t + 4 * c);
 #pragma unroll
   for (int i = 0; i < 2; ++i) v_at[i] = F8 && D == 64 ? TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g >> 1) + (g & 1) * 8 : TL::at(0, i ? (2 * t + 1) ^ 4 : 2 * t, g);
-  // rows of no sequence, and of those whose operands do not go together
-  const auto clear = [&](int row) {
-    for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.H * D + i) = make_uint4(0u, 0u, 0u, 0u);
-  };
-  for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps)
-    if (a.starts ? row < a.starts[0] || row >= a.starts[a.B] : a.lengths[row] <= 0 || !rows_of(a, row).fits) clear(row);
-  if (a.starts)
-    for (int b = blockIdx.x * kWarps + warp; b < a.B; b += gridDim.x * kWarps) {
-      const Rows r = rows_of(a, b);
-      if (!r.fits)
-        for (int row = max(r.row, 0); row < min(r.end, a.rows); ++row) clear(row);
-    }
   PartHead head{0, 0, 0, -1, 0, {0, 0, 0}};
   if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
   bool first_piece = true, lost = false;
