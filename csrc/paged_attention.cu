@@ -208,6 +208,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
@@ -239,9 +242,14 @@ template <> struct Num<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
-// Infinities and NaN among a word's two numbers of type T.
-template <typename T> __device__ __forceinline__ bool low_odd(uint32_t w) { return (w & Num<T>::kExponent) == Num<T>::kExponent; }
-template <typename T> __device__ __forceinline__ bool high_odd(uint32_t w) { return low_odd<T>(w >> 16); }
+// Infinities and NaN among a word's two numbers of type T: an exponent of ones carries into the sign's place.
+template <typename T> __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  constexpr uint32_t kOnes = Num<T>::kExponent * 0x10001u, kLast = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+  return (w & kOnes) + kLast;
+}
+template <typename T> __device__ __forceinline__ bool any_odd(const uint4& u) {
+  return ((odd_bits<T>(u.x) | odd_bits<T>(u.y) | odd_bits<T>(u.z) | odd_bits<T>(u.w)) & 0x80008000u) != 0u;
+}
 // Zeros in their place; whether there were any.
 template <typename T>
 __device__ __forceinline__ bool without_odd(uint4& u) {
@@ -249,10 +257,10 @@ __device__ __forceinline__ bool without_odd(uint4& u) {
   uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const bool low = low_odd<T>(w[i]), high = high_odd<T>(w[i]);
-    if (low) w[i] &= 0xffff0000u;
-    if (high) w[i] &= 0xffffu;
-    any |= low || high;
+    const uint32_t odd = odd_bits<T>(w[i]);
+    if (odd & 0x8000u) w[i] &= 0xffff0000u;
+    if (odd & 0x80000000u) w[i] &= 0xffffu;
+    any |= (odd & 0x80008000u) != 0u;
   }
   u = make_uint4(w[0], w[1], w[2], w[3]);
   return any;
@@ -292,6 +300,37 @@ __device__ __forceinline__ void write4(T* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(Num<T>::pack(v.x, v.y), Num<T>::pack(v.z, v.w));
 }
 
+// Values that are not finite at keys that not all rows of a piece see, to the result (or the piece's sums) of those that do: once more through this CTA's share, when all of
+// it is written.  A call of its own, so that the products' registers are none of its: among the products it took up to a quarter of every call.
+template <typename T, int D, int ROWS, int KEYS>
+__device__ __noinline__ void add_odd(const PagedAttnArgs& a) {
+  Share<ROWS, KEYS> sh(a, threadIdx.x & 31);
+  const int R = a.H / a.G;
+  for (int slot = 0; sh.next(); slot = 1) {
+    const int held = sh.s.len - sh.s.n, used = min(ROWS, sh.s.n * R - sh.row_tile * ROWS), p0 = held + sh.row_tile * ROWS / R, p1 = held + (sh.row_tile * ROWS + used - 1) / R;
+    const int seen0 = a.window > 0 ? max(0, p1 - a.window + 1) : 0, seen1 = p0 + 1;      // keys that all rows see went through the products; adding others twice is the same
+    for (int i = threadIdx.x; i < used * D; i += blockDim.x) {
+      const int in_tile = i / D, d = i % D, row = sh.row_tile * ROWS + in_tile, p = held + row / R;
+      for (int key = max(sh.first * KEYS, a.window > 0 ? p - a.window + 1 : 0); key < min(sh.last * KEYS, p + 1); ++key) {
+        if (key >= seen0 && key < seen1) {
+          key = seen1 - 1;
+          continue;
+        }
+        const int page = a.table[sh.b * a.table_row + key / a.P];
+        if (page < 0 || page >= a.pages) continue;
+        const T v = static_cast<const T*>(a.v_pages)[((static_cast<long long>(page) * a.G + sh.head) * a.P + key % a.P) * D + d];
+        if ((odd_bits<T>(reinterpret_cast<const uint16_t&>(v)) & 0x8000u) == 0u) continue;
+        if (sh.begins && sh.ends) {
+          T& out = static_cast<T*>(a.out)[((sh.s.row + static_cast<long long>(row / R)) * a.H + sh.head * R + row % R) * D + d];
+          out = static_cast<T>(static_cast<float>(out) + static_cast<float>(v));
+        } else {
+          part_sums(a, gridDim.x, ROWS, 2 * blockIdx.x + slot)[static_cast<long long>(in_tile) * D + d] += static_cast<float>(v);
+        }
+      }
+    }
+  }
+}
+
 // T: type of the queries, the results and 16-bit pages; NR: rows of a lane (1: at most 8 rows in a tile of 16).
 template <typename T, bool F8, int D, int ROWS, int NR>
 __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROWS, NR>::kAtOnce) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
@@ -309,6 +348,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* extra = smem + STAGES * 2 * TL::kSize;
   float2* s_scale = reinterpret_cast<float2*>(extra);                       // [STAGES][4]: scale of the keys, log2 of the values'
+  volatile int* met_odd = reinterpret_cast<volatile int*>(extra);             // 16-bit pages, which have no scales: whether values that are not finite were met
   uint64_t* full = reinterpret_cast<uint64_t*>(extra + STAGES * 32);
   uint64_t* empty = full + STAGES;
   float* s_stats = reinterpret_cast<float*>(empty + STAGES);                // [4][16][4], joining warps (ROWS 16)
@@ -323,6 +363,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
       mbar_init(empty + i, ROWS == 16 ? 1 : kWarps);
     }
     mbar_fence_init();
+    if (!F8) *met_odd = 0;
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
@@ -335,7 +376,7 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
   if (warp == kWarps) {
     // ---- producer ---------------------------------------------------------------------------------------------------
     const int page_rows = min(a.P, KEYS), page_bits = 31 - __clz(a.P), per_tile = KEYS >> min(page_bits, 31 - __clz(KEYS));
-    while (sh.next()) {
+    for (bool ok = true; ok && sh.next();) {
       const int last_page = (sh.s.len - 1) >> page_bits;
       const int* table = a.table + sh.b * a.table_row;
       int batch = -1, id = 0;                       // pages 32 batch .. of the sequence, one a lane
@@ -359,7 +400,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         const int n = min(per_tile, last_page - p0 + 1), from = (p0 & 31) + lane;
         const int page = __shfl_sync(0xffffffffu, id, from & 31);
         const float2 sc = make_float2(__shfl_sync(0xffffffffu, scale.x, from & 31), __shfl_sync(0xffffffffu, scale.y, from & 31));
-        if (!mbar_wait(empty + stage, phase ^ 1, a.err, 1)) return;
+        if (!mbar_wait(empty + stage, phase ^ 1, a.err, 1)) {
+          ok = false;
+          break;
+        }
         if (F8 && lane < per_tile) s_scale[stage * 4 + lane] = sc;
         __syncwarp();
         if (lane == 0) mbar_expect_tx(full + stage, static_cast<uint32_t>(2 * n * page_rows * D * TL::kBytes));
@@ -392,6 +436,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         if (!r.fits)
           for (int row = max(r.row, 0); row < min(r.end, a.rows); ++row) clear(row);
       }
+    if constexpr (!F8) {
+      __syncthreads();
+      if (*met_odd != 0) add_odd<T, D, ROWS, KEYS>(a);
+    }
     return;
   }
 
@@ -498,6 +546,8 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     const int clear0 = a.window > 0 ? (max(0, p_last - a.window + 1) + KEYS - 1) / KEYS : 0, clear1 = (p_first + 1) / KEYS;
 
     const int p_warp = held + (sh.row_tile * ROWS + min(used, warp_row + 16) - 1) / R;
+    // keys that all of this warp's rows see: from seen0 on, before seen1
+    const int seen0 = a.window > 0 ? max(0, p_warp - a.window + 1) : 0, seen1 = held + (sh.row_tile * ROWS + warp_row) / R + 1;
 
     float m[NR][2], l[NR][2], top[NR][2], o[TILES][NR][4];
 #pragma unroll
@@ -526,6 +576,34 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         continue;
       }
       const uint32_t kb = smem_u32(smem + stage * 2 * TL::kSize), vb = kb + TL::kSize;
+      const int key0 = tile * KEYS;
+      const bool masked = tile < clear0 || tile >= clear1;
+      // Values that are not finite at keys that not all of the warp's rows see: an unseen one times a probability of 0 would be NaN.  They become zeros in place, by every warp for itself
+      // (all write the same), and are added to the result of the rows that see them.  Looking takes 88 -> 92 us of 6 x 64 tokens of 20 heads over 3000 tokens of 4, and
+      // nothing while decoding, where every row sees all keys.
+      if constexpr (!F8) {
+        if (masked) {
+          const int n = min(KEYS, sh.s.len - key0), past = min(n, max(0, seen1 - key0)), ahead = min(past, seen0 - key0);      // keys before `ahead`, and from `past` on
+          const auto unseen = [&](auto f) {
+#pragma unroll 1
+            for (int i = lane; i < ahead * TL::kChunks; i += 32) f(TL::at(vb, i / TL::kChunks, i % TL::kChunks));
+#pragma unroll 1
+            for (int i = past * TL::kChunks + lane; i < n * TL::kChunks; i += 32) f(TL::at(vb, i / TL::kChunks, i % TL::kChunks));
+          };
+          bool odd = false;
+          unseen([&](uint32_t at) { odd |= any_odd<T>(lds128(at)); });
+          if (__any_sync(0xffffffffu, odd)) {
+            *met_odd = 1;
+            __threadfence_block();                                          // whoever finds zeros finds this
+            unseen([&](uint32_t at) {
+              uint4 u = lds128(at);
+              if (without_odd<T>(u)) sts128(at, u);
+            });
+            fence_proxy_async();                                            // before the stage's next copy
+            __syncwarp();
+          }
+        }
+      }
       // ---- scores: keys pi(g) and pi(g) + 8 of every 16, rows 2 t and 2 t + 1 --------------------------------------------------
       // one run of keys and rows: its products in two sums, each half as long a chain
       constexpr int CHAINS = GROUPS * NR == 1 ? 2 : 1;
@@ -579,8 +657,6 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
         for (int e = 0; e < 4; ++e) s[0][0][e] += s_odd[0][e];
       }
       // ---- running maxima --------------------------------------------------------------------------------------------------
-      const int key0 = tile * KEYS;
-      const bool masked = tile < clear0 || tile >= clear1;
       float mx[NR][2], mt[NR][2], lv[GROUPS];
 #pragma unroll
       for (int r = 0; r < NR; ++r) mx[r][0] = mx[r][1] = mt[r][0] = mt[r][1] = -INFINITY;
@@ -642,7 +718,6 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
             }
           }
       }
-      bool odd = false;                                                     // values that are not finite in a tile that not all rows see
       // ---- probabilities, turned so that a lane holds row g's keys 2 t and 2 t + 1, and their product with the values ----------------
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
@@ -697,10 +772,6 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
               if (2 * t + 8 >= left) zs = make_uint4(0u, 0u, 0u, 0u);
               if (((2 * t + 1) ^ 4) + 8 >= left) us = make_uint4(0u, 0u, 0u, 0u);
             }
-            if constexpr (!F8) {
-              // ... and no more may a value behind a row's own position, or before its window
-              if (masked) odd |= without_odd<T>(xs) | without_odd<T>(ys) | without_odd<T>(zs) | without_odd<T>(us);
-            }
             const uint32_t x[4] = {xs.x, xs.y, xs.z, xs.w}, y[4] = {ys.x, ys.y, ys.z, ys.w}, z[4] = {zs.x, zs.y, zs.z, zs.w}, u[4] = {us.x, us.y, us.z, us.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -712,30 +783,6 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
               }
             }
           }
-        }
-      }
-      if constexpr (!F8) {
-        // values that are not finite, to the rows that see them: a lane has eight channels of a box
-        if (__any_sync(0xffffffffu, odd)) {
-          for (int key = 0; key < min(KEYS, sh.s.len - key0); ++key)
-#pragma unroll
-            for (int c = 0; c < TL::kBoxes; ++c) {
-              const uint4 u = lds128(TL::at(vb, key, 8 * c + g));
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 f = Num<T>::two(w[i]);
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    const int p = pos[r][e];
-                    if (key0 + key > p || (a.window > 0 && key0 + key <= p - a.window)) continue;
-                    if (low_odd<T>(w[i])) o[4 * c + i][r][e] += f.x;
-                    if (high_odd<T>(w[i])) o[4 * c + i][r][2 + e] += f.y;
-                  }
-              }
-            }
         }
       }
       __syncwarp();
@@ -841,6 +888,10 @@ __global__ void __launch_bounds__(Form<F8, D, ROWS, NR>::kBound, Form<F8, D, ROW
     first_piece = false;
   }
   if (tid == 0 && !a.whole) *reinterpret_cast<PartHead*>(a.part + blockIdx.x * 8LL) = head;
+  if constexpr (!F8) {
+    __syncthreads();
+    if (*met_odd != 0) add_odd<T, D, ROWS, KEYS>(a);
+  }
 }
 
 // Joins the pieces of the item that begins in share blockIdx.x and goes on in the next ones; row by row over blockIdx.y, a lane for 4 channels, the pieces dealt
