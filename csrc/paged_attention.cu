@@ -18,7 +18,9 @@
 //
 // e4m3 becomes f16 two codes at a time (64 lanes a clock an SM, as the byte permutes that pair the values' rows; done by masks and shifts it took three operations
 // and bound the kernel).  Queries in bf16 are scaled by a power of two for each row into f16's range.  With M = max (s + log2 v_scale) beside m, the probabilities
-// times the page's value scale stay within f16 whatever the scales: 2^(s + log2 v_scale - M), and the result is taken times 2^(M - m) / l.
+// times the page's value scale stay below f16's upper end whatever the scales: 2^(s + log2 v_scale - M), and the result is taken times 2^(M - m) / l.  At the lower end
+// they keep all their bits down to 2^-22 of a row's largest such product and are nothing below 2^-33: beside a page with a scale some million times another's, that
+// one's values lose bits in every channel.
 //
 // Work is cut into equal shares of tiles, one for each resident CTA, whatever the lengths: a share may begin and end inside a (sequence, head).  Such pieces go to
 // a workspace of the call, and a second launch joins them in the order of the keys.
