@@ -837,3 +837,19 @@ def test_values_in_8_bits_beyond_the_types_end(monkeypatch, way):
     b.store.v_scale[page, 1] = 2.0 ** 120
     out = paged_attention(b.q, b.store, *b.args)
     assert torch.equal(out[:188], want[:188]) and torch.equal(out[:, :2], want[:, :2]) and bool((out[193:, 2:, 7] > 1e30).all())
+
+
+def test_gradients_of_norm_weights_and_rotations_are_refused():
+    """A model's own parameters among them: the result would leave them without a gradient, and the CPU path would write a graph into the pages."""
+    b = small()
+    table, lens, _ = b.args
+    need = lambda t: t.clone().requires_grad_(True)
+    w, t = torch.ones(64, dtype=torch.bfloat16), turns(30, 16, "cpu")
+    calls = (dict(k_weight=need(w)), dict(q=b.q, q_weight=need(w)), dict(cos=need(t["cos"]), sin=t["sin"]), dict(cos=t["cos"], sin=need(t["sin"])))
+    for kw in calls:
+        with pytest.raises(ValueError, match="no gradient"):
+            paged_append(b.store, b.k, b.v, table, lens, **kw)
+    with torch.no_grad():
+        for kw in calls:
+            paged_append(b.store, b.k, b.v, table, lens, **kw)
+    assert not b.store.k.requires_grad

@@ -243,7 +243,7 @@ def paged_append(store: PagedStore, k: torch.Tensor, v: torch.Tensor, table: tor
     for w in (q_weight, k_weight):
         if w is not None and (w.shape != (D,) or w.dtype != dtype or w.get_device() != dev):
             raise ValueError(f"paged_append: norm weights are {dtype} [{D}] beside the pages")
-    if (k.requires_grad or v.requires_grad or q is not None and q.requires_grad) and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, cos, sin, q_weight, k_weight)):
         raise ValueError("paged_append: serves inference and has no gradient")
     if dev < 0:
         return _append_ref(store, k, v, table, lengths, starts, q, cos, sin, q_weight, k_weight, eps, one_plus_w)
