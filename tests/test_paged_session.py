@@ -139,3 +139,28 @@ def test_drawn_rows_with_nothing_to_choose_from():
     logits[1] = float("nan")
     logits[2, 7] = 0.0
     assert sample_from_logits(logits, SamplingStrategy.drawn(0.8, 20, 0.9)).tolist() == [0, 0, 7]
+
+
+def test_a_step_takes_a_token_for_every_sequence():
+    """Fewer or more are refused before anything is counted (a captured step would hand one token to all)."""
+    lm = Q.Qwen3ForCausalLM.init(tiny())
+    s = Q.PagedQwen3Session(lm, 3, 24, page=4, cache=torch.float32)
+    s.extend(PROMPTS)
+    before = (list(s.held), list(s.free), s.lengths.tolist())
+    for n in (1, 2, 4):
+        with pytest.raises(ValueError):
+            s.step(torch.zeros(n, dtype=torch.long))
+        assert before == (s.held, s.free, s.lengths.tolist())
+    out = s.step(torch.tensor([[3], [4], [6]]))
+    assert torch.allclose(out[1], lm.forward(torch.tensor([PROMPTS[1] + [4]]))[0, -1], atol=1e-4)
+
+
+@pytest.mark.gpu
+def test_a_captured_step_refuses_other_numbers_of_tokens():
+    cfg = tiny(vocab_size=500, hidden_size=256, intermediate_size=512, num_attention_heads=6, half_head_dim=64)
+    s = Q.PagedQwen3Session(Q.Qwen3ForCausalLM.init(cfg, device="cuda", dtype=torch.bfloat16, seed=3), 3, 128, page=32)
+    s.extend([[1, 2, 3], [4], [5, 6]])
+    s.step(torch.tensor([7, 8, 9], device="cuda"))
+    with pytest.raises(ValueError):
+        s.step(torch.tensor([7], device="cuda"))
+    assert s.held == [4, 2, 3] and s.lengths.tolist() == s.held

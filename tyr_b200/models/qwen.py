@@ -376,9 +376,11 @@ class PagedQwen3Session:
     @torch.no_grad()
     def step(self, tok: torch.Tensor) -> torch.Tensor:
         """One token for every sequence that holds any -> logits [sequences, V] (rows of the others mean nothing)."""
+        tok = tok.reshape(-1)
+        if tok.shape[0] != len(self.held):
+            raise ValueError(f"a session of {len(self.held)} sequences takes that many tokens, got {tok.shape[0]}")
         self._room([int(h > 0) for h in self.held])
         self.held = [h + (h > 0) for h in self.held]
-        tok = tok.reshape(-1)
         if not self.table.is_cuda or os.environ.get("TYR_DECODE_GRAPH", "1") == "0":
             return self._device_step(tok)
         if self._graph is None:
