@@ -164,3 +164,11 @@ def test_a_captured_step_refuses_other_numbers_of_tokens():
     with pytest.raises(ValueError):
         s.step(torch.tensor([7], device="cuda"))
     assert s.held == [4, 2, 3] and s.lengths.tolist() == s.held
+
+
+@pytest.mark.gpu
+def test_gpu_draws_from_models_in_64_bits():
+    logits = torch.randn(4, 300, dtype=torch.float64, generator=torch.Generator().manual_seed(1)).cuda()
+    strategy, gen = SamplingStrategy.drawn(0.8, 20, 0.9, 0.05), torch.Generator("cuda")
+    got = sample_from_logits(logits, strategy, gen.manual_seed(4))
+    assert torch.equal(got, sample_from_logits(logits.float(), strategy, gen.manual_seed(4)))

@@ -58,6 +58,8 @@ def sample_from_logits(logits: torch.Tensor, strategy: SamplingStrategy, generat
     if strategy.kind == "greedy":
         return torch.argmax(logits, dim=-1)
     if strategy.kind == "drawn":
+        if logits.is_cuda and logits.dtype == torch.float64:      # a model in 64 bits: as the other strategies take its logits
+            logits = logits.float()
         draws = torch.rand(logits.shape[0], device=logits.device, generator=generator)
         token = sample(logits, draws, temperature=strategy.temperature, top_k=strategy.top_k, top_p=strategy.top_p, min_p=strategy.min_p)
         return token.clamp_(min=0)              # a row with nothing to choose from: what the greedy choice gives, and an index that an embedding can take
