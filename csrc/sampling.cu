@@ -11,9 +11,10 @@
 // are cut by their indices alone.  What top-k leaves of up to 1024 is listed whole, and one CTA cuts and draws among it, by bins of whole-number weights; for small k
 // the k-th largest of the threads' maxima, which bounds the k-th logit from below, saves the counts over all.  Compiled without fast math.
 //
-// Bound: neither memory nor arithmetic but the chain of some ten steps in which a row's CTAs wait for one another, and by mass the counts (atomics in shared memory,
-// 5 us for 16384 logits) and the weights in 64 bits (8 to 11 us; the units for 64 bits are half busy).  1 row of 151936, top-k 50 and top-p: 12 us, 9 of
-// them the host's; 33 rows of 248320 in bf16, settings of all kinds: 55; 256 of 50304 in fp32, no filter: 39; 128 of 262144 by mass: 280.
+// Bound: no pipe, but latencies in the chain of some ten steps in which a row's CTAs wait for one another, the longest by mass the counts (atomics in shared memory, 5 us for
+// 16384 logits) and the weights (8 to 11 us).  128 rows of 262144 by mass: 272 us, issue slots 56 % used, the pipe for 64 bits 13 %, memory 18 %; warps wait for fixed
+// latencies, loads from L2 and barriers.  256 of 50304 in fp32, no filter: 39 us, 52, 28 and 14 %.  33 rows of 248320 in bf16, settings of all kinds: 58; 1 row of 151936,
+// top-k 50 and top-p: 12, 9 of them the host's.
 #include <cooperative_groups.h>
 
 #include <type_traits>

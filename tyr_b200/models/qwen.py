@@ -401,7 +401,8 @@ class PagedQwen3Session:
 @torch.no_grad()
 def generate_paged(lm: Qwen3ForCausalLM, prompts: Sequence[Sequence[int]], max_new_tokens: int = 64, strategy: SamplingStrategy = SamplingStrategy(), eos_token_ids=None,
                    on_step=None, *, generator: Optional[torch.Generator] = None, **session) -> List[List[int]]:
-    """New tokens of every prompt, up to the first end of text (kept) each; prompts need no padding (options of :class:`PagedQwen3Session`)."""
+    """New tokens of every prompt, up to the first end of text (kept) each; prompts need no padding.  ``session``: options of :class:`PagedQwen3Session`, whose pages are
+    e4m3 unless ``cache`` names the model's type."""
     eos = set(lm.cfg.eos_token_ids if eos_token_ids is None else eos_token_ids)
     if not prompts or not all(prompts):
         raise ValueError("generate requires non-empty prompt sequence")

@@ -4,7 +4,7 @@ attention over the pages (csrc/paged_attention.cu).
 Pages ``[pages, kv heads, page, head size]`` hold ``page`` tokens each, in 16 bits or as e4m3 codes in units of a scale for each (page, head).  Sequence ``b`` has
 ``lengths[b]`` tokens, the new ones among them, at ``table[b, position // page]``; its new tokens are rows ``starts[b] .. starts[b + 1] - 1`` of the operands and its
 last positions.  Without ``starts`` every sequence has one row, and none where its length is 0.  Lengths, starts and table live on the device: a step has no shapes
-that depend on them and can be replayed from a CUDA graph.  A page that is written belongs to one sequence; full pages may be shared.
+that depend on them and can be replayed from a CUDA graph.  A page that is written belongs to one sequence and stands in its row of the table once; full pages may be shared.
 
 On the GPU, operands that do not go together (a page outside the cache, a length beyond the table or the rotation) are left out and recorded
 (:func:`tyr_b200.ops._common.raise_on_device_error`): nothing is written, the rows of a sequence that is left out are zeros, and those that would see a page outside the
@@ -30,7 +30,8 @@ PAGE_SIZES = (16, 32, 64, 128)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 # capacity up to which the keys of a (sequence, head) are not cut into pieces
 WHOLE_MAX_KEYS = 256
-# tiles of 16 keys that a share of the work has at least: two for each warp
+# runs of 16 keys of the table's capacity for each share of the work, while there are not more shares than the device holds CTAs at once (a sequence shorter than
+# its row of the table leaves its shares less)
 LEAST_TILES = 8
 
 
@@ -51,7 +52,8 @@ _ATTEND = struct.Struct("@11Q3q10ifi0q")
 
 
 class PagedStore:
-    """The pages of one layer: ``k`` and ``v`` [pages, kv heads, page, head size] in e4m3, bf16 or fp16, and the scales [pages, kv heads] of e4m3 pages."""
+    """The pages of one layer: ``k`` and ``v`` [pages, kv heads, page, head size] in e4m3, bf16 or fp16, and the scales [pages, kv heads] of e4m3 pages:
+    powers of two, as :func:`paged_append` writes them (others may be rounded to the queries' type together with their codes)."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "shape", "index")
 
@@ -328,7 +330,9 @@ def _attend_ref(q, store, table, lengths, starts, window, scale):
 def paged_attention(q: torch.Tensor, store: PagedStore, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
                     window: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
     """Attention of the new tokens' queries ``[rows, heads, D]`` over their sequences' pages, which hold the new tokens already -> ``[rows, heads, D]``; rows of no
-    sequence, and of one that is left out, come back as zeros.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
+    sequence, and of one that is left out, come back as zeros.  Scores and sums are held in 32 bits, a probability is rounded once: to the pages' 16-bit type, to f16 beside
+    e4m3, or to the queries' type where many new tokens take the kernel on tcgen05 (:func:`gathers`).  Values that are not finite show in their channel at the rows that see
+    them.  A token sees the positions up to its own, the last ``window`` of them when given; query heads share K/V heads in groups."""
     pages, G, P, D = store.shape
     shape = q.shape
     if len(shape) != 3 or shape[0] == 0 or shape[2] != D or shape[1] == 0 or shape[1] % G or q.get_device() != store.index:
